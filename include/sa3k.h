@@ -421,6 +421,35 @@ SA3K_API int sa3k_diff_attn_bwd(sa3k_ctx* ctx, const void* q1, const void* k1, c
                                 void* scratch_dOh, float* scratch_dn, float* dq1, float* dk1, float* dq2, float* dk2,
                                 float* dv);
 
+/* ---------------------------------------------------------------- layer operators */
+
+/* The parts of a transformer layer of another make than the DiT's block, next to the adapted linears:
+ * layer norm, attention with a sliding window, and products with an epilogue. No reference counterpart.
+ * Tensors are device memory; a tensor's elements are of `type`, its sums and statistics f32. Rows are
+ * `ld` elements apart (ld >= the row's length) and may start at any element. Calls with nothing to
+ * compute (no rows, no samples) return SA3K_OK and launch nothing that they need not. The calls switch
+ * the thread's HIP device to the context's and back. */
+
+/* Layer norm of rows [rows][cols] (cols <= 16384), type f32, f16 or bf16, optionally of the sum with a
+ * residual:
+ *   s = x + residual, rounded to `type` (residual null: s = x), stored to sum when that is not null;
+ *   mean = sum_c s / cols, rstd = 1 / sqrt(sum_c (s - mean)^2 / cols + eps)      (f32, nullable outputs [rows])
+ *   y = (s - mean) rstd gamma + beta            (gamma null: 1, beta null: 0; f32 [cols])
+ * y or sum may be x or residual itself (same pitch). */
+SA3K_API int sa3k_layer_norm_fwd(sa3k_ctx* ctx, int type, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                 int64_t rows, int64_t cols, const float* gamma, const float* beta, float eps, void* sum,
+                                 int64_t ldsum, void* y, int64_t ldy, float* mean, float* rstd);
+
+/* Its backward, x being the forward's s, mean and rstd its outputs: with xh = (x - mean) rstd, h = dy gamma,
+ *   dx = rstd (h - mean_c h - xh mean_c(h xh)) [+ dsum]    (dsum nullable: the gradient that reaches s itself)
+ *   dgamma = sum_rows dy xh, dbeta = sum_rows dy           (f32 [cols], nullable; added to with accumulate = 1)
+ * in a fixed order of summation. dx may be dy, x or dsum itself (same pitch). dx is the gradient of the
+ * residual too. */
+SA3K_API int sa3k_layer_norm_bwd(sa3k_ctx* ctx, int type, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                 const void* dsum, int64_t lddsum, int64_t rows, int64_t cols, const float* gamma,
+                                 const float* mean, const float* rstd, void* dx, int64_t lddx, float* dgamma,
+                                 float* dbeta, int accumulate);
+
 /* ---------------------------------------------------------------- C3: one DiT block */
 
 /* Shape of a (differential) DiT block, the DitConfig fields dit_block reads (src/dit.h:20-46). */

@@ -120,6 +120,8 @@ def _declare(lib):
         "sa3k_lora_chain_constants": (I, [P, P, P, P, C.POINTER(I)]),
         "sa3k_diff_attn_fwd": (I, [P, P, P, P, P, P, I, I, I, I, I, I, F, P, P, P, P, P]),
         "sa3k_diff_attn_bwd": (I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, P, P, P, P, P, P, P]),
+        "sa3k_layer_norm_fwd": (I, [P, I, P, I64, P, I64, I64, I64, P, P, F, P, I64, P, I64, P, P]),
+        "sa3k_layer_norm_bwd": (I, [P, I, P, I64, P, I64, P, I64, I64, I64, P, P, P, P, I64, P, P, I]),
         "sa3k_block_create": (I, [P, C.POINTER(BlockConfig), C.POINTER(BlockWeights), I, I64, I64, C.POINTER(P)]),
         "sa3k_block_destroy": (I, [P, P]),
         "sa3k_block_base_norm_sq": (I, [P, P, I, C.POINTER(P)]),
@@ -644,3 +646,26 @@ def attn_bwd(ctx, q1, k1, q2, k2, v, o1, o2, l1, l2, dO, B, H, Sq, Sk, window=0,
                                          dO.ptr, B, H, Sq, Sk, 64, window, scale, dOh.ptr, dn.ptr, g["dq1"].ptr,
                                          g["dk1"].ptr, g["dq2"].ptr, g["dk2"].ptr, g["dv"].ptr))
     return g
+
+
+def _p(a):
+    return a.ptr if a is not None else None
+
+
+def layer_norm_fwd(ctx, type, x, rows, cols, gamma, beta, eps, y, mean=None, rstd=None, residual=None, sum=None,
+                   ldx=None, ldr=None, ldsum=None, ldy=None):
+    """y = layer norm of x (+ residual, the sum stored to `sum`); every argument with a `.ptr`, pitches in
+    elements (None: cols)"""
+    ctx.check(ctx.lib.sa3k_layer_norm_fwd(ctx.h, type, _p(x), cols if ldx is None else ldx, _p(residual),
+                                          cols if ldr is None else ldr, rows, cols, _p(gamma), _p(beta), eps, _p(sum),
+                                          cols if ldsum is None else ldsum, _p(y), cols if ldy is None else ldy, _p(mean),
+                                          _p(rstd)))
+
+
+def layer_norm_bwd(ctx, type, dy, x, rows, cols, gamma, mean, rstd, dx, dsum=None, dgamma=None, dbeta=None,
+                   accumulate=False, lddy=None, ldx=None, lddsum=None, lddx=None):
+    """dx (+ dsum), dgamma and dbeta of layer_norm_fwd; x is the forward's sum"""
+    ctx.check(ctx.lib.sa3k_layer_norm_bwd(ctx.h, type, _p(dy), cols if lddy is None else lddy, _p(x),
+                                          cols if ldx is None else ldx, _p(dsum), cols if lddsum is None else lddsum, rows,
+                                          cols, _p(gamma), _p(mean), _p(rstd), _p(dx), cols if lddx is None else lddx,
+                                          _p(dgamma), _p(dbeta), int(accumulate)))
