@@ -450,6 +450,44 @@ SA3K_API int sa3k_layer_norm_bwd(sa3k_ctx* ctx, int type, const void* dy, int64_
                                  const float* mean, const float* rstd, void* dx, int64_t lddx, float* dgamma,
                                  float* dbeta, int accumulate);
 
+/* Softmax attention with a sliding window and first tokens that stay visible, for grouped heads: query head h
+ * reads key/value head h / (heads / kv_heads). */
+typedef struct {
+    int type;                   /* SA3K_TYPE_BF16 or SA3K_TYPE_F16, of every tensor */
+    int batch, heads, kv_heads; /* heads a multiple of kv_heads */
+    int head_dim;               /* 64 or 128 */
+    int q_tokens, k_tokens;     /* the most a sample has */
+    int left, right;            /* the window: keys p - left .. p + right of a query at position p; negative: no bound */
+    int sinks;                  /* the first tokens, visible at any distance */
+    int causal;                 /* 1: no query sees a key past its own position (`right` and the sinks' reach end there) */
+    float scale;                /* of the scores, > 0 */
+    /* distances in elements between samples, tokens and heads; a head's elements lie together. Multiples of 8;
+     * tokens less than 2^24 and, with more than one token, at least head_dim apart. Inputs may repeat (0) over
+     * samples and heads. o's hold for dO, and q's, k's and v's for dq, dk and dv. */
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+} sa3k_window_attn;
+
+/* Sample b has q_len[b] queries and k_len[b] keys (device int32 [batch], null: q_tokens, k_tokens; values out of
+ * range are clamped). Its queries are the last of its keys' positions: query i is at p = i + k_len[b] - q_len[b].
+ * It sees key j when j < k_len[b], (causal: j <= p), and j < sinks or p - left <= j <= p + right:
+ *   o = sum_j softmax_j(scale q . k_j) v_j,  lse = log2 sum_j 2^(scale log2(e) q . k_j)
+ * A query that sees no key gets o = 0 and lse = -inf. o and lse (f32 [batch][heads][q_tokens], nullable) of rows
+ * past q_len stay as they were; keys, values, queries and gradients past a sample's lengths are never read. Weights
+ * are rounded to `type` for the product with v, everything else is f32. Few queries (at most 32) over many
+ * keys run with the keys split over workgroups, whose sums are joined in a fixed order. Tensors 16-byte aligned. */
+SA3K_API int sa3k_window_attn_fwd(sa3k_ctx* ctx, const sa3k_window_attn* d, const void* q, const void* k, const void* v,
+                                  const int32_t* q_len, const int32_t* k_len, void* o, float* lse);
+
+/* Its backward from dO and the forward's o and lse: with p_ij = 2^(scale log2(e) q_i . k_j - lse_i) and
+ * ds_ij = p_ij (dO_i . v_j - dO_i . o_i),
+ *   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij dO_i,
+ * the sums of dk and dv also over the query heads of their group. Written, not added to, in a fixed order of
+ * summation; rows past a sample's lengths stay as they were. p and ds are rounded to `type` for these products
+ * (f16: gradients smaller than about 2^-24 a pair are lost, as in any f16 backward without loss scaling). */
+SA3K_API int sa3k_window_attn_bwd(sa3k_ctx* ctx, const sa3k_window_attn* d, const void* q, const void* k, const void* v,
+                                  const void* o, const float* lse, const void* dO, const int32_t* q_len,
+                                  const int32_t* k_len, void* dq, void* dk, void* dv);
+
 /* ---------------------------------------------------------------- C3: one DiT block */
 
 /* Shape of a (differential) DiT block, the DitConfig fields dit_block reads (src/dit.h:20-46). */

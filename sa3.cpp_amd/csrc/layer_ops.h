@@ -8,6 +8,12 @@
 
 #include "sa3k.h"
 
+#ifdef __HIPCC__
+#define SA3K_HD __host__ __device__ inline
+#else
+#define SA3K_HD inline
+#endif
+
 namespace sa3k {
 
 constexpr int64_t kMaxExtent = (int64_t)1 << 31;   // rows, columns and pitches stay below this
@@ -65,6 +71,228 @@ inline const char* norm_check(const NormArgs& a, bool bwd, int* code) {
         if (!a.x || !a.dy || !a.y || !a.mean || !a.rstd) return "dy, x, mean, rstd and dx must not be null";
     }
     return nullptr;
+}
+
+// ------------------------------------------------------------------------------------- attention
+constexpr int kFar = 1 << 29;           // no bound: further than any two positions (k_tokens, q_tokens < 2^28)
+constexpr int kMaxTokens = 1 << 28;
+constexpr int64_t kMaxTokenStride = (int64_t)1 << 24;   // 64 rows of it in bytes stay below 2^31
+constexpr int64_t kMaxStride = (int64_t)1 << 40;
+
+// an output's rows must not overlap: by growing stride, each step passes everything below it
+inline bool rows_apart(const int64_t* st, const int64_t* n, int64_t row) {
+    if (n[0] == 0 || n[1] == 0 || n[2] == 0) return true;
+    int order[3] = {0, 1, 2};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (st[order[j]] < st[order[i]]) { const int t = order[i]; order[i] = order[j]; order[j] = t; }
+    int64_t reach = row;
+    for (int i = 0; i < 3; ++i) {
+        const int d = order[i];
+        if (n[d] <= 1) continue;
+        if (st[d] < reach) return false;
+        reach += st[d] * (n[d] - 1);
+    }
+    return true;
+}
+
+struct AttnPtrs {
+    const void *q = nullptr, *k = nullptr, *v = nullptr, *o = nullptr, *dO = nullptr;
+    const void *lse = nullptr, *q_len = nullptr, *k_len = nullptr, *dq = nullptr, *dk = nullptr, *dv = nullptr;
+};
+
+inline const char* attn_check(const sa3k_window_attn* d, const AttnPtrs& p, bool bwd, int* code) {
+    *code = SA3K_ERR_INVALID;
+    if (!d) return "null shape";
+    if (d->type != SA3K_TYPE_BF16 && d->type != SA3K_TYPE_F16) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "type must be bf16 or f16";
+    }
+    if (d->head_dim != 64 && d->head_dim != 128) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "head_dim must be 64 or 128";
+    }
+    if (d->batch < 0 || d->batch > 65535 || d->heads <= 0 || d->heads > 65535) return "batch or heads out of range";
+    if (d->kv_heads <= 0 || d->heads % d->kv_heads != 0) return "heads must be a multiple of kv_heads";
+    if (d->q_tokens < 0 || d->q_tokens >= kMaxTokens || d->k_tokens < 0 || d->k_tokens >= kMaxTokens)
+        return "q_tokens or k_tokens out of range";
+    if (d->sinks < 0) return "sinks must not be negative";
+    if (d->causal != 0 && d->causal != 1) return "causal must be 0 or 1";
+    if (!(d->scale > 0.f && d->scale <= 1.0e30f)) return "scale must be positive and finite";
+    const int64_t nq[3] = {d->batch, d->q_tokens, d->heads}, nk[3] = {d->batch, d->k_tokens, d->kv_heads};
+    const int64_t* st[4] = {d->q_stride, d->k_stride, d->v_stride, d->o_stride};
+    for (int t = 0; t < 4; ++t)
+        for (int i = 0; i < 3; ++i) {
+            const int64_t v = st[t][i];
+            const int64_t n = (t == 1 || t == 2 ? nk : nq)[i];
+            if (n <= 1) continue;   // never used
+            if (v < 0 || v >= kMaxStride || v % 8 != 0) return "strides must be multiples of 8, not negative";
+            if (i == 1 && (v < d->head_dim || v >= kMaxTokenStride))
+                return "tokens must be at least head_dim and less than 2^24 elements apart";
+        }
+    if (!rows_apart(d->o_stride, nq, d->head_dim)) return "the rows of o overlap";
+    if (bwd && (!rows_apart(d->q_stride, nq, d->head_dim) || !rows_apart(d->k_stride, nk, d->head_dim) ||
+                !rows_apart(d->v_stride, nk, d->head_dim)))
+        return "the rows of q, k or v overlap, and their gradients have the same layout";
+    // workgroups of 256 threads, 64 rows or keys each at the least, in one grid dimension
+    const int64_t most = (d->q_tokens > d->k_tokens ? d->q_tokens : d->k_tokens) / 64 + 1;
+    if (most * d->batch * d->heads >= ((int64_t)1 << 23)) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "batch x heads x tokens is too large for one launch";
+    }
+    if (!elem_aligned(p.q_len, 4) || !elem_aligned(p.k_len, 4) || !elem_aligned(p.lse, 4))
+        return "lengths and lse must be 4-byte aligned";
+    const void* t[8] = {p.q, p.k, p.v, p.o, p.dO, p.dq, p.dk, p.dv};
+    for (const void* x : t)
+        if (!elem_aligned(x, 16)) return "tensors must be 16-byte aligned";
+    if (d->batch == 0) return nullptr;
+    if (d->q_tokens > 0) {
+        if (!p.q || !p.o) return "q and o must not be null";
+        if (bwd && (!p.dO || !p.lse || !p.dq)) return "lse, dO and dq must not be null";
+    }
+    if (d->k_tokens > 0) {
+        if (!p.k || !p.v) return "k and v must not be null";
+        if (bwd && (!p.dk || !p.dv)) return "dk and dv must not be null";
+    }
+    return nullptr;
+}
+
+// The kernels' view of the shape: bounds resolved, lengths in range, strides of single tokens made valid.
+struct AttnShape {
+    int B, H, K, G, D, Sq, Sk, left, right, sinks, causal;
+    float scale;
+    int64_t qs[3], ks[3], vs[3], os[3];
+    const int32_t *q_len, *k_len;
+};
+
+inline AttnShape attn_shape(const sa3k_window_attn& d, const void* q_len, const void* k_len) {
+    AttnShape a;
+    a.B = d.batch; a.H = d.heads; a.K = d.kv_heads; a.G = d.heads / d.kv_heads; a.D = d.head_dim;
+    a.Sq = d.q_tokens; a.Sk = d.k_tokens;
+    a.left = d.left < 0 || d.left > kFar ? kFar : d.left;
+    a.right = d.causal ? 0 : d.right < 0 || d.right > kFar ? kFar : d.right;
+    a.sinks = d.sinks < d.k_tokens ? d.sinks : d.k_tokens;
+    a.causal = d.causal;
+    a.scale = d.scale;
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = d.q_stride[i];
+        a.ks[i] = d.k_stride[i];
+        a.vs[i] = d.v_stride[i];
+        a.os[i] = d.o_stride[i];
+    }
+    if (a.Sq <= 1) a.qs[1] = a.os[1] = a.D;
+    if (a.Sk <= 1) a.ks[1] = a.vs[1] = a.D;
+    a.q_len = static_cast<const int32_t*>(q_len);
+    a.k_len = static_cast<const int32_t*>(k_len);
+    return a;
+}
+
+// The keys a query at position p of a sample with nk keys sees: lo .. lo + n - 1, and 0 .. first - 1.
+struct Seen {
+    int lo, n, first;
+};
+SA3K_HD Seen seen_by(int p, int nk, int left, int right, int sinks, int causal) {
+    const int last = causal && p < nk - 1 ? p : nk - 1;
+    const int lo = p - left > 0 ? p - left : 0;
+    const int top = p + right < last ? p + right : last;
+    Seen s;
+    s.lo = lo;
+    s.n = top >= lo ? top - lo + 1 : 0;
+    s.first = sinks < last + 1 ? sinks : last + 1;
+    if (s.first < 0) s.first = 0;
+    return s;
+}
+// The blocks of `blk` keys that the queries of positions pa .. pb see, in order: `head` blocks from 0, then
+// those from `from` on, `count` in all.
+struct KeyBlocks {
+    int head, from, count;
+};
+SA3K_HD KeyBlocks key_blocks(int pa, int pb, int nk, int left, int right, int sinks, int causal, int blk) {
+    const Seen a = seen_by(pa, nk, left, right, sinks, causal), b = seen_by(pb, nk, left, right, sinks, causal);
+    const int ns = (b.first + blk - 1) / blk;          // a later query sees no fewer first tokens
+    const int top = b.lo + b.n - 1;                    // nor a lower last key
+    KeyBlocks r;
+    if (b.n == 0 || top < a.lo) {
+        r.head = ns;
+        r.from = ns;
+        r.count = ns;
+        return r;
+    }
+    const int wl = a.lo / blk, wh = top / blk + 1;
+    r.head = ns < wl ? ns : wl;
+    r.from = wl;
+    r.count = r.head + (wh > ns ? wh : ns) - wl;
+    return r;
+}
+SA3K_HD int key_block(const KeyBlocks& r, int i) { return i < r.head ? i : r.from + (i - r.head); }
+
+
+// Few queries: at most this many run with the keys split over workgroups.
+constexpr int kFewQueries = 32;
+// The split count for `chunks` chunks of 32 rows a key/value head: about two workgroups a CU in all, at least two
+// blocks of 32 keys a wave.
+inline int attn_splits(const AttnShape& s, int chunks) {
+    const int64_t reach = (int64_t)s.left + s.right + s.Sq + 32;   // keys that a sample's queries see at the most
+    const int64_t keys = (reach < s.Sk ? reach : s.Sk) + s.sinks;
+    const int64_t base = (int64_t)s.B * s.K * chunks, most = keys / (32 * 4 * 2);
+    int64_t n = 512 / (base > 0 ? base : 1);
+    if (n > most) n = most;
+    return n < 1 ? 1 : (int)n;
+}
+
+// The dK/dV pass: a workgroup takes a tile of 128 keys and a share of the (query head, block of 64 queries) pairs that
+// see it. Tiles with first tokens, which every later query sees, get `first` shares, the others `rest`, so that no
+// workgroup runs much longer than the ordinary ones and there are about two workgroups a CU where the work allows.
+constexpr int kKeyTile = 128;
+struct KeySplit {
+    int tiles, first_tiles, first, rest;   // first_tiles of the tiles hold first tokens
+    SA3K_HD int items() const { return first_tiles * first + (tiles - first_tiles) * rest; }   // workgroups a k/v head
+};
+inline KeySplit key_split(const AttnShape& s) {
+    KeySplit r;
+    r.tiles = (s.Sk + kKeyTile - 1) / kKeyTile;
+    r.first_tiles = (s.sinks + kKeyTile - 1) / kKeyTile;
+    const int64_t all = (s.Sq + 63) / 64, band = ((int64_t)kKeyTile + s.left + s.right + 62) / 64 + 1;
+    const int64_t most = s.G * (all > 0 ? all : 1), usual = s.G * (band < all ? band : (all > 0 ? all : 1));
+    const int64_t base = (int64_t)s.B * s.K * (r.tiles > 0 ? r.tiles : 1);
+    int64_t n = (512 + base / 2) / base;
+    if (n > usual / 4) n = usual / 4;   // at least four blocks a workgroup
+    if (n < 1) n = 1;
+    const int64_t len = (usual + n - 1) / n;
+    int64_t f = (most + len - 1) / len;
+    r.rest = (int)n;
+    r.first = (int)(f < n ? n : f > 256 ? 256 : f);
+    return r;
+}
+struct KeyItem {
+    int tile, split, splits;
+};
+SA3K_HD KeyItem key_item(const KeySplit& r, int i) {
+    KeyItem t;
+    const int head = r.first_tiles * r.first;
+    if (i < head) {
+        t.tile = i / r.first;
+        t.split = i - t.tile * r.first;
+        t.splits = r.first;
+    } else {
+        const int j = i - head, q = j / r.rest;
+        t.tile = r.first_tiles + q;
+        t.split = j - q * r.rest;
+        t.splits = r.rest;
+    }
+    return t;
+}
+// The queries (of nq, at positions i + off) that see some key of k0 .. k1: lo .. hi (hi < lo: none).
+struct Span {
+    int lo, hi;
+};
+SA3K_HD Span seen_from(int k0, int k1, int nq, int off, int left, int right, int sinks, int causal) {
+    const bool first = k0 < sinks;
+    const int plo = causal ? k0 : first ? -kFar : k0 - right, phi = first ? kFar : k1 + left;
+    Span r;
+    r.lo = plo - off > 0 ? plo - off : 0;
+    r.hi = phi - off < nq - 1 ? phi - off : nq - 1;
+    return r;
 }
 
 }  // namespace sa3k

@@ -56,6 +56,12 @@ class DitConfig(C.Structure):
                [("local_dim", C.c_int)]
 
 
+class WindowAttnShape(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("type", "batch", "heads", "kv_heads", "head_dim", "q_tokens", "k_tokens", "left",
+                                       "right", "sinks", "causal")] + [("scale", C.c_float)] + \
+               [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride")]
+
+
 class DitTrain(C.Structure):
     _fields_ = [("rank", C.c_int), ("alpha", C.c_float), ("dora", C.c_int), ("scope", C.c_int), ("batch", C.c_int),
                 ("frames", C.c_int), ("ctx_tokens", C.c_int), ("recompute", C.c_int)]
@@ -122,6 +128,8 @@ def _declare(lib):
         "sa3k_diff_attn_bwd": (I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, P, P, P, P, P, P, P]),
         "sa3k_layer_norm_fwd": (I, [P, I, P, I64, P, I64, I64, I64, P, P, F, P, I64, P, I64, P, P]),
         "sa3k_layer_norm_bwd": (I, [P, I, P, I64, P, I64, P, I64, I64, I64, P, P, P, P, I64, P, P, I]),
+        "sa3k_window_attn_fwd": (I, [P, C.POINTER(WindowAttnShape), P, P, P, P, P, P, P]),
+        "sa3k_window_attn_bwd": (I, [P, C.POINTER(WindowAttnShape), P, P, P, P, P, P, P, P, P, P, P]),
         "sa3k_block_create": (I, [P, C.POINTER(BlockConfig), C.POINTER(BlockWeights), I, I64, I64, C.POINTER(P)]),
         "sa3k_block_destroy": (I, [P, P]),
         "sa3k_block_base_norm_sq": (I, [P, P, I, C.POINTER(P)]),
@@ -669,3 +677,31 @@ def layer_norm_bwd(ctx, type, dy, x, rows, cols, gamma, mean, rstd, dx, dsum=Non
                                           cols if ldx is None else ldx, _p(dsum), cols if lddsum is None else lddsum, rows,
                                           cols, _p(gamma), _p(mean), _p(rstd), _p(dx), cols if lddx is None else lddx,
                                           _p(dgamma), _p(dbeta), int(accumulate)))
+
+
+class WindowAttn:
+    """Attention of one shape with a sliding window (left / right keys around a query's own; negative: no bound) and
+    `sinks` first tokens that stay visible. Strides: (sample, token, head) in elements; None: [batch][tokens][heads]
+    [head_dim] without gaps."""
+
+    def __init__(self, ctx, type, batch, heads, kv_heads, q_tokens, k_tokens, head_dim, left=-1, right=-1, sinks=0,
+                 causal=False, scale=None, q_strides=None, k_strides=None, v_strides=None, o_strides=None):
+        self.ctx = ctx
+        dense = lambda n, h: (n * h * head_dim, h * head_dim, head_dim)  # noqa: E731
+        st = [s if s is not None else dense(n, h) for s, n, h in
+              ((q_strides, q_tokens, heads), (k_strides, k_tokens, kv_heads), (v_strides, k_tokens, kv_heads),
+               (o_strides, q_tokens, heads))]
+        self.shape = WindowAttnShape(type, batch, heads, kv_heads, head_dim, q_tokens, k_tokens, left, right, sinks,
+                                     int(causal), head_dim ** -0.5 if scale is None else scale,
+                                     *[(C.c_int64 * 3)(*s) for s in st])
+
+    def forward(self, q, k, v, o, lse=None, q_len=None, k_len=None):
+        c = self.ctx
+        c.check(c.lib.sa3k_window_attn_fwd(c.h, C.byref(self.shape), _p(q), _p(k), _p(v), _p(q_len), _p(k_len), _p(o),
+                                           _p(lse)))
+
+    def backward(self, q, k, v, o, lse, dO, dq, dk, dv, q_len=None, k_len=None):
+        """dq, dk and dv lie as q, k and v do, dO as o does"""
+        c = self.ctx
+        c.check(c.lib.sa3k_window_attn_bwd(c.h, C.byref(self.shape), _p(q), _p(k), _p(v), _p(o), _p(lse), _p(dO), _p(q_len),
+                                           _p(k_len), _p(dq), _p(dk), _p(dv)))

@@ -20,4 +20,55 @@ int norm(int type, int64_t rows, int64_t cols, float eps, int accumulate, int bw
     return norm_check(a, bwd != 0, &code) ? code : 0;
 }
 
+// i: type, batch, heads, kv_heads, head_dim, q_tokens, k_tokens, left, right, sinks, causal; st: the 12 strides;
+// p: q, k, v, o, dO, lse, q_len, k_len, dq, dk, dv as addresses
+static sa3k_window_attn shape(const int* i, float scale, const int64_t* st) {
+    sa3k_window_attn d;
+    d.type = i[0]; d.batch = i[1]; d.heads = i[2]; d.kv_heads = i[3]; d.head_dim = i[4]; d.q_tokens = i[5];
+    d.k_tokens = i[6]; d.left = i[7]; d.right = i[8]; d.sinks = i[9]; d.causal = i[10];
+    d.scale = scale;
+    for (int k = 0; k < 3; ++k) {
+        d.q_stride[k] = st[k]; d.k_stride[k] = st[3 + k]; d.v_stride[k] = st[6 + k]; d.o_stride[k] = st[9 + k];
+    }
+    return d;
+}
+int attn(const int* i, float scale, const int64_t* st, const int64_t* p, int bwd) {
+    const sa3k_window_attn d = shape(i, scale, st);
+    AttnPtrs a;
+    const void** f[11] = {&a.q, &a.k, &a.v, &a.o, &a.dO, &a.lse, &a.q_len, &a.k_len, &a.dq, &a.dk, &a.dv};
+    for (int k = 0; k < 11; ++k) *f[k] = at(p[k]);
+    int code = -1;
+    return attn_check(&d, a, bwd != 0, &code) ? code : 0;
+}
+int attn_null() {
+    int code = -1;
+    return attn_check(nullptr, AttnPtrs(), false, &code) ? code : 0;
+}
+// out: lo, n, first
+void seen(int p, int nk, const int* w, int* out) {
+    const Seen s = seen_by(p, nk, w[0], w[1], w[2], w[3]);
+    out[0] = s.lo; out[1] = s.n; out[2] = s.first;
+}
+// the key blocks of positions pa .. pb, at most `most` of them
+int blocks(int pa, int pb, int nk, const int* w, int blk, int* out, int most) {
+    const KeyBlocks k = key_blocks(pa, pb, nk, w[0], w[1], w[2], w[3], blk);
+    for (int i = 0; i < k.count && i < most; ++i) out[i] = key_block(k, i);
+    return k.count;
+}
+void from(int k0, int k1, int nq, int off, const int* w, int* out) {
+    const Span s = seen_from(k0, k1, nq, off, w[0], w[1], w[2], w[3]);
+    out[0] = s.lo; out[1] = s.hi;
+}
+// tile, split and splits of every item of the dK/dV pass; splits of the keys of a few queries
+int items(const int* i, const int64_t* st, int* out, int most, int* few) {
+    const AttnShape a = attn_shape(shape(i, 1.f, st), nullptr, nullptr);
+    const KeySplit k = key_split(a);
+    for (int n = 0; n < k.items() && n < most; ++n) {
+        const KeyItem t = key_item(k, n);
+        out[3 * n] = t.tile; out[3 * n + 1] = t.split; out[3 * n + 2] = t.splits;
+    }
+    *few = attn_splits(a, (a.Sq * a.G + 31) / 32);
+    return k.items();
+}
+
 }  // extern "C"

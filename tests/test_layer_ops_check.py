@@ -2,6 +2,7 @@
 arithmetic: compiled with g++ and checked without a GPU."""
 import ctypes as C
 import os
+import random
 import subprocess
 
 import pytest
@@ -65,3 +66,152 @@ def test_norm_forward_refuses(host, want, change):
 ])
 def test_norm_backward_refuses(host, want, change):
     assert norm(host, bwd=True, **change) == want
+
+
+ATTN_I = ("type", "batch", "heads", "kv_heads", "head_dim", "q_tokens", "k_tokens", "left", "right", "sinks", "causal")
+ATTN_P = ("q", "k", "v", "o", "dO", "lse", "q_len", "k_len", "dq", "dk", "dv")
+
+
+def attn(host, bwd=False, scale=0.125, strides=None, **kw):
+    i = dict(type=sa3k.TYPE_BF16, batch=2, heads=4, kv_heads=2, head_dim=64, q_tokens=10, k_tokens=20, left=3, right=0,
+             sinks=1, causal=0)
+    at = dict(q=64, k=64, v=64, o=64)
+    if bwd:
+        at.update(dO=64, lse=64, dq=64, dk=64, dv=64)
+    for n, v in kw.items():
+        (i if n in i else at)[n] = v
+    D, H, K = i["head_dim"], i["heads"], i["kv_heads"]
+    st = dict(q=(i["q_tokens"] * H * D, H * D, D), k=(i["k_tokens"] * K * D, K * D, D), v=(i["k_tokens"] * K * D, K * D, D),
+              o=(i["q_tokens"] * H * D, H * D, D))
+    st.update(strides or {})
+    host.attn.argtypes = [C.POINTER(C.c_int), C.c_float, C.POINTER(C.c_int64), C.POINTER(C.c_int64), C.c_int]
+    return host.attn((C.c_int * 11)(*[i[n] for n in ATTN_I]), scale,
+                     (C.c_int64 * 12)(*[x for t in "qkvo" for x in st[t]]),
+                     (C.c_int64 * 11)(*[at.get(n, 0) for n in ATTN_P]), int(bwd))
+
+
+def test_attn_accepts(host):
+    assert attn(host) == 0 and attn(host, bwd=True) == 0
+    assert attn(host, batch=0, q=0, k=0, v=0, o=0) == 0
+    assert attn(host, q_tokens=0, q=0, o=0) == 0 and attn(host, bwd=True, q_tokens=0, q=0, o=0, dO=0, lse=0, dq=0) == 0
+    assert attn(host, k_tokens=0, k=0, v=0) == 0
+    assert attn(host, left=-1, right=-1, sinks=1 << 30) == 0
+    assert attn(host, strides=dict(k=(0, 128, 0), v=(0, 64, 0))) == 0           # shared keys, for reading
+    assert attn(host, strides=dict(q=(8, 5120, 64))) == 0                        # samples interleaved, for reading
+    assert attn(host, bwd=True, strides=dict(q=(64 * 10 * 4, 64, 640))) == 0    # head-major
+
+
+@pytest.mark.parametrize("want,change", [
+    (UNSUPPORTED, dict(type=sa3k.TYPE_F32)), (UNSUPPORTED, dict(head_dim=96)), (INVALID, dict(heads=3)),
+    (INVALID, dict(kv_heads=0)), (INVALID, dict(heads=0)), (INVALID, dict(batch=-1)), (INVALID, dict(batch=65536)),
+    (INVALID, dict(q_tokens=-1)), (INVALID, dict(k_tokens=1 << 28)), (INVALID, dict(sinks=-1)), (INVALID, dict(causal=2)),
+    (INVALID, dict(scale=0.0)), (INVALID, dict(scale=-1.0)), (INVALID, dict(scale=float("nan"))),
+    (INVALID, dict(scale=float("inf"))), (INVALID, dict(strides=dict(q=(2560, 260, 64)))),
+    (INVALID, dict(strides=dict(k=(-2560, 128, 64)))), (INVALID, dict(strides=dict(k=(2560, 56, 64)))),
+    (INVALID, dict(strides=dict(v=(2560, 1 << 24, 64)))), (INVALID, dict(strides=dict(k=(1 << 40, 128, 64)))),
+    (INVALID, dict(strides=dict(o=(2560, 256, 0)))), (INVALID, dict(strides=dict(o=(2552, 256, 64)))),
+    (INVALID, dict(q=0)), (INVALID, dict(o=0)), (INVALID, dict(k=0)), (INVALID, dict(v=0)), (INVALID, dict(k=72)),
+    (INVALID, dict(lse=66)), (INVALID, dict(q_len=65)), (INVALID, dict(k_len=2)),
+    (UNSUPPORTED, dict(batch=65535, heads=64, q_tokens=4096)),
+])
+def test_attn_refuses(host, want, change):
+    assert attn(host, **change) == want
+
+
+@pytest.mark.parametrize("change", [
+    dict(dO=0), dict(lse=0), dict(dq=0), dict(dk=0), dict(dv=0), dict(dq=72), dict(strides=dict(k=(0, 128, 64))),
+    dict(strides=dict(v=(2560, 128, 0))), dict(strides=dict(q=(8, 5120, 64))), dict(o=0),
+])
+def test_attn_backward_refuses(host, change):
+    assert attn(host, bwd=True, **change) == INVALID
+
+
+def test_attn_null_shape(host):
+    assert host.attn_null() == INVALID
+
+
+FAR = 1 << 29
+
+
+def sees(p, j, nk, left, right, sinks, causal):
+    """the definition"""
+    return 0 <= j < nk and (not causal or j <= p) and (j < sinks or p - left <= j <= p + right)
+
+
+def windows(r):
+    causal = r.randint(0, 1)
+    return (r.choice([0, 1, 5, 40, 200, FAR]), 0 if causal else r.choice([0, 1, 5, 40, 200, FAR]), r.choice([0, 1, 4, 30, 70]),
+            causal)
+
+
+def test_seen_keys(host):
+    """lo, n and first of a query's keys against the definition"""
+    r = random.Random(1)
+    out = (C.c_int * 3)()
+    for _ in range(400):
+        nk, w = r.randint(0, 90), windows(r)
+        w = w[:2] + (min(w[2], nk),) + w[3:]
+        for p in (r.randint(-20, nk), nk - 1, 0):
+            if p >= nk:
+                continue
+            host.seen(p, nk, (C.c_int * 4)(*w), out)
+            got = {j for j in range(nk) if out[0] <= j < out[0] + out[1] or j < out[2]}
+            assert got == {j for j in range(nk) if sees(p, j, nk, *w)}, (p, nk, w)
+
+
+def test_key_blocks(host):
+    """every block with a visible key, once, in order, and none far from any"""
+    r = random.Random(2)
+    out = (C.c_int * 64)()
+    for _ in range(600):
+        nk, w, blk = r.randint(0, 260), windows(r), r.choice([8, 32, 64])
+        w = w[:2] + (min(w[2], nk),) + w[3:]
+        pa = r.randint(-30, max(nk - 1, 0))
+        pb = min(pa + r.randint(0, 40), nk - 1)
+        if pb < pa:
+            continue
+        n = host.blocks(pa, pb, nk, (C.c_int * 4)(*w), blk, out, 64)
+        got = list(out[:n])
+        assert got == sorted(set(got)) and all(0 <= b and b * blk < nk for b in got)
+        need = {j // blk for p in range(pa, pb + 1) for j in range(nk) if sees(p, j, nk, *w)}
+        assert need <= set(got), (pa, pb, nk, w, blk)
+        assert set(got) - need <= set(range(min(got), max(got) + 1)) if need else True
+        assert len(set(got) - need) <= 1 or w[0] < 0, (pa, pb, nk, w, blk, got, need)
+
+
+def test_seen_from(host):
+    """the queries that see a key exactly; those of a run of keys at least"""
+    r = random.Random(3)
+    out = (C.c_int * 2)()
+    for _ in range(600):
+        nq, nk, w = r.randint(1, 80), r.randint(1, 80), windows(r)
+        w = w[:2] + (min(w[2], nk),) + w[3:]
+        off = nk - nq
+        k0 = r.randint(0, nk - 1)
+        host.__getattr__("from")(k0, k0, nq, off, (C.c_int * 4)(*w), out)
+        assert set(range(out[0], out[1] + 1)) == {i for i in range(nq) if sees(i + off, k0, nk, *w)}, (k0, nq, nk, w)
+        k1 = min(nk - 1, k0 + r.randint(0, 50))
+        host.__getattr__("from")(k0, k1, nq, off, (C.c_int * 4)(*w), out)
+        need = {i for i in range(nq) for k in range(k0, k1 + 1) if sees(i + off, k, nk, *w)}
+        assert need <= set(range(out[0], out[1] + 1)) and out[0] >= 0 and out[1] < nq
+
+
+def test_key_items(host):
+    """every tile of keys, with its shares one after another; no more workgroups than a launch takes"""
+    r = random.Random(4)
+    for _ in range(300):
+        K, G = r.choice([1, 2, 8]), r.choice([1, 2, 8])
+        sq, sk = r.randint(1, 9000), r.randint(1, 9000)
+        i = (sa3k.TYPE_BF16, r.randint(1, 8), K * G, K, 64, sq, sk, r.choice([-1, 0, 100, 2000]), r.choice([-1, 0, 100]),
+             r.choice([0, 4, 200, 9000]), r.randint(0, 1))
+        out, few = (C.c_int * (3 * 40000))(), C.c_int()
+        n = host.items((C.c_int * 11)(*i), (C.c_int64 * 12)(*[8] * 12), out, 40000, C.byref(few))
+        assert 0 < n < 40000 and i[1] * K * n * 256 < 1 << 32
+        got = [tuple(out[3 * k:3 * k + 3]) for k in range(n)]
+        want = []
+        for t in range(-(-sk // 128)):
+            s = [g[2] for g in got if g[0] == t]
+            assert len(set(s)) == 1 and len(s) == s[0] <= 256
+            want += [(t, k, s[0]) for k in range(s[0])]
+        assert got == want
+        assert 1 <= few.value <= 512
