@@ -295,4 +295,89 @@ SA3K_HD Span seen_from(int k0, int k1, int nq, int off, int left, int right, int
     return r;
 }
 
+// --------------------------------------------------------------------------------------- product
+struct ProdArgs {
+    int type = 0, act = 0;
+    int64_t M = 0, N = 0, K = 0;
+    const void *X = nullptr, *W = nullptr, *R = nullptr, *dY = nullptr, *Z = nullptr;
+    void *Y = nullptr, *Zo = nullptr, *dX = nullptr, *dW = nullptr;   // Zo: the forward's z
+    int64_t ldx = 0, ldw = 0, ldr = 0, lddy = 0, ldz = 0, ldy = 0, lddx = 0, lddw = 0;
+    const float* bias = nullptr;
+    float* db = nullptr;
+    int dw_type = 0, accumulate = 0;
+};
+
+constexpr int64_t kProdMaxPitch = (int64_t)1 << 22;   // 256 rows of it in bytes stay below 2^31
+
+inline const char* prod_check(const ProdArgs& a, bool bwd, int* code) {
+    *code = SA3K_ERR_INVALID;
+    if (a.type != SA3K_TYPE_BF16 && a.type != SA3K_TYPE_F16) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "type must be bf16 or f16";
+    }
+    if (a.act < SA3K_ACT_NONE || a.act > SA3K_ACT_GELU_TANH) return "unknown activation";
+    if (a.M < 0 || a.M >= kMaxExtent) return "M out of range";
+    if (a.N <= 0 || a.K <= 0 || a.N >= kProdMaxPitch || a.K >= kProdMaxPitch) return "N or K out of range";
+    if (bwd && a.accumulate != 0 && a.accumulate != 1) return "accumulate must be 0 or 1";
+    if (bwd && a.dW && a.dw_type != a.type && a.dw_type != SA3K_TYPE_F32) return "dw_type must be f32 or type";
+    if (bwd && a.dW && a.accumulate && a.dw_type != SA3K_TYPE_F32) return "only an f32 dW can be added to";
+    const void* p[9] = {a.X, a.W, a.R, a.dY, a.Z, a.Y, a.Zo, a.dX, a.dW};
+    const int64_t ld[9] = {a.ldx, a.ldw, a.ldr, a.lddy, a.ldz, a.ldy, a.ldz, a.lddx, a.lddw};
+    const int64_t w[9] = {a.K, a.K, a.N, a.N, a.N, a.N, a.N, a.K, a.K};
+    for (int i = 0; i < 9; ++i) {
+        if (!p[i]) continue;
+        if (ld[i] < w[i] || ld[i] >= kProdMaxPitch) return "a row pitch is smaller than its rows or out of range";
+        if (!elem_aligned(p[i], i == 8 ? elem_bytes(a.dw_type) : 2)) return "a tensor is not aligned to its elements";
+    }
+    if (!elem_aligned(a.bias, 4) || !elem_aligned(a.db, 4)) return "an f32 vector is not 4-byte aligned";
+    // a launch has fewer than 2^24 workgroups: tiles of 64 x 64 at the least, and the split sums' 2048 values
+    if (((a.M + 63) / 64) * ((a.N > a.K ? a.N : a.K) / 64 + 1) >= ((int64_t)1 << 23)) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "M x N is too large for one launch";
+    }
+    if (!bwd) {
+        if (!a.W) return "W must not be null";
+        if (a.M > 0 && (!a.X || !a.Y)) return "X and Y must not be null";
+    } else {
+        if (a.M > 0 && !a.dY) return "dY must not be null";
+        if (a.M > 0 && a.act != SA3K_ACT_NONE && !a.Z) return "an activation needs Z";
+        if (a.M > 0 && a.dW && !a.X) return "dW needs X";
+        if (a.dX && !a.W) return "dX needs W";
+    }
+    return nullptr;
+}
+
+// The tiles (square, `edge` wide) of an M x N x K product and the split of its contraction, by estimated time in
+// microseconds. Measured on MI355X: a round of 256 x 256 tiles (one workgroup a CU) takes 1.7 a tile of 64 along K, one of
+// 128 x 128 tiles 1.05 with two workgroups a CU and 0.7 with one; a workgroup's start and its stores about 4; the
+// launch that adds up splits 4 and its traffic at 4 MB a microsecond.
+struct ProdPlan {
+    int edge, splits, per;   // per: tiles of 64 along K that a split takes
+};
+inline ProdPlan prod_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t kt = (K + 63) / 64;
+    ProdPlan best{128, 1, (int)kt};
+    double least = 1e300;
+    for (int edge = 256; edge >= 128; edge /= 2) {
+        const int64_t tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
+        for (int64_t n = 1; n <= 16 && n <= kt; ++n) {
+            if (n > 1 && (double)n * (double)M * (double)(N + 8) > 67108864.0) break;   // 256 MB of split sums
+            const int64_t per = (kt + n - 1) / n;
+            if ((n - 1) * per >= kt) continue;   // an empty split
+            const int64_t wgs = tiles * n, slots = edge == 256 ? 256 : 512;
+            const double step = edge == 256 ? 1.7 : wgs <= 256 ? 0.7 : 1.05;
+            const double rounds = (double)((wgs + slots - 1) / slots);
+            double t = rounds * ((double)per * step + 4.0);
+            if (n > 1) t += 4.0 + 8.0 * (double)n * (double)M * (double)N / 4e6;
+            if (t < least) {
+                least = t;
+                best = ProdPlan{edge, (int)n, (int)per};
+            }
+        }
+    }
+    return best;
+}
+// Few rows run on a kernel whose waves split K, without tiles in LDS.
+constexpr int64_t kFewRows = 32;
+
 }  // namespace sa3k

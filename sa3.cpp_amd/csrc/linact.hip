@@ -1,0 +1,658 @@
+// Products with bias, activation and residual in the epilogue, and their backward:
+//   z = X W^T + b, Y = act(z) + R;   dz = dY act'(z), dX = dz W, dW = dz^T X, db = sum over rows dz
+//
+// One tile kernel does the three products C[m][n] = sum_k A(m, k) B(n, k), on v_mfma_f32_32x32x16 with f32 sums. An operand
+// lies K-contiguous ([rows][K]: X, W and dz of dX) or K-major ([K][rows]: W of dX, both of dW); a K-major tile is staged as
+// it lies, as sub-tiles of [64 k][64 rows], and read transposed (ds_read_b64_tr_b16), so no operand is ever transposed
+// in memory. Tiles of 64 along K go straight into LDS (buffer_load ... lds) through a descriptor that ends where the
+// operand does: rows and K past the end are zeros. Two stages; the loads of tile t + 1 run while t is computed.
+//
+// These loads take 16 bytes: operands whose rows are not 16-byte aligned, or not a multiple of 8 long, are copied once into
+// padded rows first (a copy of M K + N K elements against M N K multiply-adds).
+#include <algorithm>
+
+#include "wattn.h"
+
+namespace sa3k {
+float* gemm_workspace_bytes(sa3k_ctx* ctx, size_t bytes);   // gemm.hip: context-owned scratch
+}
+
+namespace {
+using namespace sa3k;
+using wattn::buffer_rsrc;
+using wattn::dma16;
+using wattn::ex2;
+using wattn::f32x16;
+using wattn::lds_ptr_t;
+using wattn::swz;
+using wattn::u32x4;
+using wattn::Vec;
+using wattn::kLog2e;
+
+typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
+
+struct GemmArgs {
+    const void *A, *B;
+    int64_t lda, ldb, M, N, K;
+    void* C;             // T, or f32
+    int64_t ldc;
+    int c_f32, accumulate;
+    // the forward's epilogue
+    int act;
+    const float* bias;
+    const void* R;
+    int64_t ldr;
+    void* Z;
+    int64_t ldz;
+    float* part;         // [splits][M][pitch] sums of the K splits, or null
+    int64_t pitch;
+    int splits, per;
+};
+
+// The activations on the hardware's exp2 and reciprocal. For gelu_tanh, (1 + tanh u) / 2 = 1 / (1 + e^-2u); its argument is
+// held within +-10, where it is 0 or 1 in f32, so that a large z^3 does not overflow.
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + ex2(-kLog2e * x)); }
+__device__ __forceinline__ float act_value(float z, int act) {
+    if (act == SA3K_ACT_RELU) return z <= 0.f ? 0.f : z;
+    if (act == SA3K_ACT_SILU) return z * sigmoid(z);
+    if (act == SA3K_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if (act == SA3K_ACT_GELU_TANH) {
+        const float y = fminf(fmaxf(z, -10.f), 10.f);
+        return z * sigmoid(1.5957691216057308f * (y + 0.044715f * y * y * y));
+    }
+    return z;
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == SA3K_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if (act == SA3K_ACT_SILU) {
+        const float g = sigmoid(z);
+        return g * (1.f + z * (1.f - g));
+    }
+    if (act == SA3K_ACT_GELU)
+        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * ex2(-0.5f * kLog2e * z * z) * 0.39894228040143268f;
+    if (act == SA3K_ACT_GELU_TANH) {
+        const float y = fminf(fmaxf(z, -10.f), 10.f);
+        const float g = sigmoid(1.5957691216057308f * (y + 0.044715f * y * y * y));
+        return g + y * g * (1.f - g) * 1.5957691216057308f * (1.f + 0.134145f * y * y);
+    }
+    return 1.f;
+}
+
+// n .. n + 7 of a row of `cols` elements, zeros past its end
+template <class S>
+__device__ __forceinline__ void load8(const S* p, int64_t n, int64_t cols, float (&v)[8]) {
+    if (n + 8 <= cols) {
+        const Pack<S, 8> q = *reinterpret_cast<const Pack<S, 8>*>(p + n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)q.v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = n + e < cols ? (float)p[n + e] : 0.f;
+    }
+}
+template <class S>
+__device__ __forceinline__ void store8(S* p, int64_t n, int64_t cols, const float (&v)[8]) {
+    if (n + 8 <= cols) {
+        Pack<S, 8> q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q.v[e] = (S)v[e];
+        *reinterpret_cast<Pack<S, 8>*>(p + n) = q;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (n + e < cols) p[n + e] = (S)v[e];
+    }
+}
+
+// Eight finished sums of row m, columns n .. n + 7. FWD: bias, activation, residual.
+template <class T, bool FWD>
+__device__ __forceinline__ void finish8(const GemmArgs& a, int64_t m, int64_t n, float (&v)[8]) {
+    if constexpr (FWD) {
+        if (a.bias) {
+            float b[8];
+            load8(a.bias, n, a.N, b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += b[e];
+        }
+        if (a.Z) store8(static_cast<T*>(a.Z) + m * a.ldz, n, a.N, v);
+        if (a.act) {   // (uniform)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = act_value(v[e], a.act);
+        }
+        if (a.R) {
+            float r[8];
+            load8(static_cast<const T*>(a.R) + m * a.ldr, n, a.N, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r[e];
+        }
+        store8(static_cast<T*>(a.C) + m * a.ldc, n, a.N, v);
+    } else {
+        if (a.c_f32) {
+            float* c = static_cast<float*>(a.C) + m * a.ldc;
+            if (a.accumulate) {
+                float o[8];
+                load8(c, n, a.N, o);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += o[e];
+            }
+            store8(c, n, a.N, v);
+        } else {
+            store8(static_cast<T*>(a.C) + m * a.ldc, n, a.N, v);
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+// One operand's tile: ROWS rows x 64 of K. KMAJOR: stored [K][rows], staged as sub-tiles of [64 k][64 rows].
+template <class T, int ROWS, int NT, bool KMAJOR>
+struct Operand {
+    typedef typename Vec<T>::x8 x8;
+    static constexpr int PER = ROWS * 8 / NT;   // loads a thread makes for a tile
+    const char* base;                           // of the tile's first row at K = 0
+    int64_t step;                               // bytes from one tile of K to the next
+    uint32_t row_bytes, off[PER];
+    int rows, kc;                               // rows in range; this thread's chunk of K (K-contiguous)
+
+    __device__ __forceinline__ void init(const void* p, int64_t ld, int64_t row0, int64_t n, int tid) {
+        row_bytes = (uint32_t)(ld * 2);
+        rows = (int)min((int64_t)ROWS, n - row0);
+        base = static_cast<const char*>(p) + (KMAJOR ? row0 * 2 : row0 * ld * 2);
+        step = KMAJOR ? 64 * ld * 2 : 128;
+        // slot s = q NT + tid of an LDS row of eight 16-byte chunks holds chunk (s % 8) ^ swz(row); NT / 8 is a multiple of 16,
+        // so a thread's chunk is the same in every round
+        kc = (tid & 7) ^ swz(tid >> 3);
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int s = q * NT + tid;
+            if constexpr (KMAJOR)
+                off[q] = (uint32_t)((s & 511) >> 3) * row_bytes + (uint32_t)((s >> 9) * 128 + kc * 16);
+            else
+                off[q] = (uint32_t)(s >> 3) * row_bytes + (uint32_t)(kc * 16);
+        }
+    }
+    // tile t of K, `left` of K in range from its start on, into LDS at lds_addr
+    __device__ __forceinline__ void issue(int64_t t, int64_t left, uint32_t lds_addr, int wave) const {
+        const int k = (int)min((int64_t)64, left);
+        // The last row in range ends the descriptor: rows past it are zeros. Rows are whole chunks of 8 elements, or padded to
+        // that with zeros (a descriptor that ended inside a chunk would drop the dword that crosses its end).
+        const uint32_t bytes = KMAJOR ? (uint32_t)(k - 1) * row_bytes + (uint32_t)((rows + 7) & ~7) * 2
+                                      : (uint32_t)(rows - 1) * row_bytes + (uint32_t)((k + 7) & ~7) * 2;
+        const u32x4 rs = buffer_rsrc(base + t * step, bytes);
+        const bool none = !KMAJOR && kc * 8 >= k;   // a chunk past K lies in the next row: kept out
+#pragma unroll
+        for (int q = 0; q < PER; ++q)
+            dma16(rs, none ? 0xFFFFFFF0u : off[q], __builtin_amdgcn_readfirstlane(lds_addr + (uint32_t)((q * NT + wave * 64) * 16)));
+    }
+    // the operand of K step ks (16 of K) for rows r0 .. r0 + 31 of the tile
+    static __device__ __forceinline__ x8 frag(const char* t, int r0, int ks, int lane) {
+        const int hl = lane >> 5;
+        if constexpr (KMAJOR) {
+            const char* sub = t + (r0 >> 6) * 8192;
+            const int n = (r0 & 63) + 16 * ((lane >> 4) & 1), k = 16 * ks + 8 * hl;
+            const typename Vec<T>::x4 a = wattn::ld_tr<T>(sub, k, n, lane), b = wattn::ld_tr<T>(sub, k + 4, n, lane);
+            return x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        } else {
+            return wattn::ld_row<T, ROWS>(t, r0 + (lane & 31), 2 * ks + hl);
+        }
+    }
+};
+
+// Square tiles of EDGE. 256: eight waves of 64 x 128, one workgroup a CU; 128: four waves of 64 x 64, two.
+template <class T, int EDGE, bool AK, bool BK, bool FWD>
+__global__ __launch_bounds__(EDGE * 2, 2) void prod_tile_kernel(GemmArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    constexpr int NT = EDGE * 2, WM = EDGE / 64, WTN = EDGE == 256 ? 128 : 64, FM = 2, FN = WTN / 32;
+    constexpr int OPB = EDGE * 128, STAGE = 2 * OPB;
+    constexpr int ER = 64, EROW = EDGE + 8;
+    static_assert(ER * EROW * 4 <= 2 * STAGE, "staged rows fit the stages' memory");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+    // Workgroups go out to the 8 XCDs in turn: XCD c takes the run [c n / 8, (c + 1) n / 8) of the items in (split, raster)
+    // order, in groups of eight rows of tiles, so that tiles that share operands run on one XCD and share its L2.
+    const int tiles_m = (int)((a.M + EDGE - 1) / EDGE), tiles_n = (int)((a.N + EDGE - 1) / EDGE);
+    const int nwg = gridDim.x, L = blockIdx.x + nwg * blockIdx.y;
+    const int item = (L & 7) * ((nwg * (int)gridDim.y) >> 3) + (L >> 3);
+    const int z = __builtin_amdgcn_readfirstlane(item / nwg), bid = __builtin_amdgcn_readfirstlane(item - z * nwg);
+    if (bid >= tiles_m * tiles_n) return;
+    const int group = bid / (8 * tiles_n), gsz = min(tiles_m - group * 8, 8), in_g = bid - group * 8 * tiles_n;
+    const int64_t m0 = (int64_t)(group * 8 + in_g % gsz) * EDGE, n0 = (int64_t)(in_g / gsz) * EDGE;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm0 = (wave % WM) * 64, wn0 = (wave / WM) * WTN;
+
+    Operand<T, EDGE, NT, AK> A;
+    Operand<T, EDGE, NT, BK> B;
+    A.init(a.A, a.lda, m0, a.M, tid);
+    B.init(a.B, a.ldb, n0, a.N, tid);
+    const int64_t KT = (a.K + 63) / 64, t0 = (int64_t)z * a.per, t1 = min(KT, t0 + a.per);
+    f32x16 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+    auto issue = [&](int st, int64_t t) {
+        A.issue(t, a.K - t * 64, lds0 + st * STAGE, wave);
+        B.issue(t, a.K - t * 64, lds0 + st * STAGE + OPB, wave);
+    };
+    auto compute = [&](const char* As) {
+        const char* Bs = As + OPB;
+        x8 af[2][FM], bf[2][FN];
+        auto load = [&](int ks, int slot) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i) af[slot][i] = Operand<T, EDGE, NT, AK>::frag(As, wm0 + 32 * i, ks, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) bf[slot][j] = Operand<T, EDGE, NT, BK>::frag(Bs, wn0 + 32 * j, ks, lane);
+        };
+        auto mma = [&](int slot) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = Vec<T>::mfma(af[slot][i], bf[slot][j], acc[i][j]);
+        };
+        load(0, 0);
+        load(1, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+        mma(0);
+        load(2, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        mma(1);
+        load(3, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        mma(0);
+        mma(1);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    if (t0 < t1) issue(0, t0);
+    // one body for both stages: written out for each, the compiler moved the sums between registers and spilled some
+    for (int64_t t = t0; t < t1; ++t) {
+        const int stage = (int)(t - t0) & 1;
+        wait_vmcnt<0>();
+        asm volatile("s_barrier" ::: "memory");   // tile t is there; every wave is done with the other stage
+        if (t + 1 < t1) issue(stage ^ 1, t + 1);
+        compute(lds + stage * STAGE);
+    }
+    // the sums pass through LDS, 64 rows at a time, so that a thread stores 8 columns of a row
+    float* st = reinterpret_cast<float*>(lds);
+    constexpr int CPR = EDGE / 8;   // threads a row
+    const int cq = (tid % CPR) * 8;
+    const int64_t n = n0 + cq;
+    __syncthreads();
+#pragma unroll 1
+    for (int rb = 0; rb < EDGE; rb += ER) {
+        if (wm0 == rb) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        st[(32 * i + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3)) * EROW + wn0 + 32 * j + (lane & 31)] =
+                            acc[i][j][v];
+        }
+        __syncthreads();
+        for (int r = tid / CPR; r < ER; r += NT / CPR) {
+            const int64_t m = m0 + rb + r;
+            if (m >= a.M || n >= a.N) break;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(st + r * EROW + cq + e);
+                v[e] = x.x;
+                v[e + 1] = x.y;
+                v[e + 2] = x.z;
+                v[e + 3] = x.w;
+            }
+            if (a.part) store8(a.part + ((int64_t)z * a.M + m) * a.pitch, n, a.pitch, v);
+            else finish8<T, FWD>(a, m, n, v);
+        }
+        __syncthreads();
+    }
+}
+
+// the K splits' sums in their order, then the epilogue
+template <class T, bool FWD>
+__global__ __launch_bounds__(256) void prod_sum_kernel(GemmArgs a) {
+    const int64_t chunks = a.pitch / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / chunks, n = (i - m * chunks) * 8;
+    if (m >= a.M) return;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    const float* p = a.part + m * a.pitch + n;
+    for (int z = 0; z < a.splits; ++z, p += a.M * a.pitch)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(p + e);
+            v[e] += x.x;
+            v[e + 1] += x.y;
+            v[e + 2] += x.z;
+            v[e + 3] += x.w;
+        }
+    finish8<T, FWD>(a, m, n, v);
+}
+
+// Few rows (at most 16 MB): 16 columns of the output a workgroup, whose eight waves split K in steps of 32 and read W
+// straight from memory into the MFMA's registers (each element once); the waves' sums are joined in LDS.
+template <class T, int MB>
+__global__ __launch_bounds__(512) void prod_few_kernel(GemmArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    constexpr int W = 8, U = 4;
+    __shared__ float red[W][MB][16][17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15;
+    const int64_t n0 = (int64_t)blockIdx.x * 16, wn = n0 + r;
+    const int64_t steps = (a.K + 31) / 32;
+    const T* wp = static_cast<const T*>(a.B) + min(wn, a.N - 1) * a.ldb;
+    const T* xp[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) xp[b] = static_cast<const T*>(a.A) + min((int64_t)(16 * b + r), a.M - 1) * a.lda;
+    f32x4 acc[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // eight of K at k, zeros past its end (rows and columns past theirs repeat the last one: never stored)
+    auto ld = [&](const T* p, int64_t k) {
+        x8 v;
+        if (k + 8 <= a.K) {
+            const Pack<T, 8> q = *reinterpret_cast<const Pack<T, 8>*>(p + k);
+            v = __builtin_bit_cast(x8, q);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? p[k + e] : (T)0.f;
+        }
+        return v;
+    };
+    for (int64_t s0 = wave; s0 < steps; s0 += W * U) {
+        x8 w[U], x[U][MB];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = (s0 + u * W) * 32 + 8 * (lane >> 4);
+            w[u] = ld(wp, k);
+#pragma unroll
+            for (int b = 0; b < MB; ++b) x[u][b] = ld(xp[b], k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+                if constexpr (sizeof(T) == 2 && __is_same(T, bf16))
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u], x[u][b], acc[b], 0, 0, 0);
+                else
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[u], x[u][b], acc[b], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) red[wave][b][r][4 * (lane >> 4) + v] = acc[b][v];
+    __syncthreads();
+    for (int i = tid; i < MB * 256; i += 512) {
+        const int64_t m = i >> 4, n = n0 + (i & 15);
+        if (m >= a.M || n >= a.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v += red[w][m >> 4][m & 15][i & 15];
+        if (a.bias) v += a.bias[n];
+        if (a.Z) static_cast<T*>(a.Z)[m * a.ldz + n] = (T)v;
+        v = act_value(v, a.act);
+        if (a.R) v += (float)static_cast<const T*>(a.R)[m * a.ldr + n];
+        static_cast<T*>(a.C)[m * a.ldc + n] = (T)v;
+    }
+}
+
+// rows [rows][cols] into rows of `pitch` (a multiple of 8), zeros behind them
+template <class T>
+__global__ __launch_bounds__(256) void prod_pad_kernel(const T* src, int64_t ld, int64_t rows, int64_t cols, T* dst,
+                                                       int64_t pitch) {
+    const int64_t chunks = pitch / 8, n = rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+        float v[8];
+        load8(src + r * ld, c, cols, v);
+        store8(dst + r * pitch, c, pitch, v);
+    }
+}
+
+// dz = dY act'(z) [M][pitch] (null: not stored) and its column sums over this workgroup's rows, part [gridDim.y][N] (null:
+// none). A workgroup takes 256 columns, 8 a thread, eight rows at a time.
+template <class T>
+__global__ __launch_bounds__(256) void prod_dz_kernel(const T* dY, int64_t lddy, const T* Z, int64_t ldz, int64_t M, int64_t N,
+                                                      int act, T* dz, int64_t pitch, float* part) {
+    __shared__ float red[8][256 + 8];
+    const int c = (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 256 + c;
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = 0.f;
+    if (n < N)
+        for (int64_t m = (int64_t)blockIdx.y * 8 + rl; m < M; m += (int64_t)gridDim.y * 8) {
+            float d[8];
+            load8(dY + m * lddy, n, N, d);
+            if (act) {   // (uniform)
+                float z[8];
+                load8(Z + m * ldz, n, N, z);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[e] *= act_slope(z[e], act);
+            }
+            if (dz) store8(dz + m * pitch, n, pitch, d);   // (columns past N: 0)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += d[e];
+        }
+    if (!part) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[rl][c + e] = s[e];
+    __syncthreads();
+    const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (j >= N) return;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
+    part[(int64_t)blockIdx.y * N + j] = t;
+}
+
+// db (+)= the workgroups' sums, in their order: 64 columns a workgroup, a quarter of the sums a wave, eight in flight
+__global__ __launch_bounds__(256) void prod_db_kernel(const float* __restrict__ part, int parts, int64_t N, float* db,
+                                                      int accumulate) {
+    __shared__ float s[4][64];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+    const int per = (parts + 3) / 4, lo = min(parts, w * per), hi = min(parts, lo + per);
+    float t = 0.f;
+    if (i < N)
+        for (int k = lo; k < hi; k += 8) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)min(k + u, hi - 1) * N + i];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (k + u < hi) t += v[u];
+        }
+    s[w][lane] = t;
+    __syncthreads();
+    if (w || i >= N) return;
+    t = ((s[0][lane] + s[1][lane]) + s[2][lane]) + s[3][lane];
+    db[i] = accumulate ? db[i] + t : t;
+}
+
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// whether the tile kernel's 16-byte loads can take rows of `cols` elements
+bool loads16(const void* p, int64_t ld, int64_t cols) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && cols % 8 == 0;
+}
+
+// The context's scratch, cut into pieces: first their sizes are added up, then the one allocation is handed out.
+struct Scratch {
+    size_t need = 0;
+    size_t take(size_t bytes) {
+        const size_t at = need;
+        need += up256(bytes);
+        return at;
+    }
+};
+
+template <class T>
+const T* padded(sa3k_ctx* ctx, const void* p, int64_t ld, int64_t rows, int64_t cols, char* to) {
+    KernelScope ks(ctx, "linear_act_pad");
+    const int64_t n = rows * (up8(cols) / 8);
+    launch_k(ctx, false, prod_pad_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 65536)), dim3(256), 0,
+             static_cast<const T*>(p), ld, rows, cols, reinterpret_cast<T*>(to), up8(cols));
+    SA3K_LAUNCHED();
+    return reinterpret_cast<const T*>(to);
+}
+
+size_t split_bytes(const ProdPlan& p, int64_t M, int64_t N) {
+    return p.splits > 1 ? (size_t)p.splits * (size_t)M * (size_t)up8(N) * sizeof(float) : 0;
+}
+
+template <class T, int EDGE, bool AK, bool BK, bool FWD>
+void tile_launch(sa3k_ctx* ctx, const GemmArgs& a, const char* name) {
+    const int64_t tiles = ceil_div(a.M, EDGE) * ceil_div(a.N, EDGE);
+    KernelScope ks(ctx, name, 2.0 * (double)a.M * (double)a.N * (double)a.K);
+    launch_k(ctx, a.splits == 1, prod_tile_kernel<T, EDGE, AK, BK, FWD>,
+             dim3((unsigned)(ceil_div(tiles, 8) * 8), (unsigned)a.splits), dim3(EDGE * 2), 0, a);
+    SA3K_LAUNCHED();
+}
+template <class T, bool AK, bool BK, bool FWD>
+void tile_run(sa3k_ctx* ctx, GemmArgs& a, const ProdPlan& p, float* part, const char* name) {
+    a.splits = p.splits;
+    a.per = p.per;
+    a.part = p.splits > 1 ? part : nullptr;
+    a.pitch = up8(a.N);
+    if (p.edge == 256) tile_launch<T, 256, AK, BK, FWD>(ctx, a, name);
+    else tile_launch<T, 128, AK, BK, FWD>(ctx, a, name);
+    if (p.splits > 1) {
+        KernelScope ks(ctx, "linear_act_sum");
+        launch_k(ctx, true, prod_sum_kernel<T, FWD>, dim3((unsigned)ceil_div(a.M * (a.pitch / 8), 256)), dim3(256), 0, a);
+        SA3K_LAUNCHED();
+    }
+}
+
+template <class T>
+void fwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
+    GemmArgs a{};
+    a.A = p.X; a.lda = p.ldx; a.B = p.W; a.ldb = p.ldw;
+    a.M = p.M; a.N = p.N; a.K = p.K;
+    a.C = p.Y; a.ldc = p.ldy; a.act = p.act; a.bias = p.bias; a.R = p.R; a.ldr = p.ldr; a.Z = p.Zo; a.ldz = p.ldz;
+    if (p.M <= kFewRows) {
+        KernelScope ks(ctx, "linear_act_few", 2.0 * (double)a.M * (double)a.N * (double)a.K);
+        const dim3 grid((unsigned)ceil_div(a.N, 16));
+        if (p.M <= 16) launch_k(ctx, true, prod_few_kernel<T, 1>, grid, dim3(512), 0, a);
+        else launch_k(ctx, true, prod_few_kernel<T, 2>, grid, dim3(512), 0, a);
+        SA3K_LAUNCHED();
+        return;
+    }
+    const bool px = !loads16(p.X, p.ldx, p.K), pw = !loads16(p.W, p.ldw, p.K);
+    const int64_t Kp = px || pw ? up8(p.K) : p.K;
+    const ProdPlan plan = prod_plan(p.M, p.N, Kp);
+    Scratch s;
+    // (if one operand is padded, both are: they share K)
+    const size_t ox = s.take(px || pw ? (size_t)p.M * Kp * 2 : 0), ow = s.take(px || pw ? (size_t)p.N * Kp * 2 : 0);
+    const size_t os = s.take(split_bytes(plan, p.M, p.N));
+    char* ws = s.need ? reinterpret_cast<char*>(gemm_workspace_bytes(ctx, s.need)) : nullptr;
+    if (px || pw) {
+        a.A = padded<T>(ctx, p.X, p.ldx, p.M, p.K, ws + ox);
+        a.B = padded<T>(ctx, p.W, p.ldw, p.N, p.K, ws + ow);
+        a.lda = a.ldb = a.K = Kp;
+    }
+    tile_run<T, false, false, true>(ctx, a, plan, reinterpret_cast<float*>(ws + os), "linear_act_fwd");
+}
+
+constexpr int kDzParts = 256;   // row shares of the pass over dY and z, at the most
+
+template <class T>
+void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
+    const int64_t M = p.M, N = p.N, K = p.K, Np = up8(N), Kp = up8(K);
+    const bool products = p.dX || p.dW;
+    // dz as the products read it: dY itself, or its own rows
+    const bool own_dz = products && M > 0 && (p.act != SA3K_ACT_NONE || !loads16(p.dY, p.lddy, N));
+    const bool px = p.dW && M > 0 && !loads16(p.X, p.ldx, K), pw = p.dX && M > 0 && !loads16(p.W, p.ldw, K);
+    const ProdPlan px_plan = prod_plan(M > 0 ? M : 1, K, N), pw_plan = prod_plan(N, K, M > 0 ? M : 1);
+    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(kDzParts, ceil_div(M, 8)));
+    Scratch s;
+    const size_t oz = s.take(own_dz ? (size_t)M * Np * 2 : 0), ox = s.take(px ? (size_t)M * Kp * 2 : 0);
+    const size_t ow = s.take(pw ? (size_t)N * Kp * 2 : 0), ob = s.take(p.db ? (size_t)parts * N * 4 : 0);
+    const size_t os = s.take(std::max(p.dX ? split_bytes(px_plan, M, K) : 0, p.dW ? split_bytes(pw_plan, N, K) : 0));
+    char* ws = s.need ? reinterpret_cast<char*>(gemm_workspace_bytes(ctx, s.need)) : nullptr;
+    T* dz = own_dz ? reinterpret_cast<T*>(ws + oz) : nullptr;
+    float* part = p.db ? reinterpret_cast<float*>(ws + ob) : nullptr;
+    if (own_dz || p.db) {
+        KernelScope ks(ctx, "linear_act_dz");
+        launch_k(ctx, false, prod_dz_kernel<T>, dim3((unsigned)ceil_div(N, 256), (unsigned)parts), dim3(256), 0,
+                 static_cast<const T*>(p.dY), p.lddy, static_cast<const T*>(p.Z), p.ldz, M, N, p.act, dz, Np, part);
+        SA3K_LAUNCHED();
+    }
+    if (p.db) {
+        KernelScope ks(ctx, "linear_act_db");
+        launch_k(ctx, !products, prod_db_kernel, dim3((unsigned)ceil_div(N, 64)), dim3(256), 0, part, parts, N, p.db,
+                 p.accumulate);
+        SA3K_LAUNCHED();
+    }
+    const void* g = own_dz ? dz : p.dY;
+    const int64_t ldg = own_dz ? Np : p.lddy;
+    if (p.dX && M > 0) {   // [M][K] = dz [M][N] . W [N][K]
+        GemmArgs a{};
+        a.A = g; a.lda = ldg;
+        a.B = pw ? padded<T>(ctx, p.W, p.ldw, N, K, ws + ow) : p.W;
+        a.ldb = pw ? Kp : p.ldw;
+        a.M = M; a.N = K; a.K = N;
+        a.C = p.dX; a.ldc = p.lddx;
+        tile_run<T, false, true, false>(ctx, a, px_plan, reinterpret_cast<float*>(ws + os), "linear_act_dx");
+    }
+    if (p.dW) {   // [N][K] = dz^T [N][M] . X [M][K]
+        GemmArgs a{};
+        a.A = g; a.lda = ldg;
+        a.B = px ? padded<T>(ctx, p.X, p.ldx, M, K, ws + ox) : p.X;
+        a.ldb = px ? Kp : p.ldx;
+        a.M = N; a.N = K; a.K = M;
+        a.C = p.dW; a.ldc = p.lddw;
+        a.c_f32 = p.dw_type == SA3K_TYPE_F32;
+        a.accumulate = p.accumulate;
+        tile_run<T, true, true, false>(ctx, a, pw_plan, reinterpret_cast<float*>(ws + os), "linear_act_dw");
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+SA3K_API int sa3k_linear_act_fwd(sa3k_ctx* ctx, int type, int act, const void* X, int64_t ldx, const void* W, int64_t ldw,
+                                 const float* bias, const void* residual, int64_t ldr, int64_t M, int64_t N, int64_t K,
+                                 void* Y, int64_t ldy, void* Z, int64_t ldz) {
+    return sa3k_guard(ctx, "sa3k_linear_act_fwd", [&] {
+        ProdArgs p;
+        p.type = type; p.act = act; p.M = M; p.N = N; p.K = K;
+        p.X = X; p.ldx = ldx; p.W = W; p.ldw = ldw; p.bias = bias; p.R = residual; p.ldr = ldr;
+        p.Y = Y; p.ldy = ldy; p.Zo = Z; p.ldz = ldz;
+        int code;
+        const char* msg = prod_check(p, false, &code);
+        require_ok(msg, code);
+        if (M == 0) return;
+        DeviceScope dev(ctx);
+        if (type == SA3K_TYPE_BF16) fwd_run<bf16>(ctx, p);
+        else fwd_run<f16>(ctx, p);
+    });
+}
+
+SA3K_API int sa3k_linear_act_bwd(sa3k_ctx* ctx, int type, int act, const void* dY, int64_t lddy, const void* Z, int64_t ldz,
+                                 const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t M, int64_t N, int64_t K,
+                                 void* dX, int64_t lddx, void* dW, int dw_type, int64_t lddw, float* db, int accumulate) {
+    return sa3k_guard(ctx, "sa3k_linear_act_bwd", [&] {
+        ProdArgs p;
+        p.type = type; p.act = act; p.M = M; p.N = N; p.K = K;
+        p.dY = dY; p.lddy = lddy; p.Z = Z; p.ldz = ldz; p.X = X; p.ldx = ldx; p.W = W; p.ldw = ldw;
+        p.dX = dX; p.lddx = lddx; p.dW = dW; p.dw_type = dw_type; p.lddw = lddw; p.db = db; p.accumulate = accumulate;
+        int code;
+        const char* msg = prod_check(p, true, &code);
+        require_ok(msg, code);
+        DeviceScope dev(ctx);
+        if (type == SA3K_TYPE_BF16) bwd_run<bf16>(ctx, p);
+        else bwd_run<f16>(ctx, p);
+    });
+}
+
+}  // extern "C"

@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(HERE, "libsa3k.so")
 SA3K_OK = 0
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
 PREC_F32, PREC_BF16 = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = range(5)
 
 _lib = None
 
@@ -130,6 +131,8 @@ def _declare(lib):
         "sa3k_layer_norm_bwd": (I, [P, I, P, I64, P, I64, P, I64, I64, I64, P, P, P, P, I64, P, P, I]),
         "sa3k_window_attn_fwd": (I, [P, C.POINTER(WindowAttnShape), P, P, P, P, P, P, P]),
         "sa3k_window_attn_bwd": (I, [P, C.POINTER(WindowAttnShape), P, P, P, P, P, P, P, P, P, P, P]),
+        "sa3k_linear_act_fwd": (I, [P, I, I, P, I64, P, I64, P, P, I64, I64, I64, I64, P, I64, P, I64]),
+        "sa3k_linear_act_bwd": (I, [P, I, I, P, I64, P, I64, P, I64, P, I64, I64, I64, I64, P, I64, P, I, I64, P, I]),
         "sa3k_block_create": (I, [P, C.POINTER(BlockConfig), C.POINTER(BlockWeights), I, I64, I64, C.POINTER(P)]),
         "sa3k_block_destroy": (I, [P, P]),
         "sa3k_block_base_norm_sq": (I, [P, P, I, C.POINTER(P)]),
@@ -705,3 +708,20 @@ class WindowAttn:
         c = self.ctx
         c.check(c.lib.sa3k_window_attn_bwd(c.h, C.byref(self.shape), _p(q), _p(k), _p(v), _p(o), _p(lse), _p(dO), _p(q_len),
                                            _p(k_len), _p(dq), _p(dk), _p(dv)))
+
+
+def linear_act_fwd(ctx, type, act, x, w, M, N, K, y, bias=None, residual=None, z=None, ldx=None, ldw=None, ldr=None,
+                   ldy=None, ldz=None):
+    """y [M][N] = act(z) + residual, z = x [M][K] . w [N][K]^T + bias (z stored when given); pitches in elements"""
+    d = lambda v, n: n if v is None else v  # noqa: E731
+    ctx.check(ctx.lib.sa3k_linear_act_fwd(ctx.h, type, act, _p(x), d(ldx, K), _p(w), d(ldw, K), _p(bias), _p(residual),
+                                          d(ldr, N), M, N, K, _p(y), d(ldy, N), _p(z), d(ldz, N)))
+
+
+def linear_act_bwd(ctx, type, act, dy, x, w, M, N, K, z=None, dx=None, dw=None, db=None, dw_type=None, accumulate=False,
+                   lddy=None, ldz=None, ldx=None, ldw=None, lddx=None, lddw=None):
+    """dx, dw (of `type`, or dw_type) and db of linear_act_fwd"""
+    d = lambda v, n: n if v is None else v  # noqa: E731
+    ctx.check(ctx.lib.sa3k_linear_act_bwd(ctx.h, type, act, _p(dy), d(lddy, N), _p(z), d(ldz, N), _p(x), d(ldx, K), _p(w),
+                                          d(ldw, K), M, N, K, _p(dx), d(lddx, K), _p(dw), d(dw_type, type), d(lddw, K),
+                                          _p(db), int(accumulate)))

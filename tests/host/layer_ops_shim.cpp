@@ -71,4 +71,22 @@ int items(const int* i, const int64_t* st, int* out, int most, int* few) {
     return k.items();
 }
 
+// p: X, W, R, dY, Z, Y, z output, dX, dW, bias, db as addresses; ld: x, w, r, dy, z, y, dx, dw
+int prod(int type, int act, const int64_t* mnk, const int64_t* p, const int64_t* ld, int dw_type, int accumulate, int bwd) {
+    ProdArgs a;
+    a.type = type; a.act = act; a.M = mnk[0]; a.N = mnk[1]; a.K = mnk[2];
+    a.X = at(p[0]); a.W = at(p[1]); a.R = at(p[2]); a.dY = at(p[3]); a.Z = at(p[4]);
+    a.Y = const_cast<void*>(at(p[5])); a.Zo = const_cast<void*>(at(p[6]));
+    a.dX = const_cast<void*>(at(p[7])); a.dW = const_cast<void*>(at(p[8]));
+    a.bias = (const float*)at(p[9]); a.db = (float*)at(p[10]);
+    a.ldx = ld[0]; a.ldw = ld[1]; a.ldr = ld[2]; a.lddy = ld[3]; a.ldz = ld[4]; a.ldy = ld[5]; a.lddx = ld[6]; a.lddw = ld[7];
+    a.dw_type = dw_type; a.accumulate = accumulate;
+    int code = -1;
+    return prod_check(a, bwd != 0, &code) ? code : 0;
+}
+void plan(int64_t M, int64_t N, int64_t K, int* out) {
+    const ProdPlan p = prod_plan(M, N, K);
+    out[0] = p.edge; out[1] = p.splits; out[2] = p.per;
+}
+
 }  // extern "C"

@@ -215,3 +215,68 @@ def test_key_items(host):
             want += [(t, k, s[0]) for k in range(s[0])]
         assert got == want
         assert 1 <= few.value <= 512
+
+
+PROD_P = ("x", "w", "r", "dy", "z", "y", "zo", "dx", "dw", "bias", "db")
+
+
+def prod(host, bwd=False, type=sa3k.TYPE_BF16, act=sa3k.ACT_GELU, M=10, N=24, K=40, dw_type=None, accumulate=0, ld=None, **p):
+    at = dict(x=64, w=64, y=64) if not bwd else dict(x=64, w=64, dy=64, z=64, dx=64, dw=64, db=64)
+    at.update(p)
+    lds = dict(x=K, w=K, r=N, dy=N, z=N, y=N, dx=K, dw=K)
+    lds.update(ld or {})
+    I64 = C.POINTER(C.c_int64)
+    host.prod.argtypes = [C.c_int, C.c_int, I64, I64, I64, C.c_int, C.c_int, C.c_int]
+    return host.prod(type, act, (C.c_int64 * 3)(M, N, K), (C.c_int64 * 11)(*[at.get(n, 0) for n in PROD_P]),
+                     (C.c_int64 * 8)(*[lds[n] for n in ("x", "w", "r", "dy", "z", "y", "dx", "dw")]),
+                     type if dw_type is None else dw_type, accumulate, int(bwd))
+
+
+def test_prod_accepts(host):
+    assert prod(host) == 0 and prod(host, bwd=True) == 0
+    assert prod(host, r=64, zo=64, bias=64) == 0 and prod(host, M=1, N=1, K=1) == 0
+    assert prod(host, x=66, w=34, y=2, ld=dict(x=41, w=43, y=25)) == 0      # any element may start a row
+    assert prod(host, M=0, x=0, y=0) == 0
+    assert prod(host, bwd=True, M=0, dy=0, z=0, x=0) == 0
+    assert prod(host, bwd=True, act=sa3k.ACT_NONE, z=0) == 0
+    assert prod(host, bwd=True, dx=0, w=0) == 0 and prod(host, bwd=True, dw=0, x=0) == 0
+    assert prod(host, bwd=True, dx=0, dw=0, w=0, x=0) == 0
+    assert prod(host, bwd=True, dw_type=sa3k.TYPE_F32, accumulate=1) == 0
+
+
+@pytest.mark.parametrize("want,change", [
+    (UNSUPPORTED, dict(type=sa3k.TYPE_F32)), (INVALID, dict(act=5)), (INVALID, dict(act=-1)), (INVALID, dict(M=-1)),
+    (INVALID, dict(N=0)), (INVALID, dict(K=0)), (INVALID, dict(K=1 << 22)), (INVALID, dict(M=1 << 31)), (INVALID, dict(w=0)),
+    (INVALID, dict(x=0)), (INVALID, dict(y=0)), (INVALID, dict(ld=dict(x=39))), (INVALID, dict(ld=dict(w=1 << 22))),
+    (INVALID, dict(ld=dict(y=23))), (INVALID, dict(x=65)), (INVALID, dict(y=33)), (INVALID, dict(bias=66)),
+    (INVALID, dict(r=64, ld=dict(r=23))), (UNSUPPORTED, dict(M=1 << 27, N=1 << 14)),
+])
+def test_prod_forward_refuses(host, want, change):
+    assert prod(host, **change) == want
+
+
+@pytest.mark.parametrize("want,change", [
+    (UNSUPPORTED, dict(type=8)), (INVALID, dict(dy=0)), (INVALID, dict(z=0)), (INVALID, dict(x=0)), (INVALID, dict(w=0)),
+    (INVALID, dict(accumulate=2)), (INVALID, dict(accumulate=1)), (INVALID, dict(dw_type=sa3k.TYPE_F16)),
+    (INVALID, dict(dw_type=sa3k.TYPE_F32, dw=66)), (INVALID, dict(db=2)), (INVALID, dict(ld=dict(dx=39))),
+    (INVALID, dict(ld=dict(dw=39))), (INVALID, dict(ld=dict(dy=23))), (INVALID, dict(ld=dict(z=23))),
+])
+def test_prod_backward_refuses(host, want, change):
+    assert prod(host, bwd=True, **change) == want
+
+
+def test_prod_plan(host):
+    """the splits cover K, none is empty, their sums fit"""
+    r = random.Random(5)
+    out = (C.c_int * 3)()
+    host.plan.argtypes = [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_int)]
+    seen = set()
+    for _ in range(3000):
+        M, N, K = (int(2 ** r.uniform(0, 14)) for _ in range(3))
+        host.plan(M, N, K, out)
+        edge, splits, per = out
+        kt = -(-K // 64)
+        assert edge in (128, 256) and splits * per >= kt and (splits - 1) * per < kt
+        assert splits == 1 or splits * M * (N + 8) <= 1 << 26
+        seen.add((edge, splits > 1))
+    assert len(seen) == 4   # both tiles, split and not
