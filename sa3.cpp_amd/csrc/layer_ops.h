@@ -241,8 +241,7 @@ inline int attn_splits(const AttnShape& s, int chunks) {
 }
 
 // The dK/dV pass: a workgroup takes a tile of 128 keys and a share of the (query head, block of 64 queries) pairs that
-// see it. Tiles with first tokens, which every later query sees, get `first` shares, the others `rest`, so that no
-// workgroup runs much longer than the ordinary ones and there are about two workgroups a CU where the work allows.
+// see it. Tiles with first tokens, which every later query sees, get `first` shares, the others `rest`.
 constexpr int kKeyTile = 128;
 struct KeySplit {
     int tiles, first_tiles, first, rest;   // first_tiles of the tiles hold first tokens
@@ -252,16 +251,32 @@ inline KeySplit key_split(const AttnShape& s) {
     KeySplit r;
     r.tiles = (s.Sk + kKeyTile - 1) / kKeyTile;
     r.first_tiles = (s.sinks + kKeyTile - 1) / kKeyTile;
-    const int64_t all = (s.Sq + 63) / 64, band = ((int64_t)kKeyTile + s.left + s.right + 62) / 64 + 1;
-    const int64_t most = s.G * (all > 0 ? all : 1), usual = s.G * (band < all ? band : (all > 0 ? all : 1));
-    const int64_t base = (int64_t)s.B * s.K * (r.tiles > 0 ? r.tiles : 1);
-    int64_t n = (512 + base / 2) / base;
-    if (n > usual / 4) n = usual / 4;   // at least four blocks a workgroup
-    if (n < 1) n = 1;
-    const int64_t len = (usual + n - 1) / n;
-    int64_t f = (most + len - 1) / len;
-    r.rest = (int)n;
-    r.first = (int)(f < n ? n : f > 256 ? 256 : f);
+    const int64_t all = s.Sq > 0 ? (s.Sq + 63) / 64 : 1, band = ((int64_t)kKeyTile + s.left + s.right + 62) / 64 + 1;
+    const int64_t most = s.G * all, usual = s.G * (band < all ? band : all);
+    const int64_t pairs = (int64_t)s.B * s.K, later = r.tiles - r.first_tiles;
+    // By estimated time in microseconds, measured on MI355X: two workgroups that share a CU take 0.9 (heads of 64) or 1.95 (of
+    // 128) each for a block of 64 queries, one alone 1.35 times that, and a workgroup starts within the time of two blocks; the
+    // launch that adds up shares takes 4, its sums 4 MB a microsecond.
+    const double block = s.D == 64 ? 0.9 : 1.95, share = 2.0 * kKeyTile * s.D * 4 * 2 / 4e6;
+    double least = 1e300;
+    r.first = r.rest = 1;
+    for (int64_t n = 1; n <= 64 && (n == 1 || usual / n >= 4); ++n) {   // at least four blocks a workgroup
+        const int64_t len = (usual + n - 1) / n;
+        for (int64_t f = r.first_tiles > 0 ? n : 1; f <= 256 && (f == n || f == 1 || most / f >= 4); ++f) {
+            const int64_t flen = (most + f - 1) / f;
+            const int64_t wgs = pairs * (r.first_tiles * f + later * n);
+            const double turns = wgs <= 256 ? 1.35 : wgs <= 512 ? 2.0 : (double)wgs / 256.0 + 0.5;
+            double t = turns * ((double)(r.first_tiles > 0 && flen > len ? flen : len) + 2.0) * block;
+            if (n > 1) t += 4.0 + (double)wgs * share;
+            else if (r.first_tiles > 0 && f > 1) t += 4.0 + (double)(pairs * r.first_tiles * f) * share;
+            if (t < least) {
+                least = t;
+                r.rest = (int)n;
+                r.first = (int)f;
+            }
+            if (r.first_tiles == 0) break;
+        }
+    }
     return r;
 }
 struct KeyItem {

@@ -57,12 +57,44 @@ __device__ __forceinline__ typename Vec<T>::x4 ld_tr(const char* t, int k0, int 
     return __builtin_bit_cast(typename Vec<T>::x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                        (__attribute__((address_space(3))) v4s*)(lds_ptr_t)a));
 }
-// rows k0 .. + 3 and k0 + 8 .. + 11: the eight rows that a 32 x 32 product's result holds in two groups of four
-template <class T, int R = BLK>
-__device__ __forceinline__ typename Vec<T>::x8 ld_tr8(const char* t, int k0, int n0, int lane) {
-    const typename Vec<T>::x4 a = ld_tr<T, R>(t, k0, n0, lane), b = ld_tr<T, R>(t, k0 + 8, n0, lane);
-    return typename Vec<T>::x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+// A lane's places in a tile, the same in every tile: eight addresses that a kernel works out once; the rest of a read's
+// address is a constant.
+//   row  chunk 2 (ks % 4) + lane / 32 of row lane % 32: eight dims of the row, for K step ks of a product
+//   tr   transposed: lane j of a 16-lane group gets four rows' column n0 + j; rows 4 (lane / 32) + 8 u .. + 3, u = 0, 1,
+//        are the rows that a 32 x 32 product's result holds; columns 32 i + 16 ((lane / 16) % 2) .. + 15
+struct LaneOff {
+    uint32_t row[4], tr[2][2];
+    __device__ __forceinline__ void init(int lane) {
+        const int c32 = lane & 31, hl = lane >> 5, j = lane & 15;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) row[k] = (uint32_t)(c32 * 128 + (((2 * k + hl) ^ swz(c32)) << 4));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = 4 * hl + 8 * u + (j >> 2), n = 32 * i + 16 * ((lane >> 4) & 1) + 4 * (j & 3);
+                tr[i][u] = (uint32_t)(r * 128 + (((n >> 3) ^ swz(r)) << 4) + (n & 7) * 2);
+            }
+    }
+};
+// the fragment of rows 32 h .. 32 h + 31 and K step ks of the tile of R rows at LDS address t
+template <class T, int R>
+__device__ __forceinline__ typename Vec<T>::x8 rd_row(uint32_t t, const LaneOff& o, int h, int ks) {
+    return *(const __attribute__((address_space(3))) typename Vec<T>::x8*)(uintptr_t)(t + o.row[ks & 3] +
+                                                                                    (uint32_t)((ks >> 2) * R * 128 + h * 4096));
 }
+// the transposed fragment of rows 16 m .. 16 m + 15 and columns 32 i .. 32 i + 31
+template <class T, int R>
+__device__ __forceinline__ typename Vec<T>::x8 rd_tr(uint32_t t, const LaneOff& o, int m, int i) {
+    typename Vec<T>::x4 q[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        q[u] = __builtin_bit_cast(typename Vec<T>::x4,
+                                  __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(uintptr_t)(
+                                      t + o.tr[i & 1][u] + (uint32_t)((i >> 1) * R * 128 + m * 2048))));
+    return typename Vec<T>::x8{q[0][0], q[0][1], q[0][2], q[0][3], q[1][0], q[1][1], q[1][2], q[1][3]};
+}
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_ptr_t)p; }
 
 __device__ __forceinline__ u32x4 buffer_rsrc(const void* base, uint32_t bytes) {
     const unsigned long long a = (unsigned long long)(uintptr_t)base;
@@ -83,21 +115,20 @@ __device__ __forceinline__ void dma16(const u32x4& rs, uint32_t voff, uint32_t l
 // ROWS rows from row0 on of a tensor of n rows `pitch` elements apart, D elements each, into a tile, by NT threads
 // (thread tid of wave `wave` of them). Slot s of a sub-tile is row s / 8, chunk (s % 8) ^ swz(row).
 template <int D, int ROWS, int NT>
-__device__ __forceinline__ void tile_dma(const void* base, int64_t pitch, int n, int row0, const char* tile, int tid,
+__device__ __forceinline__ void tile_dma(const void* base, int64_t pitch, int n, int row0, uint32_t tile, int tid,
                                          int wave) {
     constexpr int SUBS = D / 64, PER = ROWS * 8 / NT;   // loads a thread makes for a sub-tile
     static_assert(ROWS * 8 % NT == 0, "whole rounds of loads");
     const int valid = max(0, min(ROWS, n - row0));
     const u32x4 rs = buffer_rsrc(static_cast<const char*>(base) + (int64_t)row0 * pitch * 2,
                                  valid > 0 ? (uint32_t)(((valid - 1) * pitch + D) * 2) : 0u);
-    const uint32_t dst = (uint32_t)(uintptr_t)(lds_ptr_t)tile;
 #pragma unroll
     for (int u = 0; u < SUBS; ++u)
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             const int sl = q * NT + tid, row = sl >> 3, kc = (sl & 7) ^ swz(row);
             const uint32_t voff = (uint32_t)row * (uint32_t)(pitch * 2) + (uint32_t)(u * 128 + kc * 16);
-            dma16(rs, voff, __builtin_amdgcn_readfirstlane(dst + (uint32_t)(u * ROWS * 128 + (q * NT + wave * 64) * 16)));
+            dma16(rs, voff, __builtin_amdgcn_readfirstlane(tile + (uint32_t)(u * ROWS * 128 + (q * NT + wave * 64) * 16)));
         }
 }
 // 64 floats v[i0 .. i0 + 63] (zeros past n) into LDS, by one wave
@@ -108,7 +139,6 @@ __device__ __forceinline__ void vec_dma(const float* v, int n, int i0, const flo
     asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(m0), "v"((uint32_t)lane * 4), "s"(rs)
                  : "memory");
 }
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }   // vmcnt(0)
 // all but the last N of this wave's loads have landed, and its earlier LDS reads have returned: memory that only this
 // wave uses is ordered by this alone
 template <int N>
@@ -117,14 +147,58 @@ __device__ __forceinline__ void wait_own_loads() {
     __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (0 << 8) | ((N >> 4) << 14));
     asm volatile("" ::: "memory");
 }
-// this wave's loads have landed; then a barrier makes every wave's visible
-__device__ __forceinline__ void wait_loads_all() {
-    wait_loads();
+// The tiles of a workgroup run through STAGES pieces of LDS, LOADS loads a wave and tile. Before tile i is used: its loads
+// have landed, `later` tiles' (at most STAGES - 2) that were issued after it may be under way; then a barrier makes
+// every wave's visible, and says that every wave is done with the tile before, whose piece the next loads overwrite.
+template <int LATER, int LOADS>
+__device__ __forceinline__ void wait_tile(int later) {
+    static_assert(LATER * LOADS < 64, "vmcnt range");
+    if constexpr (LATER > 0) {
+        if (later < LATER) return wait_tile<LATER - 1, LOADS>(later);
+    }
+    constexpr int N = LATER * LOADS;
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
     asm volatile("s_barrier" ::: "memory");
+}
+
+// this wave's LDS writes are done; then a barrier, past which the other waves see them (loads stay under way)
+__device__ __forceinline__ void wait_lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+// The sums of a loop, after it, as the registers that the loop used. Without this the compiler takes the vectors apart for
+// the code behind the loop and copies every element to a register of its own in every round.
+template <int N>
+__device__ __forceinline__ void settle(f32x16 (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
 // 2^x on the hardware's exp unit: results below 2^-126 flush to zero
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Visible bits. A lane holds rows 8 (v / 4) + 4 (lane / 32) + v % 4, v = 0 .. 15, of each 32 rows of a tile: bit
+// 8 (v / 4) + v % 4 of a 32-bit word once that is shifted by 4 (lane / 32). Two instructions an element: the bit spread over a
+// word, and a select by it.
+__device__ __forceinline__ unsigned long long bits_below(int n) {
+    return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+}
+struct Bits {
+    uint32_t w[2];
+    // rows r0 .. r0 + 63: those of lo .. lo + n - 1, and those below first
+    __device__ __forceinline__ void set(int r0, int lo, int n, int first, int lane) {
+        const unsigned long long m = (bits_below(lo + n - r0) & ~bits_below(lo - r0)) | bits_below(first - r0);
+        const int sh = 4 * (lane >> 5);
+        w[0] = (uint32_t)m >> sh;
+        w[1] = (uint32_t)(m >> 32) >> sh;
+    }
+    __device__ __forceinline__ uint32_t spread(int h, int v) const {   // all ones where visible
+        return (uint32_t)__builtin_amdgcn_sbfe((int)w[h], 8 * (v >> 2) + (v & 3), 1);
+    }
+};
+__device__ __forceinline__ float keep(float x, uint32_t m) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & m); }
+__device__ __forceinline__ float keep_or_none(float x, uint32_t m) {   // -inf where hidden
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & m) | (~m & 0xFF800000u));
+}
 
 // a sample's lengths, in range
 __device__ __forceinline__ int clamp_len(const int32_t* len, int b, int most) {

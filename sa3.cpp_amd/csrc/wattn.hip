@@ -48,29 +48,40 @@ struct Running {
     }
     // R keys kbase .. of the tiles kt, vt (this query's row sees of them what `see` says; all: every key)
     template <int R>
-    __device__ __forceinline__ void block(const char* kt, const char* vt, const x8 (&qf)[D / 16], int kbase, const Seen& see,
-                                          bool all, float c, int lane) {
+    __device__ __forceinline__ void block(uint32_t kt, uint32_t vt, const LaneOff& off, const x8 (&qf)[D / 16], int kbase,
+                                          const Seen& see, bool all, float c, int lane) {
         constexpr int HALVES = R / 32;
-        const int hl = lane >> 5, c32 = lane & 31;
+        // Every fragment of K first, then the products, the two halves in turn: left to itself the compiler reads each
+        // fragment right before its product and waits for it there.
         f32x16 s[HALVES];
+        x8 kf[HALVES][D / 16];
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
+        for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) kf[h][ks] = rd_row<T, R>(kt, off, h, ks);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[h][v] = 0.f;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-                s[h] = Vec<T>::mfma(ld_row<T, R>(kt, 32 * h + c32, 2 * ks + hl), qf[ks], s[h]);
-        }
+        for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) s[h] = Vec<T>::mfma(kf[h][ks], qf[ks], s[h]);
+        // the fragments of V arrive while the weights are worked out
+        x8 vf[HALVES * 2][D / 32];
+#pragma unroll
+        for (int j = 0; j < HALVES * 2; ++j)
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) vf[j][i] = rd_tr<T, R>(vt, off, j, i);
+        __builtin_amdgcn_sched_barrier(0);
         if (!all) {   // (wave-uniform)
-            const int j0 = kbase + 4 * hl;
+            Bits bits;
+            bits.set(kbase, see.lo, see.n, see.first, lane);
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int j = j0 + 32 * h + 8 * (v >> 2) + (v & 3);
-                    const bool ok = (unsigned)(j - see.lo) < (unsigned)see.n || j < see.first;
-                    s[h][v] = ok ? s[h][v] : -INFINITY;
-                }
+                for (int v = 0; v < 16; ++v) s[h][v] = keep_or_none(s[h][v], bits.spread(h, v));
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -105,18 +116,15 @@ struct Running {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i)
-                    o[i] = Vec<T>::mfma(ld_tr8<T, R>(vt, 32 * h + 16 * j + 4 * hl, 32 * i + 16 * ((lane >> 4) & 1), lane), p[h][j],
-                                        o[i]);
+                for (int i = 0; i < D / 32; ++i) o[i] = Vec<T>::mfma(vf[2 * h + j][i], p[h][j], o[i]);
     }
 };
 
-// 128 queries of one head a workgroup, 32 a wave; tiles of 64 keys, two stages: the loads of block i + 1 run while
-// block i is computed.
+// 128 queries of one head a workgroup, 32 a wave; tiles of 64 keys, whose loads run STAGES - 1 tiles ahead.
 template <class T, int D>
 __global__ __launch_bounds__(kThreads, 2) void wattn_fwd_kernel(FwdArgs a) {
-    constexpr int TILE = BLK * D * 2;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * TILE];
+    constexpr int TILE = BLK * D * 2, STAGES = 2, LOADS = 2 * (D / 64) * (BLK * 8 / kThreads);
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * TILE];
     const AttnShape& s = a.s;
     const Place pl = place(s, (s.Sq + 127) / 128);
     const int nq = clamp_len(s.q_len, pl.b, s.Sq), nk = clamp_len(s.k_len, pl.b, s.Sk), off = nk - nq;
@@ -143,23 +151,24 @@ __global__ __launch_bounds__(kThreads, 2) void wattn_fwd_kernel(FwdArgs a) {
 
     Running<T, D> run;
     run.clear();
+    LaneOff at;
+    at.init(lane);
+    const uint32_t base = lds_addr(lds);
     auto issue = [&](int st, int i) {
         const int row0 = key_block(kb, i) * BLK;
-        tile_dma<D, BLK, kThreads>(kp, s.ks[1], nk, row0, lds + st * 2 * TILE, tid, wave);
-        tile_dma<D, BLK, kThreads>(vp, s.vs[1], nk, row0, lds + st * 2 * TILE + TILE, tid, wave);
+        tile_dma<D, BLK, kThreads>(kp, s.ks[1], nk, row0, base + st * 2 * TILE, tid, wave);
+        tile_dma<D, BLK, kThreads>(vp, s.vs[1], nk, row0, base + st * 2 * TILE + TILE, tid, wave);
     };
-    if (kb.count > 0) issue(0, 0);
-    for (int i = 0; i < kb.count; ++i) {
-        const int st = i & 1;
-        wait_loads_all();   // block i landed; every wave is done with block i - 1 (the other stage)
-        if (i + 1 < kb.count) issue(st ^ 1, i + 1);
+    for (int i = 0; i < STAGES - 1 && i < kb.count; ++i) issue(i, i);
+    for (int i = 0, st = 0; i < kb.count; ++i, st = st + 1 < STAGES ? st + 1 : 0) {
+        wait_tile<STAGES - 2, LOADS>(kb.count - 1 - i);
+        if (i + STAGES - 1 < kb.count) issue(st > 0 ? st - 1 : STAGES - 1, i + STAGES - 1);
         const int k0 = key_block(kb, i) * BLK, k1 = k0 + BLK - 1;
-        if (q0w >= nq) continue;
-        const bool near = k1 >= sa.lo && k0 < sb.lo + sb.n;
-        if (!near && k0 >= sb.first) continue;   // nothing of this block for this wave
+        const bool near = q0w < nq && ((k1 >= sa.lo && k0 < sb.lo + sb.n) || k0 < sb.first);
         const bool all = q0w + QW <= nq && ((k0 >= sb.lo && k1 < sa.lo + sa.n) || k1 < sa.first);
-        run.template block<BLK>(lds + st * 2 * TILE, lds + st * 2 * TILE + TILE, qf, k0, see, all, c, lane);
+        if (near) run.template block<BLK>(base + st * 2 * TILE, base + st * 2 * TILE + TILE, at, qf, k0, see, all, c, lane);
     }
+    settle(run.o);
     if (q >= nq) return;
     const float l = run.l + __shfl_xor(run.l, 32, 64);
     if (a.lse && hl == 0) a.lse[((int64_t)pl.b * s.H + pl.h) * s.Sq + q] = run.m + log2f(l);
@@ -212,7 +221,9 @@ __global__ __launch_bounds__(kThreads) void wattn_split_kernel(FwdArgs a) {
 
     Running<T, D> run;
     run.clear();
-    char* mine = lds + wave * 4 * TILE;
+    LaneOff at;
+    at.init(lane);
+    const uint32_t mine = lds_addr(lds) + wave * 4 * TILE;
     auto issue = [&](int st, int i) {
         const int row0 = key_block(kb, i) * R;
         tile_dma<D, R, 64>(kp, s.ks[1], nk, row0, mine + st * 2 * TILE, lane, 0);
@@ -231,8 +242,9 @@ __global__ __launch_bounds__(kThreads) void wattn_split_kernel(FwdArgs a) {
         }
         const int k0 = key_block(kb, i) * R, k1 = k0 + R - 1;
         const bool all = r0 + R <= rows && ((k0 >= sb.lo && k1 < sa.lo + sa.n) || k1 < sa.first);
-        run.template block<R>(mine + st * 2 * TILE, mine + st * 2 * TILE + TILE, qf, k0, see, all, c, lane);
+        run.template block<R>(mine + st * 2 * TILE, mine + st * 2 * TILE + TILE, at, qf, k0, see, all, c, lane);
     }
+    settle(run.o);
     // join the waves: common maximum, then the sums of the rescaled o and l in wave order
     const float l = run.l + __shfl_xor(run.l, 32, 64);
     if (hl == 0) {

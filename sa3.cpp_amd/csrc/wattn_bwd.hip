@@ -8,6 +8,7 @@
 // By queries: S^T = K Q^T and dP^T = V dO^T leave a lane with one query, dq^T += K^T dS^T reads K transposed.
 // By keys: S = Q K^T and dP = dO V^T leave it with one key, dv^T += dO^T P and dk^T += Q^T dS read dO and Q transposed.
 #include <algorithm>
+#include <type_traits>
 
 #include "wattn.h"
 
@@ -54,8 +55,8 @@ __device__ __forceinline__ void store_row(T* p, const f32x16 (&x)[D / 32], float
 template <class T, int D>
 __global__ __launch_bounds__(kThreads, 2) void wattn_dq_kernel(BwdArgs a) {
     typedef typename Vec<T>::x8 x8;
-    constexpr int TILE = BLK * D * 2;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * TILE];
+    constexpr int TILE = BLK * D * 2, STAGES = 2, LOADS = 2 * (D / 64) * (BLK * 8 / kThreads);
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * TILE];
     const AttnShape& s = a.s;
     const Place pl = place(s, (s.Sq + 127) / 128);
     const int nq = clamp_len(s.q_len, pl.b, s.Sq), nk = clamp_len(s.k_len, pl.b, s.Sk), off = nk - nq;
@@ -94,66 +95,76 @@ __global__ __launch_bounds__(kThreads, 2) void wattn_dq_kernel(BwdArgs a) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) dq[i][v] = 0.f;
 
+    LaneOff at;
+    at.init(lane);
+    const uint32_t base = lds_addr(lds);
     auto issue = [&](int st, int i) {
         const int row0 = key_block(kb, i) * BLK;
-        tile_dma<D, BLK, kThreads>(kp, s.ks[1], nk, row0, lds + st * 2 * TILE, tid, wave);
-        tile_dma<D, BLK, kThreads>(vp, s.vs[1], nk, row0, lds + st * 2 * TILE + TILE, tid, wave);
+        tile_dma<D, BLK, kThreads>(kp, s.ks[1], nk, row0, base + st * 2 * TILE, tid, wave);
+        tile_dma<D, BLK, kThreads>(vp, s.vs[1], nk, row0, base + st * 2 * TILE + TILE, tid, wave);
     };
-    if (kb.count > 0) issue(0, 0);
-    for (int it = 0; it < kb.count; ++it) {
-        const int st = it & 1;
-        wait_loads_all();   // block it landed; every wave is done with the other stage
-        if (it + 1 < kb.count) issue(st ^ 1, it + 1);
+    for (int it = 0; it < STAGES - 1 && it < kb.count; ++it) issue(it, it);
+    for (int it = 0, st = 0; it < kb.count; ++it, st = st + 1 < STAGES ? st + 1 : 0) {
+        wait_tile<STAGES - 2, LOADS>(kb.count - 1 - it);
+        if (it + STAGES - 1 < kb.count) issue(st > 0 ? st - 1 : STAGES - 1, it + STAGES - 1);
         const int k0 = key_block(kb, it) * BLK, k1 = k0 + BLK - 1;
-        if (q0w >= nq) continue;
-        const bool near = k1 >= sa.lo && k0 < sb.lo + sb.n;
-        if (!near && k0 >= sb.first) continue;
+        const bool near = (k1 >= sa.lo && k0 < sb.lo + sb.n) || k0 < sb.first;
+        if (q0w >= nq || !near) continue;   // this wave sees nothing of this block
         const bool all = q0w + 32 <= nq && ((k0 >= sb.lo && k1 < sa.lo + sa.n) || k1 < sa.first);
-        const char* kt = lds + st * 2 * TILE;
-        const char* vt = kt + TILE;
+        Bits bits;
+        bits.set(k0, see.lo, see.n, see.first, lane);
+        const uint32_t kt = base + st * 2 * TILE, vt = kt + TILE;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            // K and V fragments first, then their products in turn, then the transposed K while the weights are worked out
+            x8 kf[D / 16], vf[D / 16];
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+                kf[ks] = rd_row<T, BLK>(kt, at, h, ks);
+                vf[ks] = rd_row<T, BLK>(vt, at, h, ks);
+            }
             f32x16 sc, dp;
 #pragma unroll
             for (int v = 0; v < 16; ++v) sc[v] = dp[v] = 0.f;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
-                sc = Vec<T>::mfma(ld_row<T>(kt, 32 * h + c32, 2 * ks + hl), qf[ks], sc);
-                dp = Vec<T>::mfma(ld_row<T>(vt, 32 * h + c32, 2 * ks + hl), dof[ks], dp);
+                sc = Vec<T>::mfma(kf[ks], qf[ks], sc);
+                dp = Vec<T>::mfma(vf[ks], dof[ks], dp);
             }
+            x8 tf[2][D / 32];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) tf[j][i] = rd_tr<T, BLK>(kt, at, 2 * h + j, i);
+            __builtin_amdgcn_sched_barrier(0);
             x8 ds[2];
-            const int j0 = k0 + 32 * h + 4 * hl;
             if (all) {
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
                     ds[v >> 3][v & 7] = (T)(ex2(__builtin_fmaf(sc[v], c, -lse)) * (dp[v] - delta));
             } else {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int j = j0 + 8 * (v >> 2) + (v & 3);
-                    const bool ok = (unsigned)(j - see.lo) < (unsigned)see.n || j < see.first;
-                    const float x = ex2(__builtin_fmaf(sc[v], c, -lse)) * (dp[v] - delta);
-                    ds[v >> 3][v & 7] = (T)(ok ? x : 0.f);   // (a row that sees nothing has lse = -inf)
-                }
+                for (int v = 0; v < 16; ++v)   // (a row that sees nothing has lse = -inf)
+                    ds[v >> 3][v & 7] = (T)keep(ex2(__builtin_fmaf(sc[v], c, -lse)) * (dp[v] - delta), bits.spread(h, v));
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i)
-                    dq[i] = Vec<T>::mfma(ld_tr8<T>(kt, 32 * h + 16 * j + 4 * hl, 32 * i + 16 * ((lane >> 4) & 1), lane), ds[j],
-                                         dq[i]);
+                for (int i = 0; i < D / 32; ++i) dq[i] = Vec<T>::mfma(tf[j][i], ds[j], dq[i]);
         }
     }
+    settle(dq);
     if (q < nq) store_row<T, D>(static_cast<T*>(a.dq) + qoff, dq, s.scale, hl);
 }
 
 // 128 keys of one key/value head a workgroup, 32 a wave; tiles of 64 queries' q and dO with their lse and delta.
 template <class T, int D>
-__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void wattn_dkdv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void wattn_dkdv_kernel(BwdArgs a) {
     typedef typename Vec<T>::x8 x8;
-    constexpr int TILE = BLK * D * 2;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * TILE];
-    __shared__ __attribute__((aligned(16))) float vec[2][2][BLK];   // lse, delta
+    constexpr int TILE = BLK * D * 2, STAGES = 2, LOADS = 2 * (D / 64) * (BLK * 8 / kThreads) + 1;
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * TILE];
+    __shared__ __attribute__((aligned(16))) float vec[STAGES][2][BLK];   // lse, delta
     const AttnShape& s = a.s;
     const int BK = s.B * s.K, bk = blockIdx.x % BK, item = blockIdx.x / BK;
     const int b = bk / s.K, kh = bk - b * s.K;
@@ -194,67 +205,101 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void wattn_dkdv_kernel(B
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int v = 0; v < 16; ++v) dk[i][v] = dv[i][v] = 0.f;
+    LaneOff at;
+    at.init(lane);
+    const uint32_t base = lds_addr(lds);
     auto issue = [&](int st, int it) {
         const int g = it / nqb, row0 = (qb_lo + it - g * nqb) * BLK, h = kh * s.G + g;
         const T* qp = static_cast<const T*>(a.q) + b * s.qs[0] + h * s.qs[2];
         const T* op = static_cast<const T*>(a.dO) + b * s.os[0] + h * s.os[2];
-        tile_dma<D, BLK, kThreads>(qp, s.qs[1], nq, row0, lds + st * 2 * TILE, tid, wave);
-        tile_dma<D, BLK, kThreads>(op, s.os[1], nq, row0, lds + st * 2 * TILE + TILE, tid, wave);
+        tile_dma<D, BLK, kThreads>(qp, s.qs[1], nq, row0, base + st * 2 * TILE, tid, wave);
+        tile_dma<D, BLK, kThreads>(op, s.os[1], nq, row0, base + st * 2 * TILE + TILE, tid, wave);
         const int64_t r = ((int64_t)b * s.H + h) * s.Sq;
-        if (wave == 0) vec_dma(a.lse + r, nq, row0, vec[st][0], lane);
-        if (wave == 1) vec_dma(a.delta + r, nq, row0, vec[st][1], lane);
+        // (two waves load each, the same values, so that every wave has the same number of loads under way)
+        vec_dma((wave & 1 ? a.delta : a.lse) + r, nq, row0, vec[st][wave & 1], lane);
     };
-    if (lo < hi) issue(0, lo);
-    for (int it = lo; it < hi; ++it) {
-        const int st = (it - lo) & 1;
-        wait_loads_all();   // block it landed; every wave is done with the other stage
-        if (it + 1 < hi) issue(st ^ 1, it + 1);
+    for (int it = 0; it < STAGES - 1 && lo + it < hi; ++it) issue(it, lo + it);
+    for (int it = lo, st = 0; it < hi; ++it, st = st + 1 < STAGES ? st + 1 : 0) {
+        wait_tile<STAGES - 2, LOADS>(hi - 1 - it);
+        if (it + STAGES - 1 < hi) issue(st > 0 ? st - 1 : STAGES - 1, it + STAGES - 1);
         const int q0 = (qb_lo + it % nqb) * BLK, q1 = q0 + BLK - 1;
-        if (k0w >= nk || q0 > reach.hi || q1 < reach.lo) continue;   // nothing of this block for this wave
+        if (k0w >= nk || q0 > reach.hi || q1 < reach.lo) continue;   // nothing of this block sees the wave's keys
         const bool all = q0 >= full_lo && q1 <= full_hi;
-        const char* qt = lds + st * 2 * TILE;
-        const char* ot = qt + TILE;
-#pragma unroll
+        Bits bits;
+        bits.set(q0, mine.lo, (int)mine_n, 0, lane);
+        const uint32_t qt = base + st * 2 * TILE, ot = qt + TILE;
+#pragma unroll 1   // (unrolled, more sums are alive than a lane's 256 registers hold)
         for (int h = 0; h < 2; ++h) {
+            // fragments in batches, each read while the batch before is multiplied
+            constexpr int FB = D == 64 ? 4 : 1, NB = D / 16 / FB;   // FB fragments of q and of dO a batch
             f32x16 sc, dp;
 #pragma unroll
             for (int v = 0; v < 16; ++v) sc[v] = dp[v] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-                sc = Vec<T>::mfma(ld_row<T>(qt, 32 * h + c32, 2 * ks + hl), kf[ks], sc);
-                dp = Vec<T>::mfma(ld_row<T>(ot, 32 * h + c32, 2 * ks + hl), vf[ks], dp);
+            for (int nb = 0; nb < NB; ++nb) {
+                x8 qf[FB], of[FB];
+#pragma unroll
+                for (int k4 = 0; k4 < FB; ++k4) {
+                    qf[k4] = rd_row<T, BLK>(qt, at, h, FB * nb + k4);
+                    of[k4] = rd_row<T, BLK>(ot, at, h, FB * nb + k4);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k4 = 0; k4 < FB; ++k4) {
+                    sc = Vec<T>::mfma(qf[k4], kf[FB * nb + k4], sc);
+                    dp = Vec<T>::mfma(of[k4], vf[FB * nb + k4], dp);
+                }
             }
             x8 p[2], ds[2];
+            const uint32_t word = h ? bits.w[1] : bits.w[0];
+            // MASK 0: every pair visible, 1: by the bits, 2: by the bits if not all are. For heads of 64 the code is written out
+            // for both; for heads of 128 that spills sums, and a branch an element costs less.
+            auto weights = [&](auto mask) {
+                constexpr int MASK = decltype(mask)::value;
 #pragma unroll
-            for (int vg = 0; vg < 4; ++vg) {
-                const int i0 = 32 * h + 8 * vg + 4 * hl;
-                const float4 l4 = *reinterpret_cast<const float4*>(&vec[st][0][i0]);
-                const float4 d4 = *reinterpret_cast<const float4*>(&vec[st][1][i0]);
-                const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+                for (int vg = 0; vg < 4; ++vg) {
+                    const float4 l4 = *reinterpret_cast<const float4*>(&vec[st][0][32 * h + 8 * vg + 4 * hl]);
+                    const float4 d4 = *reinterpret_cast<const float4*>(&vec[st][1][32 * h + 8 * vg + 4 * hl]);
+                    const float ls[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int v = 4 * vg + u;
-                    float w = ex2(__builtin_fmaf(sc[v], c, -ls[u]));
-                    float x = w * (dp[v] - dl[u]);
-                    if (!all) {   // (wave-uniform)
-                        const bool ok = (unsigned)(q0 + i0 + u - mine.lo) < mine_n;
-                        w = ok ? w : 0.f;
-                        x = ok ? x : 0.f;
+                    for (int u = 0; u < 4; ++u) {
+                        const int v = 4 * vg + u;
+                        float w = ex2(__builtin_fmaf(sc[v], c, -ls[u]));
+                        float x = w * (dp[v] - dl[u]);
+                        if (MASK == 1 || (MASK == 2 && !all)) {
+                            const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)word, 8 * vg + u, 1);
+                            w = keep(w, m);
+                            x = keep(x, m);
+                        }
+                        p[v >> 3][v & 7] = (T)w;
+                        ds[v >> 3][v & 7] = (T)x;
                     }
-                    p[v >> 3][v & 7] = (T)w;
-                    ds[v >> 3][v & 7] = (T)x;
                 }
+            };
+            if constexpr (D == 128) {
+                weights(std::integral_constant<int, 2>{});
+            } else {
+                if (all) weights(std::integral_constant<int, 0>{});
+                else weights(std::integral_constant<int, 1>{});
             }
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j) {
+                x8 tf[D / 32];
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const int r0 = 32 * h + 16 * j + 4 * hl, n0 = 32 * i + 16 * ((lane >> 4) & 1);
-                    dv[i] = Vec<T>::mfma(ld_tr8<T>(ot, r0, n0, lane), p[j], dv[i]);
-                    dk[i] = Vec<T>::mfma(ld_tr8<T>(qt, r0, n0, lane), ds[j], dk[i]);
-                }
+                for (int i = 0; i < D / 32; ++i) tf[i] = rd_tr<T, BLK>(ot, at, 2 * h + j, i);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) dv[i] = Vec<T>::mfma(tf[i], p[j], dv[i]);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) tf[i] = rd_tr<T, BLK>(qt, at, 2 * h + j, i);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) dk[i] = Vec<T>::mfma(tf[i], ds[j], dk[i]);
+            }
         }
     }
+    settle(dk);
+    settle(dv);
     if (key >= nk) return;
     if (ki.splits == 1) {
         store_row<T, D>(static_cast<T*>(a.dk) + koff, dk, s.scale, hl);
