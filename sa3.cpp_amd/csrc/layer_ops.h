@@ -134,9 +134,9 @@ inline const char* attn_check(const sa3k_window_attn* d, const AttnPtrs& p, bool
     if (bwd && (!rows_apart(d->q_stride, nq, d->head_dim) || !rows_apart(d->k_stride, nk, d->head_dim) ||
                 !rows_apart(d->v_stride, nk, d->head_dim)))
         return "the rows of q, k or v overlap, and their gradients have the same layout";
-    // workgroups of 256 threads, 64 rows or keys each at the least, in one grid dimension
+    // one grid dimension, of fewer than 2^32 threads: at the most 16 a row
     const int64_t most = (d->q_tokens > d->k_tokens ? d->q_tokens : d->k_tokens) / 64 + 1;
-    if (most * d->batch * d->heads >= ((int64_t)1 << 23)) {
+    if (most * d->batch * d->heads >= ((int64_t)1 << 21)) {
         *code = SA3K_ERR_UNSUPPORTED;
         return "batch x heads x tokens is too large for one launch";
     }

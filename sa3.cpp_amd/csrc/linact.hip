@@ -174,18 +174,25 @@ struct Operand {
                 off[q] = (uint32_t)(s >> 3) * row_bytes + (uint32_t)(kc * 16);
         }
     }
-    // tile t of K, `left` of K in range from its start on, into LDS at lds_addr
-    __device__ __forceinline__ void issue(int64_t t, int64_t left, uint32_t lds_addr, int wave) const {
-        const int k = (int)min((int64_t)64, left);
+    // the descriptor of tile t of K, `left` of K in range from its start on (none: every load gives zeros)
+    __device__ __forceinline__ u32x4 tile(int64_t t, int64_t left) const {
+        const int k = (int)max((int64_t)0, min((int64_t)64, left));
         // The last row in range ends the descriptor: rows past it are zeros. Rows are whole chunks of 8 elements, or padded to
         // that with zeros (a descriptor that ended inside a chunk would drop the dword that crosses its end).
-        const uint32_t bytes = KMAJOR ? (uint32_t)(k - 1) * row_bytes + (uint32_t)((rows + 7) & ~7) * 2
-                                      : (uint32_t)(rows - 1) * row_bytes + (uint32_t)((k + 7) & ~7) * 2;
-        const u32x4 rs = buffer_rsrc(base + t * step, bytes);
-        const bool none = !KMAJOR && kc * 8 >= k;   // a chunk past K lies in the next row: kept out
+        const uint32_t bytes = k == 0 ? 0u
+                               : KMAJOR ? (uint32_t)(k - 1) * row_bytes + (uint32_t)((rows + 7) & ~7) * 2
+                                        : (uint32_t)(rows - 1) * row_bytes + (uint32_t)((k + 7) & ~7) * 2;
+        return buffer_rsrc(base + t * step, bytes);
+    }
+    // load q of tile t into the LDS piece at lds_addr
+    __device__ __forceinline__ void load(const u32x4& rs, int q, int64_t left, uint32_t lds_addr, int wave) const {
+        const bool none = !KMAJOR && kc * 8 >= left;   // a chunk past K lies in the next row: kept out
+        dma16(rs, none ? 0xFFFFFFF0u : off[q], __builtin_amdgcn_readfirstlane(lds_addr + (uint32_t)((q * NT + wave * 64) * 16)));
+    }
+    __device__ __forceinline__ void issue(int64_t t, int64_t left, uint32_t lds_addr, int wave) const {
+        const u32x4 rs = tile(t, left);
 #pragma unroll
-        for (int q = 0; q < PER; ++q)
-            dma16(rs, none ? 0xFFFFFFF0u : off[q], __builtin_amdgcn_readfirstlane(lds_addr + (uint32_t)((q * NT + wave * 64) * 16)));
+        for (int q = 0; q < PER; ++q) load(rs, q, left, lds_addr, wave);
     }
     // the operand of K step ks (16 of K) for rows r0 .. r0 + 31 of the tile
     static __device__ __forceinline__ x8 frag(const char* t, int r0, int ks, int lane) {
@@ -201,32 +208,68 @@ struct Operand {
     }
 };
 
-// Square tiles of EDGE. 256: eight waves of 64 x 128, one workgroup a CU; 128: four waves of 64 x 64, two.
-template <class T, int EDGE, bool AK, bool BK, bool FWD>
-__global__ __launch_bounds__(EDGE * 2, 2) void prod_tile_kernel(GemmArgs a) {
-    typedef typename Vec<T>::x8 x8;
-    constexpr int NT = EDGE * 2, WM = EDGE / 64, WTN = EDGE == 256 ? 128 : 64, FM = 2, FN = WTN / 32;
-    constexpr int OPB = EDGE * 128, STAGE = 2 * OPB;
-    constexpr int ER = 64, EROW = EDGE + 8;
-    static_assert(ER * EROW * 4 <= 2 * STAGE, "staged rows fit the stages' memory");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-    // Workgroups go out to the 8 XCDs in turn: XCD c takes the run [c n / 8, (c + 1) n / 8) of the items in (split, raster)
-    // order, in groups of eight rows of tiles, so that tiles that share operands run on one XCD and share its L2.
+// Which tile a workgroup takes, in tiles of EDGE: workgroups go out to the 8 XCDs in turn; XCD c takes the run
+// [c n / 8, (c + 1) n / 8) of the items in (split, raster) order, in groups of eight rows of tiles, so that tiles that share
+// operands run on one XCD and share its L2.
+struct TilePlace {
+    int z;
+    int64_t m0, n0;
+    bool none;
+};
+template <int EDGE>
+__device__ __forceinline__ TilePlace tile_place(const GemmArgs& a) {
     const int tiles_m = (int)((a.M + EDGE - 1) / EDGE), tiles_n = (int)((a.N + EDGE - 1) / EDGE);
     const int nwg = gridDim.x, L = blockIdx.x + nwg * blockIdx.y;
     const int item = (L & 7) * ((nwg * (int)gridDim.y) >> 3) + (L >> 3);
-    const int z = __builtin_amdgcn_readfirstlane(item / nwg), bid = __builtin_amdgcn_readfirstlane(item - z * nwg);
-    if (bid >= tiles_m * tiles_n) return;
+    TilePlace p;
+    p.z = __builtin_amdgcn_readfirstlane(item / nwg);
+    const int bid = __builtin_amdgcn_readfirstlane(item - p.z * nwg);
+    p.none = bid >= tiles_m * tiles_n;
     const int group = bid / (8 * tiles_n), gsz = min(tiles_m - group * 8, 8), in_g = bid - group * 8 * tiles_n;
-    const int64_t m0 = (int64_t)(group * 8 + in_g % gsz) * EDGE, n0 = (int64_t)(in_g / gsz) * EDGE;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm0 = (wave % WM) * 64, wn0 = (wave / WM) * WTN;
+    p.m0 = p.none ? 0 : (int64_t)(group * 8 + in_g % gsz) * EDGE;
+    p.n0 = p.none ? 0 : (int64_t)(in_g / gsz) * EDGE;
+    return p;
+}
 
+// Rows rb .. rb + 63 of a tile's sums, staged in LDS as f32: a thread finishes 8 columns of a row.
+template <class T, bool FWD, int EDGE, int NT, int EROW>
+__device__ __forceinline__ void finish_rows(const GemmArgs& a, const TilePlace& tp, const float* st, int rb, int tid) {
+    constexpr int CPR = EDGE / 8;   // threads a row
+    const int cq = (tid % CPR) * 8;
+    const int64_t n = tp.n0 + cq;
+    for (int r = tid / CPR; r < 64; r += NT / CPR) {
+        const int64_t m = tp.m0 + rb + r;
+        if (m >= a.M || n >= a.N) break;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(st + r * EROW + cq + e);
+            v[e] = x.x;
+            v[e + 1] = x.y;
+            v[e + 2] = x.z;
+            v[e + 3] = x.w;
+        }
+        if (a.part) store8(a.part + ((int64_t)tp.z * a.M + m) * a.pitch, n, a.pitch, v);
+        else finish8<T, FWD>(a, m, n, v);
+    }
+}
+
+// Tiles of 256 x 256: eight waves of 64 x 128, one workgroup a CU.
+template <class T, bool AK, bool BK, bool FWD>
+__global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    constexpr int EDGE = 256, NT = 512, FM = 2, FN = 4, OPB = EDGE * 128, STAGE = 2 * OPB, EROW = EDGE + 8;
+    static_assert(64 * EROW * 4 <= 2 * STAGE, "staged rows fit the stages' memory");
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+    const TilePlace tp = tile_place<EDGE>(a);
+    if (tp.none) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm0 = (wave & 3) * 64, wn0 = (wave >> 2) * 128;
     Operand<T, EDGE, NT, AK> A;
     Operand<T, EDGE, NT, BK> B;
-    A.init(a.A, a.lda, m0, a.M, tid);
-    B.init(a.B, a.ldb, n0, a.N, tid);
-    const int64_t KT = (a.K + 63) / 64, t0 = (int64_t)z * a.per, t1 = min(KT, t0 + a.per);
+    A.init(a.A, a.lda, tp.m0, a.M, tid);
+    B.init(a.B, a.ldb, tp.n0, a.N, tid);
+    const int64_t KT = (a.K + 63) / 64, t0 = (int64_t)tp.z * a.per, t1 = min(KT, t0 + a.per);
     f32x16 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -239,52 +282,51 @@ __global__ __launch_bounds__(EDGE * 2, 2) void prod_tile_kernel(GemmArgs a) {
         A.issue(t, a.K - t * 64, lds0 + st * STAGE, wave);
         B.issue(t, a.K - t * 64, lds0 + st * STAGE + OPB, wave);
     };
-    auto compute = [&](const char* As) {
+    // Two groups of four waves, one of each on a SIMD, half a step apart: while one multiplies, the other reads its
+    // fragments. A step is 16 of K: fragments | barrier | eight products | barrier; the second group is one barrier late. The
+    // loads of tile t + 1 go out during the first steps of t, when both groups have read the last of t - 1, and have landed before
+    // the last step's first barrier, which comes before either group's first read of t + 1.
+    const bool late = wave >= 4;
+    if (t0 < t1) issue(0, t0);
+    wait_vmcnt<0>();
+    asm volatile("s_barrier" ::: "memory");
+    if (late) asm volatile("s_barrier" ::: "memory");
+    for (int64_t t = t0; t < t1; ++t) {
+        const int stage = (int)(t - t0) & 1;
+        const char* As = lds + stage * STAGE;
         const char* Bs = As + OPB;
-        x8 af[2][FM], bf[2][FN];
-        auto load = [&](int ks, int slot) {
 #pragma unroll
-            for (int i = 0; i < FM; ++i) af[slot][i] = Operand<T, EDGE, NT, AK>::frag(As, wm0 + 32 * i, ks, lane);
+        for (int ks = 0; ks < 4; ++ks) {
+            x8 af[FM], bf[FN];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) bf[slot][j] = Operand<T, EDGE, NT, BK>::frag(Bs, wn0 + 32 * j, ks, lane);
-        };
-        auto mma = [&](int slot) {
+            for (int j = 0; j < FN; ++j) bf[j] = Operand<T, EDGE, NT, BK>::frag(Bs, wn0 + 32 * j, ks, lane);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) af[i] = Operand<T, EDGE, NT, AK>::frag(As, wm0 + 32 * i, ks, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < t1) {
+                if (ks == 0) A.issue(t + 1, a.K - (t + 1) * 64, lds0 + (stage ^ 1) * STAGE, wave);
+                if (ks == 1) B.issue(t + 1, a.K - (t + 1) * 64, lds0 + (stage ^ 1) * STAGE + OPB, wave);
+            }
+            if (ks == 3) wait_vmcnt<0>();
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = Vec<T>::mfma(af[slot][i], bf[slot][j], acc[i][j]);
-        };
-        load(0, 0);
-        load(1, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(1);
-        mma(0);
-        load(2, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        mma(1);
-        load(3, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        mma(0);
-        mma(1);
-        __builtin_amdgcn_s_setprio(0);
-    };
-    if (t0 < t1) issue(0, t0);
-    // one body for both stages: written out for each, the compiler moved the sums between registers and spilled some
-    for (int64_t t = t0; t < t1; ++t) {
-        const int stage = (int)(t - t0) & 1;
-        wait_vmcnt<0>();
-        asm volatile("s_barrier" ::: "memory");   // tile t is there; every wave is done with the other stage
-        if (t + 1 < t1) issue(stage ^ 1, t + 1);
-        compute(lds + stage * STAGE);
+                for (int j = 0; j < FN; ++j) acc[i][j] = Vec<T>::mfma(af[i], bf[j], acc[i][j]);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_barrier" ::: "memory");
+        }
     }
-    // the sums pass through LDS, 64 rows at a time, so that a thread stores 8 columns of a row
+    if (!late) asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < FM; ++i) wattn::settle(acc[i]);
     float* st = reinterpret_cast<float*>(lds);
-    constexpr int CPR = EDGE / 8;   // threads a row
-    const int cq = (tid % CPR) * 8;
-    const int64_t n = n0 + cq;
     __syncthreads();
 #pragma unroll 1
-    for (int rb = 0; rb < EDGE; rb += ER) {
+    for (int rb = 0; rb < EDGE; rb += 64) {
         if (wm0 == rb) {
 #pragma unroll
             for (int i = 0; i < FM; ++i)
@@ -296,21 +338,117 @@ __global__ __launch_bounds__(EDGE * 2, 2) void prod_tile_kernel(GemmArgs a) {
                             acc[i][j][v];
         }
         __syncthreads();
-        for (int r = tid / CPR; r < ER; r += NT / CPR) {
-            const int64_t m = m0 + rb + r;
-            if (m >= a.M || n >= a.N) break;
-            float v[8];
+        finish_rows<T, FWD, EDGE, NT, EROW>(a, tp, st, rb, tid);
+        __syncthreads();
+    }
+}
+
+// Tiles of 128 x 128: four waves of 64 x 64. STAGES 2: 64 KB of LDS, two workgroups a CU; STAGES 4: one. A wave keeps its MFMAs
+// fed by itself: the fragments of K step ks + 1 are read between the products of ks. Before the last step's products every wave
+// has read the last of tile t and tile t + 1 has landed; the one barrier a tile is there, and behind it the first fragments of
+// t + 1 are read and the loads of tile t + STAGES begin to go out into t's piece, a quarter of them a K step. (Loads of tiles past
+// the end give zeros and touch no memory, so that every round has the same number under way.)
+template <class T, int STAGES, bool AK, bool BK, bool FWD>
+__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void prod_tile_kernel(GemmArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    constexpr int EDGE = 128, NT = 256, F = 2, OPB = EDGE * 128, STAGE = 2 * OPB, EROW = EDGE + 8;
+    typedef Operand<T, EDGE, NT, AK> OpA;
+    typedef Operand<T, EDGE, NT, BK> OpB;
+    constexpr int LOADS = OpA::PER + OpB::PER;
+    static_assert(64 * EROW * 4 <= STAGES * STAGE, "staged rows fit the stages' memory");
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
+    const TilePlace tp = tile_place<EDGE>(a);
+    if (tp.none) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm0 = (wave & 1) * 64, wn0 = (wave >> 1) * 64;
+    OpA A;
+    OpB B;
+    A.init(a.A, a.lda, tp.m0, a.M, tid);
+    B.init(a.B, a.ldb, tp.n0, a.N, tid);
+    const int64_t KT = (a.K + 63) / 64, t0 = (int64_t)tp.z * a.per, t1 = min(KT, t0 + a.per);
+    f32x16 acc[F][F];
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(st + r * EROW + cq + e);
-                v[e] = x.x;
-                v[e + 1] = x.y;
-                v[e + 2] = x.z;
-                v[e + 3] = x.w;
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+    // K left at tile t: none past this split's end
+    auto left = [&](int64_t t) { return t < t1 ? a.K - t * 64 : (int64_t)0; };
+    x8 f[2][2 * F];   // two sets of fragments: A's, then B's
+    auto read = [&](const char* s, int ks, int n, x8& to) {
+        if (n < F) to = OpA::frag(s, wm0 + 32 * n, ks, lane);
+        else to = OpB::frag(s + OPB, wn0 + 32 * (n - F), ks, lane);
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+        A.issue(t0 + s, left(t0 + s), lds0 + s * STAGE, wave);
+        B.issue(t0 + s, left(t0 + s), lds0 + s * STAGE + OPB, wave);
+    }
+    // the tile whose loads are going out: its descriptors, its K, its place
+    int64_t lp = left(t0 + STAGES - 1);
+    u32x4 ra = A.tile(t0 + STAGES - 1, lp), rb = B.tile(t0 + STAGES - 1, lp);
+    uint32_t dst = lds0 + (STAGES - 1) * STAGE;
+    auto load = [&](int q) {
+        A.load(ra, q, lp, dst, wave);
+        B.load(rb, q, lp, dst + OPB, wave);
+    };
+    static_assert(OpA::PER == 4 && OpB::PER == 4, "a load of each operand a K step");
+    load(0);
+    wait_vmcnt<(STAGES - 2) * LOADS + 2>();   // tile t0
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int n = 0; n < 2 * F; ++n) read(lds, 0, n, f[0][n]);
+    int stage = 0;
+    for (int64_t t = t0; t < t1; ++t) {
+        const int after = stage + 1 < STAGES ? stage + 1 : 0;
+        const char* now = lds + stage * STAGE;
+        const char* next = lds + after * STAGE;
+#pragma unroll
+        for (int ks = 0; ks < 3; ++ks)
+#pragma unroll
+            for (int n = 0; n < F * F; ++n) {
+                acc[n / F][n % F] = Vec<T>::mfma(f[ks & 1][n / F], f[ks & 1][F + n % F], acc[n / F][n % F]);
+                read(now, ks + 1, n, f[(ks & 1) ^ 1][n]);
+                if (n == F) load(ks + 1);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (a.part) store8(a.part + ((int64_t)z * a.M + m) * a.pitch, n, a.pitch, v);
-            else finish8<T, FWD>(a, m, n, v);
+        lp = left(t + STAGES);
+        ra = A.tile(t + STAGES, lp);
+        rb = B.tile(t + STAGES, lp);
+        dst = lds0 + stage * STAGE;
+        wait_vmcnt<(STAGES - 2) * LOADS>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int n = 0; n < F * F; ++n) {
+            acc[n / F][n % F] = Vec<T>::mfma(f[1][n / F], f[1][F + n % F], acc[n / F][n % F]);
+            read(next, 0, n, f[0][n]);
+            if (n == F) load(0);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        stage = after;
+    }
+#pragma unroll
+    for (int i = 0; i < F; ++i) wattn::settle(acc[i]);
+    wait_vmcnt<0>();   // (loads past the end: zeros, but into this memory)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    float* st = reinterpret_cast<float*>(lds);
+    __syncthreads();
+#pragma unroll 1
+    for (int rb = 0; rb < EDGE; rb += 64) {
+        if (wm0 == rb) {
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < F; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        st[(32 * i + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3)) * EROW + wn0 + 32 * j + (lane & 31)] =
+                            acc[i][j][v];
+        }
+        __syncthreads();
+        finish_rows<T, FWD, EDGE, NT, EROW>(a, tp, st, rb, tid);
         __syncthreads();
     }
 }
@@ -509,22 +647,22 @@ size_t split_bytes(const ProdPlan& p, int64_t M, int64_t N) {
     return p.splits > 1 ? (size_t)p.splits * (size_t)M * (size_t)up8(N) * sizeof(float) : 0;
 }
 
-template <class T, int EDGE, bool AK, bool BK, bool FWD>
-void tile_launch(sa3k_ctx* ctx, const GemmArgs& a, const char* name) {
-    const int64_t tiles = ceil_div(a.M, EDGE) * ceil_div(a.N, EDGE);
-    KernelScope ks(ctx, name, 2.0 * (double)a.M * (double)a.N * (double)a.K);
-    launch_k(ctx, a.splits == 1, prod_tile_kernel<T, EDGE, AK, BK, FWD>,
-             dim3((unsigned)(ceil_div(tiles, 8) * 8), (unsigned)a.splits), dim3(EDGE * 2), 0, a);
-    SA3K_LAUNCHED();
-}
 template <class T, bool AK, bool BK, bool FWD>
 void tile_run(sa3k_ctx* ctx, GemmArgs& a, const ProdPlan& p, float* part, const char* name) {
     a.splits = p.splits;
     a.per = p.per;
     a.part = p.splits > 1 ? part : nullptr;
     a.pitch = up8(a.N);
-    if (p.edge == 256) tile_launch<T, 256, AK, BK, FWD>(ctx, a, name);
-    else tile_launch<T, 128, AK, BK, FWD>(ctx, a, name);
+    {
+        const int64_t tiles = ceil_div(a.M, p.edge) * ceil_div(a.N, p.edge);
+        const dim3 grid((unsigned)(ceil_div(tiles, 8) * 8), (unsigned)a.splits);
+        KernelScope ks(ctx, name, 2.0 * (double)a.M * (double)a.N * (double)a.K);
+        if (p.edge == 256) launch_k(ctx, a.splits == 1, prod_big_kernel<T, AK, BK, FWD>, grid, dim3(512), 0, a);
+        else if (tiles * a.splits <= 256)   // one workgroup a CU at the most: deeper stages
+            launch_k(ctx, a.splits == 1, prod_tile_kernel<T, 4, AK, BK, FWD>, grid, dim3(256), 0, a);
+        else launch_k(ctx, a.splits == 1, prod_tile_kernel<T, 2, AK, BK, FWD>, grid, dim3(256), 0, a);
+        SA3K_LAUNCHED();
+    }
     if (p.splits > 1) {
         KernelScope ks(ctx, "linear_act_sum");
         launch_k(ctx, true, prod_sum_kernel<T, FWD>, dim3((unsigned)ceil_div(a.M * (a.pitch / 8), 256)), dim3(256), 0, a);

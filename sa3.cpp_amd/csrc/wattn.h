@@ -220,8 +220,8 @@ __device__ __forceinline__ typename Vec<T>::x8 ld_global(const T* p, bool ok) {
 struct Place {
     int b, kh, h, blk;
 };
-__device__ __forceinline__ Place place(const AttnShape& a, int blocks) {
-    const int L = blockIdx.x, BH = a.B * a.H, BK = a.B * a.K;
+__device__ __forceinline__ Place place(const AttnShape& a, int blocks, int index) {
+    const int L = index, BH = a.B * a.H, BK = a.B * a.K;
     const int i = L % BH, bk = i % BK, g = i / BK;
     Place p;
     p.b = bk / a.K;

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(kThreads, 2) void wattn_fwd_kernel(FwdArgs a) {
     constexpr int TILE = BLK * D * 2, STAGES = 2, LOADS = 2 * (D / 64) * (BLK * 8 / kThreads);
     __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * TILE];
     const AttnShape& s = a.s;
-    const Place pl = place(s, (s.Sq + 127) / 128);
+    const Place pl = place(s, (s.Sq + 127) / 128, blockIdx.x);
     const int nq = clamp_len(s.q_len, pl.b, s.Sq), nk = clamp_len(s.k_len, pl.b, s.Sk), off = nk - nq;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hl = lane >> 5;
     const int q0 = pl.blk * 128;

@@ -1,9 +1,9 @@
 // Windowed attention with first tokens that stay visible: the backward. With p_ij = 2^(c q_i . k_j - lse_i) from
-// recomputed scores, delta_i = dO_i . o_i and ds_ij = p_ij (dO_i . v_j - delta_i):
+// recomputed scores, delta_i = dO_i . o_i (a launch of its own) and ds_ij = p_ij (dO_i . v_j - delta_i):
 //   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij dO_i
 // Two passes, each over the scores of every visible block, so that no sum is shared between workgroups (no atomics:
-// the same bits in every run): one by queries (dq, and delta for the other), one by keys (dk, dv, over all the
-// query heads of a group). Seven products of 2 D a pair where five would do with dq summed by atomics.
+// the same bits in every run): one by queries (dq), one by keys (dk, dv, over all the query heads of a group). Seven
+// products of 2 D a pair where five would do with dq summed by atomics.
 //
 // By queries: S^T = K Q^T and dP^T = V dO^T leave a lane with one query, dq^T += K^T dS^T reads K transposed.
 // By keys: S = Q K^T and dP = dO V^T leave it with one key, dv^T += dO^T P and dk^T += Q^T dS read dO and Q transposed.
@@ -51,14 +51,30 @@ __device__ __forceinline__ void store_row(T* p, const f32x16 (&x)[D / 32], float
         }
 }
 
-// 128 queries of one head a workgroup, 32 a wave; key tiles as in the forward.
+// delta = dO . o of every row: D / 8 lanes a row, 8 dims each.
 template <class T, int D>
-__global__ __launch_bounds__(kThreads, 2) void wattn_dq_kernel(BwdArgs a) {
+__global__ __launch_bounds__(kThreads) void wattn_delta_kernel(BwdArgs a) {
+    constexpr int L = D / 8;
+    const AttnShape& s = a.s;
+    const int64_t i = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;   // row [b][q][h]: heads lie together
+    const int h = (int)(i % s.H);
+    const int64_t bq = i / s.H;
+    const int b = (int)(bq / s.Sq), q = (int)(bq - (int64_t)b * s.Sq);
+    const bool ok = b < s.B && q < clamp_len(s.q_len, min(b, s.B - 1), s.Sq);
+    const int64_t off = b * s.os[0] + (int64_t)q * s.os[1] + h * s.os[2] + (threadIdx.x % L) * 8;
+    float d = dot8<T>(ld_global(static_cast<const T*>(a.dO) + off, ok), ld_global(static_cast<const T*>(a.o) + off, ok));
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) d += __shfl_xor(d, o, 64);
+    if (ok && threadIdx.x % L == 0) a.delta[((int64_t)b * s.H + h) * s.Sq + q] = d;
+}
+
+// 128 queries of one head a workgroup (`index` of them), 32 a wave; key tiles as in the forward.
+template <class T, int D>
+__device__ __forceinline__ void dq_body(const BwdArgs& a, int index, char* lds) {
     typedef typename Vec<T>::x8 x8;
     constexpr int TILE = BLK * D * 2, STAGES = 2, LOADS = 2 * (D / 64) * (BLK * 8 / kThreads);
-    __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * TILE];
     const AttnShape& s = a.s;
-    const Place pl = place(s, (s.Sq + 127) / 128);
+    const Place pl = place(s, (s.Sq + 127) / 128, index);
     const int nq = clamp_len(s.q_len, pl.b, s.Sq), nk = clamp_len(s.k_len, pl.b, s.Sk), off = nk - nq;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hl = lane >> 5;
     const int c32 = lane & 31;
@@ -72,16 +88,12 @@ __global__ __launch_bounds__(kThreads, 2) void wattn_dq_kernel(BwdArgs a) {
     const T* vp = static_cast<const T*>(a.v) + pl.b * s.vs[0] + pl.kh * s.vs[2];
     const int64_t row = ((int64_t)pl.b * s.H + pl.h) * s.Sq + q;
     x8 qf[D / 16], dof[D / 16];
-    float delta = 0.f;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
         qf[ks] = ld_global(static_cast<const T*>(a.q) + qoff + ks * 16 + hl * 8, q < nq);
         dof[ks] = ld_global(static_cast<const T*>(a.dO) + ooff + ks * 16 + hl * 8, q < nq);
-        delta += dot8<T>(dof[ks], ld_global(static_cast<const T*>(a.o) + ooff + ks * 16 + hl * 8, q < nq));
     }
-    delta += __shfl_xor(delta, 32, 64);
-    if (q < nq && hl == 0) a.delta[row] = delta;
-    const float lse = q < nq ? a.lse[row] : 0.f;
+    const float lse = q < nq ? a.lse[row] : 0.f, delta = q < nq ? a.delta[row] : 0.f;
 
     Seen see = seen_by(q + off, nk, s.left, s.right, s.sinks, s.causal);
     if (q >= nq) see = Seen{0, 0, 0};
@@ -160,13 +172,11 @@ __global__ __launch_bounds__(kThreads, 2) void wattn_dq_kernel(BwdArgs a) {
 
 // 128 keys of one key/value head a workgroup, 32 a wave; tiles of 64 queries' q and dO with their lse and delta.
 template <class T, int D>
-__global__ __launch_bounds__(kThreads, 2) void wattn_dkdv_kernel(BwdArgs a) {
+__device__ __forceinline__ void dkdv_body(const BwdArgs& a, int index, char* lds, float (&vec)[2][2][BLK]) {
     typedef typename Vec<T>::x8 x8;
     constexpr int TILE = BLK * D * 2, STAGES = 2, LOADS = 2 * (D / 64) * (BLK * 8 / kThreads) + 1;
-    __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * TILE];
-    __shared__ __attribute__((aligned(16))) float vec[STAGES][2][BLK];   // lse, delta
     const AttnShape& s = a.s;
-    const int BK = s.B * s.K, bk = blockIdx.x % BK, item = blockIdx.x / BK;
+    const int BK = s.B * s.K, bk = index % BK, item = index / BK;
     const int b = bk / s.K, kh = bk - b * s.K;
     const KeyItem ki = key_item(a.split, item);
     const int nq = clamp_len(s.q_len, b, s.Sq), nk = clamp_len(s.k_len, b, s.Sk), off = nk - nq;
@@ -320,6 +330,17 @@ __global__ __launch_bounds__(kThreads, 2) void wattn_dkdv_kernel(BwdArgs a) {
         }
 }
 
+// Both passes in one launch: the workgroups by keys, which run longer, first, then those by queries, so that neither
+// pass's last turn leaves the chip partly empty.
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, 2) void wattn_bwd_kernel(BwdArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * BLK * D * 2];
+    __shared__ __attribute__((aligned(16))) float vec[2][2][BLK];   // lse, delta
+    const int by_key = a.s.Sk > 0 ? a.s.B * a.s.K * a.split.items() : 0, i = blockIdx.x;
+    if (i < by_key) dkdv_body<T, D>(a, i, lds, vec);
+    else dq_body<T, D>(a, i - by_key, lds);
+}
+
 // dk and dv of the tiles with more than one share: the shares' sums in their order, 8 dims a thread.
 template <class T, int D>
 __global__ __launch_bounds__(kThreads) void wattn_dkdv_sum_kernel(BwdArgs a, int tiles) {
@@ -370,16 +391,16 @@ void bwd_run(sa3k_ctx* ctx, BwdArgs& a) {
     a.delta = gemm_workspace_bytes(ctx, (nd + np) * sizeof(float));
     a.part = a.delta + nd;
     if (s.Sq > 0) {
-        KernelScope ks(ctx, "window_attn_dq");
-        launch_k(ctx, s.Sk == 0, wattn_dq_kernel<T, D>, dim3((unsigned)(ceil_div(s.Sq, 128) * s.B * s.H)), dim3(kThreads), 0,
-                 a);
+        KernelScope ks(ctx, "window_attn_delta");
+        launch_k(ctx, false, wattn_delta_kernel<T, D>, dim3((unsigned)ceil_div((int64_t)s.B * s.H * s.Sq, kThreads / (D / 8))),
+                 dim3(kThreads), 0, a);
         SA3K_LAUNCHED();
     }
-    if (s.Sk == 0) return;
     {
-        KernelScope ks(ctx, "window_attn_dkdv");
-        launch_k(ctx, summed == 0, wattn_dkdv_kernel<T, D>, dim3((unsigned)(s.B * s.K) * a.split.items()), dim3(kThreads), 0,
-                 a);
+        const int64_t by_key = s.Sk > 0 ? (int64_t)s.B * s.K * a.split.items() : 0, by_query = ceil_div(s.Sq, 128) * s.B * s.H;
+        if (by_key + by_query == 0) return;
+        KernelScope ks(ctx, "window_attn_bwd");
+        launch_k(ctx, summed == 0, wattn_bwd_kernel<T, D>, dim3((unsigned)(by_key + by_query)), dim3(kThreads), 0, a);
         SA3K_LAUNCHED();
     }
     if (summed) {
