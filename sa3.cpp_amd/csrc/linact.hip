@@ -479,7 +479,7 @@ __global__ __launch_bounds__(256) void prod_sum_kernel(GemmArgs a) {
 template <class T, int MB>
 __global__ __launch_bounds__(512) void prod_few_kernel(GemmArgs a) {
     typedef typename Vec<T>::x8 x8;
-    constexpr int W = 8, U = 4;
+    constexpr int W = 8, U = 8;
     __shared__ float red[W][MB][16][17];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15;
     const int64_t n0 = (int64_t)blockIdx.x * 16, wn = n0 + r;
@@ -591,28 +591,10 @@ __global__ __launch_bounds__(256) void prod_dz_kernel(const T* dY, int64_t lddy,
     part[(int64_t)blockIdx.y * N + j] = t;
 }
 
-// db (+)= the workgroups' sums, in their order: 64 columns a workgroup, a quarter of the sums a wave, eight in flight
-__global__ __launch_bounds__(256) void prod_db_kernel(const float* __restrict__ part, int parts, int64_t N, float* db,
-                                                      int accumulate) {
-    __shared__ float s[4][64];
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t i = (int64_t)blockIdx.x * 64 + lane;
-    const int per = (parts + 3) / 4, lo = min(parts, w * per), hi = min(parts, lo + per);
-    float t = 0.f;
-    if (i < N)
-        for (int k = lo; k < hi; k += 8) {
-            float v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)min(k + u, hi - 1) * N + i];
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (k + u < hi) t += v[u];
-        }
-    s[w][lane] = t;
-    __syncthreads();
-    if (w || i >= N) return;
-    t = ((s[0][lane] + s[1][lane]) + s[2][lane]) + s[3][lane];
-    db[i] = accumulate ? db[i] + t : t;
+// db (+)= the workgroups' sums
+__global__ __launch_bounds__(kColumnSumThreads) void prod_db_kernel(const float* __restrict__ part, int parts, int64_t N,
+                                                                    float* db, int accumulate) {
+    column_sums(part, parts, N, [&](int64_t i, float t) { db[i] = accumulate ? db[i] + t : t; });
 }
 
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
@@ -726,7 +708,7 @@ void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     }
     if (p.db) {
         KernelScope ks(ctx, "linear_act_db");
-        launch_k(ctx, !products, prod_db_kernel, dim3((unsigned)ceil_div(N, 64)), dim3(256), 0, part, parts, N, p.db,
+        launch_k(ctx, !products, prod_db_kernel, dim3((unsigned)ceil_div(N, 64)), dim3(kColumnSumThreads), 0, part, parts, N, p.db,
                  p.accumulate);
         SA3K_LAUNCHED();
     }

@@ -228,31 +228,14 @@ __global__ __launch_bounds__(kNormThreads<TG>) void norm_bwd_kernel(NormArgs a, 
         }
 }
 
-// The sums over `parts` workspace rows: a workgroup takes 64 of the 2 cols sums, a quarter of the rows a
-// wave, eight rows in flight, added in row order within a quarter and then quarter by quarter.
-__global__ __launch_bounds__(256) void norm_bwd_sum_kernel(const float* __restrict__ part, int parts, int cols,
-                                                           float* dgamma, float* dbeta, int accumulate) {
-    __shared__ float s[4][64];
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t n = 2 * (int64_t)cols, i = (int64_t)blockIdx.x * 64 + lane;
-    const int per = (parts + 3) / 4, lo = min(parts, w * per), hi = min(parts, lo + per);
-    float t = 0.f;
-    if (i < n)
-        for (int k = lo; k < hi; k += 8) {
-            float v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)min(k + u, hi - 1) * n + i];
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (k + u < hi) t += v[u];
-        }
-    s[w][lane] = t;
-    __syncthreads();
-    if (w || i >= n) return;
-    t = ((s[0][lane] + s[1][lane]) + s[2][lane]) + s[3][lane];
-    float* d = i < cols ? dgamma : dbeta;
-    const int64_t c = i < cols ? i : i - cols;
-    if (d) d[c] = accumulate ? d[c] + t : t;
+// dgamma and dbeta from the workgroups' sums
+__global__ __launch_bounds__(kColumnSumThreads) void norm_bwd_sum_kernel(const float* __restrict__ part, int parts, int cols,
+                                                                         float* dgamma, float* dbeta, int accumulate) {
+    column_sums(part, parts, 2 * (int64_t)cols, [&](int64_t i, float t) {
+        float* d = i < cols ? dgamma : dbeta;
+        const int64_t c = i < cols ? i : i - cols;
+        if (d) d[c] = accumulate ? d[c] + t : t;
+    });
 }
 
 // Workgroups of the backward with gradients of gain and offset. Each writes 8 cols bytes that the second
@@ -280,7 +263,7 @@ void norm_launch(sa3k_ctx* ctx, const NormArgs& a, bool bwd) {
     }
     if (sums) {
         KernelScope ks(ctx, "layer_norm_bwd_sum");
-        launch_k(ctx, true, norm_bwd_sum_kernel, dim3((unsigned)ceil_div(2 * a.cols, 64)), dim3(256), 0, part, grid,
+        launch_k(ctx, true, norm_bwd_sum_kernel, dim3((unsigned)ceil_div(2 * a.cols, 64)), dim3(kColumnSumThreads), 0, part, grid,
                  (int)a.cols, a.dgamma, a.dbeta, a.accumulate);
         SA3K_LAUNCHED();
     }
@@ -309,7 +292,7 @@ void norm_dispatch(sa3k_ctx* ctx, const NormArgs& a, bool bwd) {
         if (bwd && !a.accumulate)
             for (float* d : {a.dgamma, a.dbeta})
                 if (d) {
-                    norm_bwd_sum_kernel<<<(unsigned)ceil_div(2 * a.cols, 64), 256, 0, ctx->stream>>>(
+                    norm_bwd_sum_kernel<<<(unsigned)ceil_div(2 * a.cols, 64), kColumnSumThreads, 0, ctx->stream>>>(
                         nullptr, 0, (int)a.cols, d == a.dgamma ? d : nullptr, d == a.dgamma ? nullptr : d, 0);
                     SA3K_LAUNCHED();
                 }

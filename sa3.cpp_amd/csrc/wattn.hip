@@ -333,18 +333,36 @@ __global__ __launch_bounds__(kThreads) void wattn_join_kernel(FwdArgs a) {
     const int64_t step = R * (D + 2);
     const float* p = a.part + ((int64_t)bk * a.chunks + chunk) * a.splits * step;
     const float *pm = p + R * D + row, *plw = pm + R, *po = p + row * D + d0;
+    // a lane a split for the maximum and the factors, the row's 32 lanes in step; then the sums, eight splits in flight
+    const int z0 = threadIdx.x & 31;
     float M = -INFINITY;
-    for (int z = 0; z < a.splits; ++z) M = fmaxf(M, pm[z * step]);
+    for (int z = z0; z < a.splits; z += 32) M = fmaxf(M, pm[z * step]);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
     const float base = M == -INFINITY ? 0.f : M;
     float acc[PER], L = 0.f;
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    for (int z = 0; z < a.splits; ++z) {
-        const float f = ex2(pm[z * step] - base);
-        L += plw[z * step] * f;
+    for (int zb = 0; zb < a.splits; zb += 32) {
+        const int z = zb + z0;
+        const float mine = z < a.splits ? ex2(pm[z * step] - base) : 0.f;
+        L += z < a.splits ? plw[z * step] * mine : 0.f;
+        for (int k = 0; k < 32 && zb + k < a.splits; k += 8) {
+            float v[8][PER];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] = __builtin_fmaf(po[z * step + e], f, acc[e]);
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < PER; ++e) v[u][e] = po[min(zb + k + u, a.splits - 1) * step + e];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float f = __shfl(mine, (threadIdx.x & 32) + k + u, 64);   // 0 past the last split
+#pragma unroll
+                for (int e = 0; e < PER; ++e) acc[e] = __builtin_fmaf(v[u][e], f, acc[e]);
+            }
+        }
     }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) L += __shfl_xor(L, o, 64);
     const int q = r / s.G, h = kh * s.G + (r - q * s.G);
     const float il = L == 0.f ? 0.f : 1.f / L;
     T* op = static_cast<T*>(a.o) + b * s.os[0] + (int64_t)q * s.os[1] + h * s.os[2] + d0;
