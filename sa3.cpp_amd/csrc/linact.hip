@@ -50,12 +50,29 @@ struct GemmArgs {
 };
 
 // The activations on the hardware's exp2 and reciprocal. For gelu_tanh, (1 + tanh u) / 2 = 1 / (1 + e^-2u); its argument is
-// held within +-10, where it is 0 or 1 in f32, so that a large z^3 does not overflow.
+// held within +-10, where it is 0 or 1 in f32, so that a large z^3 does not overflow. For gelu, (1 + erf(z / sqrt 2)) / 2 by
+// Abramowitz and Stegun's approximation 7.1.26 of erf (off by at most 1.5e-7): with x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x),
+// 1 - erf x = (a1 t + .. + a5 t^5) e^-x^2, whose exponential is also the slope's. (The library's erff made the pass over dY and z
+// bound by its arithmetic.)
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + ex2(-kLog2e * x)); }
+// (1 + erf(z / sqrt 2)) / 2, and e^(-z^2 / 2)
+__device__ __forceinline__ float normal_below(float z, float& bell) {
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f);
+    bell = ex2(-0.5f * kLog2e * z * z);
+    const float tail = 0.5f * p * t * bell;   // the part beyond |z|
+    return z < 0.f ? tail : 1.f - tail;
+}
 __device__ __forceinline__ float act_value(float z, int act) {
     if (act == SA3K_ACT_RELU) return z <= 0.f ? 0.f : z;
     if (act == SA3K_ACT_SILU) return z * sigmoid(z);
-    if (act == SA3K_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if (act == SA3K_ACT_GELU) {
+        float bell;
+        return z * normal_below(z, bell);
+    }
     if (act == SA3K_ACT_GELU_TANH) {
         const float y = fminf(fmaxf(z, -10.f), 10.f);
         return z * sigmoid(1.5957691216057308f * (y + 0.044715f * y * y * y));
@@ -68,8 +85,11 @@ __device__ __forceinline__ float act_slope(float z, int act) {
         const float g = sigmoid(z);
         return g * (1.f + z * (1.f - g));
     }
-    if (act == SA3K_ACT_GELU)
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * ex2(-0.5f * kLog2e * z * z) * 0.39894228040143268f;
+    if (act == SA3K_ACT_GELU) {
+        float bell;
+        const float below = normal_below(z, bell);
+        return below + z * bell * 0.39894228040143268f;
+    }
     if (act == SA3K_ACT_GELU_TANH) {
         const float y = fminf(fmaxf(z, -10.f), 10.f);
         const float g = sigmoid(1.5957691216057308f * (y + 0.044715f * y * y * y));
@@ -682,7 +702,11 @@ void fwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     tile_run<T, false, false, true>(ctx, a, plan, reinterpret_cast<float*>(ws + os), "linear_act_fwd");
 }
 
-constexpr int kDzParts = 256;   // row shares of the pass over dY and z, at the most
+// Row shares of the pass over dY and z: about 128, each of the same number of rounds of eight rows.
+int dz_parts(int64_t M) {
+    const int64_t groups = std::max<int64_t>(1, ceil_div(M, 8)), rounds = ceil_div(groups, 128);
+    return (int)ceil_div(groups, rounds);
+}
 
 template <class T>
 void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
@@ -692,7 +716,7 @@ void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     const bool own_dz = products && M > 0 && (p.act != SA3K_ACT_NONE || !loads16(p.dY, p.lddy, N));
     const bool px = p.dW && M > 0 && !loads16(p.X, p.ldx, K), pw = p.dX && M > 0 && !loads16(p.W, p.ldw, K);
     const ProdPlan px_plan = prod_plan(M > 0 ? M : 1, K, N), pw_plan = prod_plan(N, K, M > 0 ? M : 1);
-    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(kDzParts, ceil_div(M, 8)));
+    const int parts = dz_parts(M);
     Scratch s;
     const size_t oz = s.take(own_dz ? (size_t)M * Np * 2 : 0), ox = s.take(px ? (size_t)M * Kp * 2 : 0);
     const size_t ow = s.take(pw ? (size_t)N * Kp * 2 : 0), ob = s.take(p.db ? (size_t)parts * N * 4 : 0);

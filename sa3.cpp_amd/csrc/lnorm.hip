@@ -254,7 +254,9 @@ void norm_launch(sa3k_ctx* ctx, const NormArgs& a, bool bwd) {
         return;
     }
     const bool sums = a.dgamma || a.dbeta;
-    const int grid = (int)std::min<int64_t>(blocks, sums ? kNormBwdGroups : 1 << 20);
+    // workgroups of the same number of rounds each
+    const int64_t rounds = ceil_div(blocks, sums ? kNormBwdGroups : 1 << 20);
+    const int grid = (int)ceil_div(blocks, rounds);
     float* part = sums ? gemm_workspace_bytes(ctx, (size_t)grid * 2 * (size_t)a.cols * sizeof(float)) : nullptr;
     {
         KernelScope ks(ctx, "layer_norm_bwd");
