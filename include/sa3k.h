@@ -427,8 +427,9 @@ SA3K_API int sa3k_diff_attn_bwd(sa3k_ctx* ctx, const void* q1, const void* k1, c
  * layer norm, attention with a sliding window, and products with an epilogue. No reference counterpart.
  * Tensors are device memory; a tensor's elements are of `type`, its sums and statistics f32. Rows are
  * `ld` elements apart (ld >= the row's length) and may start at any element. Calls with nothing to
- * compute (no rows, no samples) return SA3K_OK and launch nothing that they need not. The calls switch
- * the thread's HIP device to the context's and back. */
+ * compute (no rows, no samples) return SA3K_OK and launch nothing that they need not. Outputs overlap neither
+ * inputs nor each other unless a call says that they may. The calls switch the thread's HIP device to the
+ * context's and back. */
 
 /* Layer norm of rows [rows][cols] (cols <= 16384), type f32, f16 or bf16, optionally of the sum with a
  * residual:
@@ -473,8 +474,9 @@ typedef struct {
  *   o = sum_j softmax_j(scale q . k_j) v_j,  lse = log2 sum_j 2^(scale log2(e) q . k_j)
  * A query that sees no key gets o = 0 and lse = -inf. o and lse (f32 [batch][heads][q_tokens], nullable) of rows
  * past q_len stay as they were; keys, values, queries and gradients past a sample's lengths are never read. Weights
- * are rounded to `type` for the product with v, everything else is f32. Few queries (at most 32) over many
- * keys run with the keys split over workgroups, whose sums are joined in a fixed order. Tensors 16-byte aligned. */
+ * are rounded to `type` for the product with v, everything else is f32. Few queries over many keys run with the
+ * keys split over workgroups, whose sums are joined in a fixed order. Tensors 16-byte aligned. Within a sample's lengths
+ * keys and values must be finite: a hidden key's weight is 0, but 0 times an infinite or NaN value is NaN. */
 SA3K_API int sa3k_window_attn_fwd(sa3k_ctx* ctx, const sa3k_window_attn* d, const void* q, const void* k, const void* v,
                                   const int32_t* q_len, const int32_t* k_len, void* o, float* lse);
 

@@ -227,15 +227,27 @@ SA3K_HD KeyBlocks key_blocks(int pa, int pb, int nk, int left, int right, int si
 SA3K_HD int key_block(const KeyBlocks& r, int i) { return i < r.head ? i : r.from + (i - r.head); }
 
 
-// Few queries: at most this many run with the keys split over workgroups.
-constexpr int kFewQueries = 32;
-// The split count for `chunks` chunks of 32 rows a key/value head: about two workgroups a CU in all, at least two
-// blocks of 32 keys a wave.
+// The most keys that a sample's queries see.
+inline int64_t keys_seen(const AttnShape& s) {
+    const int64_t reach = (int64_t)s.left + s.right + s.Sq + 32;
+    return (reach < s.Sk ? reach : s.Sk) + s.sinks;
+}
+// Whether the keys are split over workgroups and waves, 32 rows (query, member of the group) at a time, instead of running by
+// tiles of 128 queries a head. Measured on MI355X (tiles / split, us; 32 heads of 128 on 8, all keys visible):
+//   one query:       1 x 16384 keys 337 / 20.0, 8 x 4096 keys 87 / 30
+//   32 queries:      1 x 16384 keys 289 / 35.6, 8 x 2048 keys 41 / 35, 8 x 512 keys 13.3 / 21.7
+//   64 queries:      1 x 16384 keys 300 / 54
+// Tiles win where there are rows for more than one chunk, few keys and enough heads to fill the chip.
+inline bool attn_split_keys(const AttnShape& s) {
+    const int64_t tiles = (int64_t)s.B * s.H * ((s.Sq + 127) / 128), keys = keys_seen(s);
+    if (s.Sq <= 32) return s.Sq * s.G <= 32 || tiles < 256 || keys > 1024;
+    return tiles < 128 && keys >= 2048;
+}
+// The split count for `chunks` chunks of 32 rows a key/value head: a workgroup a CU in all (8 x one query over windows of 4096
+// keys: 128 / 256 / 512 / 1024 workgroups 34.0 / 29.5 / 33.1 / 41.5 us), at least two blocks of 32 keys a wave.
 inline int attn_splits(const AttnShape& s, int chunks) {
-    const int64_t reach = (int64_t)s.left + s.right + s.Sq + 32;   // keys that a sample's queries see at the most
-    const int64_t keys = (reach < s.Sk ? reach : s.Sk) + s.sinks;
-    const int64_t base = (int64_t)s.B * s.K * chunks, most = keys / (32 * 4 * 2);
-    int64_t n = 512 / (base > 0 ? base : 1);
+    const int64_t base = (int64_t)s.B * s.K * chunks, most = keys_seen(s) / (32 * 4 * 2);
+    int64_t n = 256 / (base > 0 ? base : 1);
     if (n > most) n = most;
     return n < 1 ? 1 : (int)n;
 }
@@ -363,9 +375,11 @@ inline const char* prod_check(const ProdArgs& a, bool bwd, int* code) {
 }
 
 // The tiles (square, `edge` wide) of an M x N x K product and the split of its contraction, by estimated time in
-// microseconds. Measured on MI355X: a round of 256 x 256 tiles (one workgroup a CU) takes 1.7 a tile of 64 along K, one of
-// 128 x 128 tiles 1.05 with two workgroups a CU and 0.7 with one; a workgroup's start and its stores about 4; the
-// launch that adds up splits 4 and its traffic at 4 MB a microsecond.
+// microseconds. Measured on MI355X: a round of 256 x 256 tiles (one workgroup a CU) takes 1.75 a tile of 64 along K, one of
+// 128 x 128 tiles 1.0 with two workgroups a CU and 0.57 with one; a workgroup's start and its stores about 4; the
+// launch that adds up splits 4 and its traffic at 4 MB a microsecond. What it chooses is within 3% of the best of both tiles
+// and 1 to 6 splits on twelve shapes from 128 to 6144 rows (2176 x 6144 x 1536: 128 x 128 whole 58 us, in two splits 63,
+// 256 x 256 in four splits 61, whole 125; 4096 x 1024 x 4096: 256 x 256 43, 128 x 128 51).
 struct ProdPlan {
     int edge, splits, per;   // per: tiles of 64 along K that a split takes
 };
@@ -380,7 +394,7 @@ inline ProdPlan prod_plan(int64_t M, int64_t N, int64_t K) {
             const int64_t per = (kt + n - 1) / n;
             if ((n - 1) * per >= kt) continue;   // an empty split
             const int64_t wgs = tiles * n, slots = edge == 256 ? 256 : 512;
-            const double step = edge == 256 ? 1.7 : wgs <= 256 ? 0.7 : 1.05;
+            const double step = edge == 256 ? 1.75 : wgs <= 256 ? 0.57 : 1.0;
             const double rounds = (double)((wgs + slots - 1) / slots);
             double t = rounds * ((double)per * step + 4.0);
             if (n > 1) t += 4.0 + 8.0 * (double)n * (double)M * (double)N / 4e6;
@@ -392,7 +406,8 @@ inline ProdPlan prod_plan(int64_t M, int64_t N, int64_t K) {
     }
     return best;
 }
-// Few rows run on a kernel whose waves split K, without tiles in LDS.
-constexpr int64_t kFewRows = 32;
+// Few rows run on a kernel whose waves split K, without tiles in LDS. Measured on MI355X (few / tiles, us): 1 x 1536 x 6144
+// 7.0 / 12.8, 8 rows 7.9 / 13.6, 16 rows 8.9 / 12.1; with a second block of 16 rows, 32 rows 14.3 / 12.8.
+constexpr int64_t kFewRows = 16;
 
 }  // namespace sa3k

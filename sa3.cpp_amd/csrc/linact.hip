@@ -494,23 +494,19 @@ __global__ __launch_bounds__(256) void prod_sum_kernel(GemmArgs a) {
     finish8<T, FWD>(a, m, n, v);
 }
 
-// Few rows (at most 16 MB): 16 columns of the output a workgroup, whose eight waves split K in steps of 32 and read W
+// Few rows (at most 16): 16 columns of the output a workgroup, whose eight waves split K in steps of 32 and read W
 // straight from memory into the MFMA's registers (each element once); the waves' sums are joined in LDS.
-template <class T, int MB>
+template <class T>
 __global__ __launch_bounds__(512) void prod_few_kernel(GemmArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int W = 8, U = 8;
-    __shared__ float red[W][MB][16][17];
+    __shared__ float red[W][16][17];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15;
     const int64_t n0 = (int64_t)blockIdx.x * 16, wn = n0 + r;
     const int64_t steps = (a.K + 31) / 32;
     const T* wp = static_cast<const T*>(a.B) + min(wn, a.N - 1) * a.ldb;
-    const T* xp[MB];
-#pragma unroll
-    for (int b = 0; b < MB; ++b) xp[b] = static_cast<const T*>(a.A) + min((int64_t)(16 * b + r), a.M - 1) * a.lda;
-    f32x4 acc[MB];
-#pragma unroll
-    for (int b = 0; b < MB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const T* xp = static_cast<const T*>(a.A) + min((int64_t)r, a.M - 1) * a.lda;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     // eight of K at k, zeros past its end (rows and columns past theirs repeat the last one: never stored)
     auto ld = [&](const T* p, int64_t k) {
         x8 v;
@@ -524,35 +520,28 @@ __global__ __launch_bounds__(512) void prod_few_kernel(GemmArgs a) {
         return v;
     };
     for (int64_t s0 = wave; s0 < steps; s0 += W * U) {
-        x8 w[U], x[U][MB];
+        x8 w[U], x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t k = (s0 + u * W) * 32 + 8 * (lane >> 4);
             w[u] = ld(wp, k);
-#pragma unroll
-            for (int b = 0; b < MB; ++b) x[u][b] = ld(xp[b], k);
+            x[u] = ld(xp, k);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int b = 0; b < MB; ++b) {
-                if constexpr (sizeof(T) == 2 && __is_same(T, bf16))
-                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u], x[u][b], acc[b], 0, 0, 0);
-                else
-                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[u], x[u][b], acc[b], 0, 0, 0);
-            }
+        for (int u = 0; u < U; ++u) {
+            if constexpr (__is_same(T, bf16)) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[u], x[u], acc, 0, 0, 0);
+            else acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[u], x[u], acc, 0, 0, 0);
+        }
     }
 #pragma unroll
-    for (int b = 0; b < MB; ++b)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) red[wave][b][r][4 * (lane >> 4) + v] = acc[b][v];
+    for (int v = 0; v < 4; ++v) red[wave][r][4 * (lane >> 4) + v] = acc[v];
     __syncthreads();
-    for (int i = tid; i < MB * 256; i += 512) {
-        const int64_t m = i >> 4, n = n0 + (i & 15);
-        if (m >= a.M || n >= a.N) continue;
+    if (tid < 256) {
+        const int64_t m = tid >> 4, n = n0 + (tid & 15);
+        if (m >= a.M || n >= a.N) return;
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) v += red[w][m >> 4][m & 15][i & 15];
+        for (int w = 0; w < W; ++w) v += red[w][m][tid & 15];
         if (a.bias) v += a.bias[n];
         if (a.Z) static_cast<T*>(a.Z)[m * a.ldz + n] = (T)v;
         v = act_value(v, a.act);
@@ -680,9 +669,7 @@ void fwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     a.C = p.Y; a.ldc = p.ldy; a.act = p.act; a.bias = p.bias; a.R = p.R; a.ldr = p.ldr; a.Z = p.Zo; a.ldz = p.ldz;
     if (p.M <= kFewRows) {
         KernelScope ks(ctx, "linear_act_few", 2.0 * (double)a.M * (double)a.N * (double)a.K);
-        const dim3 grid((unsigned)ceil_div(a.N, 16));
-        if (p.M <= 16) launch_k(ctx, true, prod_few_kernel<T, 1>, grid, dim3(512), 0, a);
-        else launch_k(ctx, true, prod_few_kernel<T, 2>, grid, dim3(512), 0, a);
+        launch_k(ctx, true, prod_few_kernel<T>, dim3((unsigned)ceil_div(a.N, 16)), dim3(512), 0, a);
         SA3K_LAUNCHED();
         return;
     }

@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kThreads) void wattn_join_kernel(FwdArgs a) {
 template <class T, int D>
 void fwd_run(sa3k_ctx* ctx, FwdArgs& a) {
     const AttnShape& s = a.s;
-    if (s.Sq <= kFewQueries) {
+    if (attn_split_keys(s)) {
         a.chunks = (int)ceil_div((int64_t)s.Sq * s.G, 32);
         a.splits = attn_splits(s, a.chunks);
         if (a.splits > 1)

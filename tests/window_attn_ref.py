@@ -70,8 +70,11 @@ CASES = [
          layout="cache", ql=[1, 1, 1], kl=[3000, 200, 1]),
     case("five new tokens, two chunks of rows", b=1, h=16, kv=2, d=128, sq=5, sk=777, left=100, sinks=64, causal=True,
          layout="cache"),
-    case("the most queries that split keys", h=2, kv=2, sq=32, sk=2500, causal=True, layout="cache"),
-    case("one past them", h=2, kv=2, sq=33, sk=2500, causal=True, layout="cache"),
+    case("32 queries, keys split", h=2, kv=2, sq=32, sk=2500, causal=True, layout="cache"),
+    case("33 queries, keys split", h=4, kv=2, sq=33, sk=2500, causal=True, layout="cache", ql=[33], kl=[2441]),
+    case("33 queries, few keys: tiles", h=2, kv=2, sq=33, sk=1500, causal=True, layout="cache"),
+    case("many heads, few keys: tiles", b=3, h=96, kv=2, sq=2, sk=70, causal=True, layout="cache", ql=[2, 1, 2], kl=[70, 3, 66]),
+    case("200 queries over many keys, split", h=2, kv=1, d=128, sq=200, sk=3500, left=3000, causal=True, sinks=4, layout="cache"),
     case("split over many workgroups", h=1, sq=3, sk=20000, layout="cache", d=128),
     case("small scale", sq=80, scale=0.01),
 ]
