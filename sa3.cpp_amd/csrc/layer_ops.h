@@ -233,15 +233,15 @@ inline int64_t keys_seen(const AttnShape& s) {
     return (reach < s.Sk ? reach : s.Sk) + s.sinks;
 }
 // Whether the keys are split over workgroups and waves, 32 rows (query, member of the group) at a time, instead of running by
-// tiles of 128 queries a head. Measured on MI355X (tiles / split, us; 32 heads of 128 on 8, all keys visible):
-//   one query:       1 x 16384 keys 337 / 20.0, 8 x 4096 keys 87 / 30
-//   32 queries:      1 x 16384 keys 289 / 35.6, 8 x 2048 keys 41 / 35, 8 x 512 keys 13.3 / 21.7
-//   64 queries:      1 x 16384 keys 300 / 54
-// Tiles win where there are rows for more than one chunk, few keys and enough heads to fill the chip.
+// tiles of 128 queries a head. Measured on MI355X (tiles / split, us; bf16, all keys visible but where a window is named):
+//   one query, 32 heads of 128 on 8:   1 x 16384 keys 337 / 20.0, 8 x 4096 keys 87 / 30, 8 x 512 keys 14.7 / 11.6
+//   32 queries of such heads:          1 x 16384 keys 289 / 35.6, 8 x 2048 keys 41 / 35, 8 x 512 keys 13.3 / 21.7
+//   self-attention, by its tiles:      24 tiles 9.6 / 7.3, 64 tiles 19.1 / 11.2, 120 tiles 13.9 / 11.5, 128 tiles 46.5 / 35.8 and
+//                                      (window 256) 9.5 / 8.8, 160 tiles 29.1 / 32.5, 192 tiles 18.2 / 20.7, 432 tiles 28.5 / 43
+// The split serves where there are rows for one chunk only, or too few tiles for the chip.
 inline bool attn_split_keys(const AttnShape& s) {
-    const int64_t tiles = (int64_t)s.B * s.H * ((s.Sq + 127) / 128), keys = keys_seen(s);
-    if (s.Sq <= 32) return s.Sq * s.G <= 32 || tiles < 256 || keys > 1024;
-    return tiles < 128 && keys >= 2048;
+    const int64_t tiles = (int64_t)s.B * s.H * ((s.Sq + 127) / 128);
+    return (int64_t)s.Sq * s.G <= 32 || tiles <= 128 || (s.Sq <= 32 && keys_seen(s) > 1024);
 }
 // The split count for `chunks` chunks of 32 rows a key/value head: a workgroup a CU in all (8 x one query over windows of 4096
 // keys: 128 / 256 / 512 / 1024 workgroups 34.0 / 29.5 / 33.1 / 41.5 us), at least two blocks of 32 keys a wave.

@@ -89,4 +89,6 @@ void plan(int64_t M, int64_t N, int64_t K, int* out) {
     out[0] = p.edge; out[1] = p.splits; out[2] = p.per;
 }
 
+int split_keys(const int* i, const int64_t* st) { return attn_split_keys(attn_shape(shape(i, 1.f, st), nullptr, nullptr)); }
+
 }  // extern "C"

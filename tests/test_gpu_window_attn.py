@@ -10,7 +10,7 @@ import torch
 
 from conftest import sa3k
 from layer_ops_util import TORCH, TYPE, U32, down, draw, half_step, up
-from window_attn_ref import CASES, case, forward, visible
+from window_attn_ref import CASES, case, forward, widened
 
 pytestmark = pytest.mark.gpu
 SENTINEL = 9.0
@@ -105,6 +105,17 @@ def check_forward(c, kind, o, lse, r):
 @pytest.mark.parametrize("c", CASES, ids=[c["name"] for c in CASES])
 def test_forward(ctx, c, kind):
     run = Run(ctx, c, kind)
+    o, lse = run.forward()
+    check_forward(c, kind, o, lse, run.reference())
+
+
+WIDE = [w for w in map(widened, CASES) if w]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("c", WIDE, ids=[c["name"] for c in WIDE])
+def test_forward_by_tiles(ctx, c, kind):
+    run = Run(ctx, c, kind, seed=21)
     o, lse = run.forward()
     check_forward(c, kind, o, lse, run.reference())
 

@@ -217,6 +217,24 @@ def test_key_items(host):
         assert 1 <= few.value <= 512
 
 
+def test_split_keys(host):
+    """the rule that picks the forward's kernel, and that the widened cases of the attention's tests run by tiles"""
+    from window_attn_ref import CASES, widened
+
+    def split(c):
+        i = (sa3k.TYPE_BF16, c["batch"], c["heads"], c["kv"], c["dim"], c["sq"], c["sk"], c["left"], c["right"], c["sinks"],
+             int(c["causal"]))
+        return host.split_keys((C.c_int * 11)(*i), (C.c_int64 * 12)(*[8] * 12))
+
+    base = dict(batch=1, heads=32, kv=8, dim=128, sq=1, sk=100, left=-1, right=-1, sinks=0, causal=True)
+    assert split(base) == 1 and split(dict(base, sq=512)) == 1 and split(dict(base, sq=513)) == 0
+    assert split(dict(base, batch=8, sq=8)) == 1 and split(dict(base, batch=8, sq=9)) == 0
+    assert split(dict(base, batch=8, sq=32, sk=1025)) == 1 and split(dict(base, batch=8, sq=33, sk=1025)) == 0
+    wide = [w for w in map(widened, CASES) if w]
+    assert len(wide) > 15 and not any(split(w) for w in wide)
+    assert any(split(c) for c in CASES)
+
+
 PROD_P = ("x", "w", "r", "dy", "z", "y", "zo", "dx", "dw", "bias", "db")
 
 

@@ -46,6 +46,15 @@ def case(name, b=1, h=2, kv=None, d=64, sq=1, sk=None, left=-1, right=-1, sinks=
                 kl is not None, layout=layout, scale=scale or d ** -0.5)
 
 
+def widened(c):
+    """the case with so many heads that it runs by tiles of 128 queries; None where it never does"""
+    g = c["heads"] // c["kv"]
+    if c["sq"] * g <= 32 or (c["sq"] <= 32 and c["sk"] > 1024):
+        return None
+    f = 128 // (c["batch"] * c["heads"] * -(-c["sq"] // 128)) + 1
+    return dict(c, name=c["name"] + ", many heads", heads=c["heads"] * f, kv=c["kv"] * f)
+
+
 CASES = [
     case("one token", h=3),
     case("a few tokens", h=2, kv=1, sq=5),
@@ -72,8 +81,8 @@ CASES = [
          layout="cache"),
     case("32 queries, keys split", h=2, kv=2, sq=32, sk=2500, causal=True, layout="cache"),
     case("33 queries, keys split", h=4, kv=2, sq=33, sk=2500, causal=True, layout="cache", ql=[33], kl=[2441]),
-    case("33 queries, few keys: tiles", h=2, kv=2, sq=33, sk=1500, causal=True, layout="cache"),
-    case("many heads, few keys: tiles", b=3, h=96, kv=2, sq=2, sk=70, causal=True, layout="cache", ql=[2, 1, 2], kl=[70, 3, 66]),
+    case("33 queries, few keys", h=2, kv=2, sq=33, sk=1500, causal=True, layout="cache"),
+    case("many heads, few keys", b=3, h=96, kv=2, sq=2, sk=70, causal=True, layout="cache", ql=[2, 1, 2], kl=[70, 3, 66]),
     case("200 queries over many keys, split", h=2, kv=1, d=128, sq=200, sk=3500, left=3000, causal=True, sinks=4, layout="cache"),
     case("split over many workgroups", h=1, sq=3, sk=20000, layout="cache", d=128),
     case("small scale", sq=80, scale=0.01),
