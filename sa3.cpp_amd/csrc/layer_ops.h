@@ -267,18 +267,25 @@ inline KeySplit key_split(const AttnShape& s) {
     const int64_t most = s.G * all, usual = s.G * (band < all ? band : all);
     const int64_t pairs = (int64_t)s.B * s.K, later = r.tiles - r.first_tiles;
     // By estimated time in microseconds, measured on MI355X: two workgroups that share a CU take 0.9 (heads of 64) or 1.95 (of
-    // 128) each for a block of 64 queries, one alone 1.35 times that, and a workgroup starts within the time of two blocks; the
-    // launch that adds up shares takes 4, its sums 4 MB a microsecond.
+    // 128) each for a block, one alone 1.35 times that, and a workgroup starts within the time of two blocks; the pass by queries
+    // in the same launch takes 0.85 of that a block. The launch lasts as long as its work or its longest workgroup; the one that
+    // adds up shares 4, its sums 4 MB a microsecond. (What it chooses is within 5% of the best of 1 to 8 shares on eight shapes:
+    // 2 x 24 x 1088, window 128 both ways, 64 first tokens: whole 44.6 us, the first tile in two shares 46.6.)
     const double block = s.D == 64 ? 0.9 : 1.95, share = 2.0 * kKeyTile * s.D * 4 * 2 / 4e6;
+    const int64_t q_wgs = (int64_t)s.B * s.H * ((s.Sq + 127) / 128), k_all = (s.Sk + 63) / 64;
+    const int64_t k_band = ((int64_t)128 + s.left + s.right + 62) / 64 + 1 + (s.sinks + 63) / 64;
+    const double by_query = 0.85 * (double)q_wgs * (double)((k_band < k_all ? k_band : k_all) + 2);
     double least = 1e300;
     r.first = r.rest = 1;
     for (int64_t n = 1; n <= 64 && (n == 1 || usual / n >= 4); ++n) {   // at least four blocks a workgroup
         const int64_t len = (usual + n - 1) / n;
         for (int64_t f = r.first_tiles > 0 ? n : 1; f <= 256 && (f == n || f == 1 || most / f >= 4); ++f) {
-            const int64_t flen = (most + f - 1) / f;
+            const int64_t flen = (most + f - 1) / f, longest = r.first_tiles > 0 && flen > len ? flen : later > 0 ? len : flen;
             const int64_t wgs = pairs * (r.first_tiles * f + later * n);
-            const double turns = wgs <= 256 ? 1.35 : wgs <= 512 ? 2.0 : (double)wgs / 256.0 + 0.5;
-            double t = turns * ((double)(r.first_tiles > 0 && flen > len ? flen : len) + 2.0) * block;
+            const double work = (double)pairs * (double)(r.first_tiles * most + later * usual) + 2.0 * (double)wgs + by_query;
+            const double all_of_it = work * block / 256.0;
+            const double last = (double)(longest + 2) * block * (wgs + q_wgs <= 256 ? 1.35 : 2.0);
+            double t = all_of_it > last ? all_of_it : last;
             if (n > 1) t += 4.0 + (double)wgs * share;
             else if (r.first_tiles > 0 && f > 1) t += 4.0 + (double)(pairs * r.first_tiles * f) * share;
             if (t < least) {
