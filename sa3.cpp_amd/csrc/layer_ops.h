@@ -389,28 +389,52 @@ inline const char* prod_check(const ProdArgs& a, bool bwd, int* code) {
 // 256 x 256 in four splits 61, whole 125; 4096 x 1024 x 4096: 256 x 256 43, 128 x 128 51).
 struct ProdPlan {
     int edge, splits, per;   // per: tiles of 64 along K that a split takes
+    double us;
 };
+inline double split_sum_us(int64_t n, int64_t M, int64_t N) {
+    return n > 1 ? 4.0 + 8.0 * (double)n * (double)M * (double)N / 4e6 : 0.0;
+}
+inline bool split_fits(int64_t n, int64_t kt, int64_t M, int64_t N) {   // no empty split, at most 256 MB of split sums
+    return n == 1 || (n <= kt && (n - 1) * ((kt + n - 1) / n) < kt && (double)n * (double)M * (double)(N + 8) <= 67108864.0);
+}
 inline ProdPlan prod_plan(int64_t M, int64_t N, int64_t K) {
     const int64_t kt = (K + 63) / 64;
-    ProdPlan best{128, 1, (int)kt};
-    double least = 1e300;
+    ProdPlan best{128, 1, (int)kt, 1e300};
     for (int edge = 256; edge >= 128; edge /= 2) {
         const int64_t tiles = ((M + edge - 1) / edge) * ((N + edge - 1) / edge);
-        for (int64_t n = 1; n <= 16 && n <= kt; ++n) {
-            if (n > 1 && (double)n * (double)M * (double)(N + 8) > 67108864.0) break;   // 256 MB of split sums
-            const int64_t per = (kt + n - 1) / n;
-            if ((n - 1) * per >= kt) continue;   // an empty split
-            const int64_t wgs = tiles * n, slots = edge == 256 ? 256 : 512;
+        for (int64_t n = 1; n <= 16; ++n) {
+            if (!split_fits(n, kt, M, N)) continue;
+            const int64_t per = (kt + n - 1) / n, wgs = tiles * n, slots = edge == 256 ? 256 : 512;
             const double step = edge == 256 ? 1.75 : wgs <= 256 ? 0.57 : 1.0;
-            const double rounds = (double)((wgs + slots - 1) / slots);
-            double t = rounds * ((double)per * step + 4.0);
-            if (n > 1) t += 4.0 + 8.0 * (double)n * (double)M * (double)N / 4e6;
-            if (t < least) {
-                least = t;
-                best = ProdPlan{edge, (int)n, (int)per};
-            }
+            const double t = (double)((wgs + slots - 1) / slots) * ((double)per * step + 4.0) + split_sum_us(n, M, N);
+            if (t < best.us) best = ProdPlan{edge, (int)n, (int)per, t};
         }
     }
+    return best;
+}
+// Two products of a backward pass, in one launch of 128 x 128 tiles or one after the other. Together they last as long as their
+// work, half a microsecond a tile of 64 along K with two workgroups a CU, or their longest workgroup; a launch saved is 4.
+struct ProdPair {
+    bool together;
+    ProdPlan a, b;
+};
+inline ProdPair prod_pair(const int64_t (&x)[3], const int64_t (&y)[3]) {   // {M, N, K} of each
+    ProdPair best{false, prod_plan(x[0], x[1], x[2]), prod_plan(y[0], y[1], y[2])};
+    double least = best.a.us + best.b.us + 4.0;
+    const int64_t ka = (x[2] + 63) / 64, kb = (y[2] + 63) / 64;
+    const int64_t ta = ((x[0] + 127) / 128) * ((x[1] + 127) / 128), tb = ((y[0] + 127) / 128) * ((y[1] + 127) / 128);
+    for (int64_t n = 1; n <= 8; ++n)
+        for (int64_t m = 1; m <= 8; ++m) {
+            if (!split_fits(n, ka, x[0], x[1]) || !split_fits(m, kb, y[0], y[1])) continue;
+            const int64_t pa = (ka + n - 1) / n, pb = (kb + m - 1) / m, wgs = ta * n + tb * m;
+            const double work = 0.5 * ((double)(ta * ka) + (double)(tb * kb) + 4.0 * (double)wgs) / 256.0;
+            const double last = (double)(pa > pb ? pa : pb) * (wgs <= 256 ? 0.65 : 1.0) + 4.0;
+            const double t = (work > last ? work : last) + split_sum_us(n, x[0], x[1]) + split_sum_us(m, y[0], y[1]);
+            if (t < least) {
+                least = t;
+                best = ProdPair{true, ProdPlan{128, (int)n, (int)pa, t}, ProdPlan{128, (int)m, (int)pb, t}};
+            }
+        }
     return best;
 }
 // Few rows run on a kernel whose waves split K, without tiles in LDS. Measured on MI355X (few / tiles, us): 1 x 1536 x 6144

@@ -237,10 +237,10 @@ struct TilePlace {
     bool none;
 };
 template <int EDGE>
-__device__ __forceinline__ TilePlace tile_place(const GemmArgs& a) {
+__device__ __forceinline__ TilePlace tile_place(const GemmArgs& a, int L) {   // L: the workgroup's number among this product's
     const int tiles_m = (int)((a.M + EDGE - 1) / EDGE), tiles_n = (int)((a.N + EDGE - 1) / EDGE);
-    const int nwg = gridDim.x, L = blockIdx.x + nwg * blockIdx.y;
-    const int item = (L & 7) * ((nwg * (int)gridDim.y) >> 3) + (L >> 3);
+    const int nwg = (tiles_m * tiles_n + 7) & ~7;   // a split's workgroups
+    const int item = (L & 7) * ((nwg * a.splits) >> 3) + (L >> 3);
     TilePlace p;
     p.z = __builtin_amdgcn_readfirstlane(item / nwg);
     const int bid = __builtin_amdgcn_readfirstlane(item - p.z * nwg);
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
     constexpr int EDGE = 256, NT = 512, FM = 2, FN = 4, OPB = EDGE * 128, STAGE = 2 * OPB, EROW = EDGE + 8;
     static_assert(64 * EROW * 4 <= 2 * STAGE, "staged rows fit the stages' memory");
     __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-    const TilePlace tp = tile_place<EDGE>(a);
+    const TilePlace tp = tile_place<EDGE>(a, blockIdx.x);
     if (tp.none) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm0 = (wave & 3) * 64, wn0 = (wave >> 2) * 128;
@@ -369,15 +369,14 @@ __global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
 // t + 1 are read and the loads of tile t + STAGES begin to go out into t's piece, a quarter of them a K step. (Loads of tiles past
 // the end give zeros and touch no memory, so that every round has the same number under way.)
 template <class T, int STAGES, bool AK, bool BK, bool FWD>
-__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void prod_tile_kernel(GemmArgs a) {
+__device__ __forceinline__ void tile_body(const GemmArgs& a, int L, char* lds) {
     typedef typename Vec<T>::x8 x8;
     constexpr int EDGE = 128, NT = 256, F = 2, OPB = EDGE * 128, STAGE = 2 * OPB, EROW = EDGE + 8;
     typedef Operand<T, EDGE, NT, AK> OpA;
     typedef Operand<T, EDGE, NT, BK> OpB;
     constexpr int LOADS = OpA::PER + OpB::PER;
     static_assert(64 * EROW * 4 <= STAGES * STAGE, "staged rows fit the stages' memory");
-    __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
-    const TilePlace tp = tile_place<EDGE>(a);
+    const TilePlace tp = tile_place<EDGE>(a, L);
     if (tp.none) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm0 = (wave & 1) * 64, wn0 = (wave >> 1) * 64;
@@ -473,6 +472,22 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void prod_tile_kernel(Gem
     }
 }
 
+template <class T, int STAGES, bool AK, bool BK, bool FWD>
+__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void prod_tile_kernel(GemmArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * 2 * 128 * 128];
+    tile_body<T, STAGES, AK, BK, FWD>(a, blockIdx.x, lds);
+}
+
+// dX (x_wgs workgroups, a multiple of 8) and dW in one launch: each alone leaves CUs empty in its last turn. Measured on MI355X
+// with the pass over dz: 2176 x 1536 x 6144 122 us against 137 one after the other, 1024 x 1024 x 4096 40 against 48,
+// 64 x 1536 x 1536 18 against 23; from about 4096 x 2048 x 2048 on the 256 x 256 tiles' two launches are chosen.
+template <class T>
+__global__ __launch_bounds__(256, 2) void prod_pair_kernel(GemmArgs x, GemmArgs w, int x_wgs) {
+    __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * 128 * 128];
+    if ((int)blockIdx.x < x_wgs) tile_body<T, 2, false, true, false>(x, blockIdx.x, lds);
+    else tile_body<T, 2, true, true, false>(w, (int)blockIdx.x - x_wgs, lds);
+}
+
 // the K splits' sums in their order, then the epilogue
 template <class T, bool FWD>
 __global__ __launch_bounds__(256) void prod_sum_kernel(GemmArgs a) {
@@ -564,10 +579,10 @@ __global__ __launch_bounds__(256) void prod_pad_kernel(const T* src, int64_t ld,
 }
 
 // dz = dY act'(z) [M][pitch] (null: not stored) and its column sums over this workgroup's rows, part [gridDim.y][N] (null:
-// none). A workgroup takes 256 columns, 8 a thread, eight rows at a time.
+// none; a single row of workgroups writes db itself). A workgroup takes 256 columns, 8 a thread, eight rows at a time.
 template <class T>
 __global__ __launch_bounds__(256) void prod_dz_kernel(const T* dY, int64_t lddy, const T* Z, int64_t ldz, int64_t M, int64_t N,
-                                                      int act, T* dz, int64_t pitch, float* part) {
+                                                      int act, T* dz, int64_t pitch, float* part, int accumulate) {
     __shared__ float red[8][256 + 8];
     const int c = (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
     const int64_t n = (int64_t)blockIdx.x * 256 + c;
@@ -597,6 +612,7 @@ __global__ __launch_bounds__(256) void prod_dz_kernel(const T* dY, int64_t lddy,
     float t = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
+    if (gridDim.y == 1 && accumulate) t += part[j];
     part[(int64_t)blockIdx.y * N + j] = t;
 }
 
@@ -638,27 +654,34 @@ size_t split_bytes(const ProdPlan& p, int64_t M, int64_t N) {
     return p.splits > 1 ? (size_t)p.splits * (size_t)M * (size_t)up8(N) * sizeof(float) : 0;
 }
 
-template <class T, bool AK, bool BK, bool FWD>
-void tile_run(sa3k_ctx* ctx, GemmArgs& a, const ProdPlan& p, float* part, const char* name) {
+// the plan's numbers into the arguments; the workgroups of the launch
+int64_t plan_into(GemmArgs& a, const ProdPlan& p, float* part) {
     a.splits = p.splits;
     a.per = p.per;
     a.part = p.splits > 1 ? part : nullptr;
     a.pitch = up8(a.N);
+    return ceil_div(ceil_div(a.M, p.edge) * ceil_div(a.N, p.edge), 8) * 8 * p.splits;
+}
+template <class T, bool FWD>
+void sum_splits(sa3k_ctx* ctx, const GemmArgs& a) {
+    if (a.splits == 1) return;
+    KernelScope ks(ctx, "linear_act_sum");
+    launch_k(ctx, true, prod_sum_kernel<T, FWD>, dim3((unsigned)ceil_div(a.M * (a.pitch / 8), 256)), dim3(256), 0, a);
+    SA3K_LAUNCHED();
+}
+template <class T, bool AK, bool BK, bool FWD>
+void tile_run(sa3k_ctx* ctx, GemmArgs& a, const ProdPlan& p, float* part, const char* name) {
+    const int64_t wgs = plan_into(a, p, part);
     {
-        const int64_t tiles = ceil_div(a.M, p.edge) * ceil_div(a.N, p.edge);
-        const dim3 grid((unsigned)(ceil_div(tiles, 8) * 8), (unsigned)a.splits);
+        const dim3 grid((unsigned)wgs);
         KernelScope ks(ctx, name, 2.0 * (double)a.M * (double)a.N * (double)a.K);
         if (p.edge == 256) launch_k(ctx, a.splits == 1, prod_big_kernel<T, AK, BK, FWD>, grid, dim3(512), 0, a);
-        else if (tiles * a.splits <= 256)   // one workgroup a CU at the most: deeper stages
+        else if (wgs <= 256)   // one workgroup a CU at the most: deeper stages
             launch_k(ctx, a.splits == 1, prod_tile_kernel<T, 4, AK, BK, FWD>, grid, dim3(256), 0, a);
         else launch_k(ctx, a.splits == 1, prod_tile_kernel<T, 2, AK, BK, FWD>, grid, dim3(256), 0, a);
         SA3K_LAUNCHED();
     }
-    if (p.splits > 1) {
-        KernelScope ks(ctx, "linear_act_sum");
-        launch_k(ctx, true, prod_sum_kernel<T, FWD>, dim3((unsigned)ceil_div(a.M * (a.pitch / 8), 256)), dim3(256), 0, a);
-        SA3K_LAUNCHED();
-    }
+    sum_splits<T, FWD>(ctx, a);
 }
 
 template <class T>
@@ -689,8 +712,10 @@ void fwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     tile_run<T, false, false, true>(ctx, a, plan, reinterpret_cast<float*>(ws + os), "linear_act_fwd");
 }
 
-// Row shares of the pass over dY and z: about 128, each of the same number of rounds of eight rows.
+// Row shares of the pass over dY and z: one for up to 64 rows (which saves the launch that adds up shares), else about 128, each
+// of the same number of rounds of eight rows.
 int dz_parts(int64_t M) {
+    if (M <= 64) return 1;
     const int64_t groups = std::max<int64_t>(1, ceil_div(M, 8)), rounds = ceil_div(groups, 128);
     return (int)ceil_div(groups, rounds);
 }
@@ -702,22 +727,25 @@ void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     // dz as the products read it: dY itself, or its own rows
     const bool own_dz = products && M > 0 && (p.act != SA3K_ACT_NONE || !loads16(p.dY, p.lddy, N));
     const bool px = p.dW && M > 0 && !loads16(p.X, p.ldx, K), pw = p.dX && M > 0 && !loads16(p.W, p.ldw, K);
-    const ProdPlan px_plan = prod_plan(M > 0 ? M : 1, K, N), pw_plan = prod_plan(N, K, M > 0 ? M : 1);
+    const bool do_x = p.dX && M > 0, do_w = p.dW != nullptr;
+    ProdPair plan{false, prod_plan(M > 0 ? M : 1, K, N), prod_plan(N, K, M > 0 ? M : 1)};
+    if (do_x && do_w) plan = prod_pair({M, K, N}, {N, K, M});
     const int parts = dz_parts(M);
     Scratch s;
     const size_t oz = s.take(own_dz ? (size_t)M * Np * 2 : 0), ox = s.take(px ? (size_t)M * Kp * 2 : 0);
-    const size_t ow = s.take(pw ? (size_t)N * Kp * 2 : 0), ob = s.take(p.db ? (size_t)parts * N * 4 : 0);
-    const size_t os = s.take(std::max(p.dX ? split_bytes(px_plan, M, K) : 0, p.dW ? split_bytes(pw_plan, N, K) : 0));
+    const size_t ow = s.take(pw ? (size_t)N * Kp * 2 : 0), ob = s.take(p.db && parts > 1 ? (size_t)parts * N * 4 : 0);
+    const size_t sx = do_x ? split_bytes(plan.a, M, K) : 0, sw = do_w ? split_bytes(plan.b, N, K) : 0;
+    const size_t osx = s.take(plan.together ? sx : std::max(sx, sw)), osw = plan.together ? s.take(sw) : osx;
     char* ws = s.need ? reinterpret_cast<char*>(gemm_workspace_bytes(ctx, s.need)) : nullptr;
     T* dz = own_dz ? reinterpret_cast<T*>(ws + oz) : nullptr;
-    float* part = p.db ? reinterpret_cast<float*>(ws + ob) : nullptr;
+    float* part = !p.db ? nullptr : parts > 1 ? reinterpret_cast<float*>(ws + ob) : p.db;
     if (own_dz || p.db) {
         KernelScope ks(ctx, "linear_act_dz");
-        launch_k(ctx, false, prod_dz_kernel<T>, dim3((unsigned)ceil_div(N, 256), (unsigned)parts), dim3(256), 0,
-                 static_cast<const T*>(p.dY), p.lddy, static_cast<const T*>(p.Z), p.ldz, M, N, p.act, dz, Np, part);
+        launch_k(ctx, !products && parts == 1, prod_dz_kernel<T>, dim3((unsigned)ceil_div(N, 256), (unsigned)parts), dim3(256), 0,
+                 static_cast<const T*>(p.dY), p.lddy, static_cast<const T*>(p.Z), p.ldz, M, N, p.act, dz, Np, part, p.accumulate);
         SA3K_LAUNCHED();
     }
-    if (p.db) {
+    if (p.db && parts > 1) {
         KernelScope ks(ctx, "linear_act_db");
         launch_k(ctx, !products, prod_db_kernel, dim3((unsigned)ceil_div(N, 64)), dim3(kColumnSumThreads), 0, part, parts, N, p.db,
                  p.accumulate);
@@ -725,26 +753,38 @@ void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     }
     const void* g = own_dz ? dz : p.dY;
     const int64_t ldg = own_dz ? Np : p.lddy;
-    if (p.dX && M > 0) {   // [M][K] = dz [M][N] . W [N][K]
-        GemmArgs a{};
-        a.A = g; a.lda = ldg;
-        a.B = pw ? padded<T>(ctx, p.W, p.ldw, N, K, ws + ow) : p.W;
-        a.ldb = pw ? Kp : p.ldw;
-        a.M = M; a.N = K; a.K = N;
-        a.C = p.dX; a.ldc = p.lddx;
-        tile_run<T, false, true, false>(ctx, a, px_plan, reinterpret_cast<float*>(ws + os), "linear_act_dx");
+    GemmArgs x{}, w{};
+    if (do_x) {   // [M][K] = dz [M][N] . W [N][K]
+        x.A = g; x.lda = ldg;
+        x.B = pw ? padded<T>(ctx, p.W, p.ldw, N, K, ws + ow) : p.W;
+        x.ldb = pw ? Kp : p.ldw;
+        x.M = M; x.N = K; x.K = N;
+        x.C = p.dX; x.ldc = p.lddx;
     }
-    if (p.dW) {   // [N][K] = dz^T [N][M] . X [M][K]
-        GemmArgs a{};
-        a.A = g; a.lda = ldg;
-        a.B = px ? padded<T>(ctx, p.X, p.ldx, M, K, ws + ox) : p.X;
-        a.ldb = px ? Kp : p.ldx;
-        a.M = N; a.N = K; a.K = M;
-        a.C = p.dW; a.ldc = p.lddw;
-        a.c_f32 = p.dw_type == SA3K_TYPE_F32;
-        a.accumulate = p.accumulate;
-        tile_run<T, true, true, false>(ctx, a, pw_plan, reinterpret_cast<float*>(ws + os), "linear_act_dw");
+    if (do_w) {   // [N][K] = dz^T [N][M] . X [M][K]
+        w.A = g; w.lda = ldg;
+        w.B = px ? padded<T>(ctx, p.X, p.ldx, M, K, ws + ox) : p.X;
+        w.ldb = px ? Kp : p.ldx;
+        w.M = N; w.N = K; w.K = M;
+        w.C = p.dW; w.ldc = p.lddw;
+        w.c_f32 = p.dw_type == SA3K_TYPE_F32;
+        w.accumulate = p.accumulate;
     }
+    float *part_x = reinterpret_cast<float*>(ws + osx), *part_w = reinterpret_cast<float*>(ws + osw);
+    if (plan.together) {
+        const int64_t nx = plan_into(x, plan.a, part_x), nw = plan_into(w, plan.b, part_w);
+        {
+            KernelScope ks(ctx, "linear_act_dx_dw", 4.0 * (double)M * (double)N * (double)K);
+            launch_k(ctx, x.splits == 1 && w.splits == 1, prod_pair_kernel<T>, dim3((unsigned)(nx + nw)), dim3(256), 0, x, w,
+                     (int)nx);
+            SA3K_LAUNCHED();
+        }
+        sum_splits<T, false>(ctx, x);
+        sum_splits<T, false>(ctx, w);
+        return;
+    }
+    if (do_x) tile_run<T, false, true, false>(ctx, x, plan.a, part_x, "linear_act_dx");
+    if (do_w) tile_run<T, true, true, false>(ctx, w, plan.b, part_w, "linear_act_dw");
 }
 
 }  // namespace

@@ -91,4 +91,13 @@ void plan(int64_t M, int64_t N, int64_t K, int* out) {
 
 int split_keys(const int* i, const int64_t* st) { return attn_split_keys(attn_shape(shape(i, 1.f, st), nullptr, nullptr)); }
 
+// together, then edge, splits and per of each
+void pair(const int64_t* x, const int64_t* y, int* out) {
+    const int64_t a[3] = {x[0], x[1], x[2]}, b[3] = {y[0], y[1], y[2]};
+    const ProdPair p = prod_pair(a, b);
+    out[0] = p.together;
+    out[1] = p.a.edge; out[2] = p.a.splits; out[3] = p.a.per;
+    out[4] = p.b.edge; out[5] = p.b.splits; out[6] = p.b.per;
+}
+
 }  // extern "C"

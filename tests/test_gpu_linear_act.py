@@ -19,7 +19,7 @@ F64 = {"none": lambda z: z, "relu": torch.relu, "silu": torch.nn.functional.silu
 
 SHAPES = [(1, 1, 1), (1, 6, 40), (3, 17, 33), (5, 64, 7), (16, 100, 256), (17, 64, 1000), (32, 300, 520), (33, 40, 64),
           (64, 128, 64), (100, 130, 72), (129, 257, 201), (300, 264, 1000), (256, 256, 64), (257, 520, 136), (40, 48, 4096),
-          (1030, 1800, 96), (2050, 2052, 80), (4100, 4360, 72)]
+          (1030, 1800, 96), (2050, 2052, 80), (4100, 4360, 72), (2176, 192, 640), (65, 1536, 1032)]
 
 
 def whole(seed, shape, most=3, kind="f32"):

@@ -298,3 +298,19 @@ def test_prod_plan(host):
         assert splits == 1 or splits * M * (N + 8) <= 1 << 26
         seen.add((edge, splits > 1))
     assert len(seen) == 4   # both tiles, split and not
+
+
+def test_prod_pair(host):
+    """as the plan of one product; together only on tiles of 128"""
+    r = random.Random(6)
+    out, I = (C.c_int * 7)(), C.c_int64 * 3
+    seen = set()
+    for _ in range(2000):
+        M, N, K = (int(2 ** r.uniform(0, 13)) for _ in range(3))
+        host.pair(I(M, K, N), I(N, K, M), out)
+        for (edge, splits, per), (m, n, k) in ((out[1:4], (M, K, N)), (out[4:7], (N, K, M))):
+            kt = -(-k // 64)
+            assert edge == 128 or (edge == 256 and not out[0])
+            assert splits * per >= kt and (splits - 1) * per < kt and (splits == 1 or splits * m * (n + 8) <= 1 << 26)
+        seen.add(out[0])
+    assert seen == {0, 1}
