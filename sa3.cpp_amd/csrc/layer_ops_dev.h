@@ -31,6 +31,23 @@ inline void require_ok(const char* msg, int code) {
     if (msg) sa3k_throw(code, msg);
 }
 
+// The layer operators' scratch, at least `bytes` of it, used in turn on the context's stream. Not the products' workspace: that
+// one's address is in the DiT's captured steps, and these calls, whose needs are larger, would move it by growing it.
+inline float* layer_workspace(sa3k_ctx* ctx, size_t bytes) {
+    if (bytes > ctx->layer_ws_bytes) {
+        SA3K_REQUIRE(!ctx->capturing, "the layer operators' scratch cannot grow while a graph is being captured");
+        if (ctx->layer_ws) {
+            SA3K_HIP(hipStreamSynchronize(ctx->stream));
+            SA3K_HIP(hipFree(ctx->layer_ws));
+            ctx->layer_ws = nullptr;
+            ctx->layer_ws_bytes = 0;
+        }
+        SA3K_HIP(hipMalloc(&ctx->layer_ws, bytes));
+        ctx->layer_ws_bytes = bytes;
+    }
+    return static_cast<float*>(ctx->layer_ws);
+}
+
 // N elements at p, which need only be aligned to their size: global memory takes wide accesses at any
 // address, so a row that starts at an odd element costs one more cache line and no second code path
 template <class T, int N>

@@ -13,10 +13,6 @@
 
 #include "wattn.h"
 
-namespace sa3k {
-float* gemm_workspace_bytes(sa3k_ctx* ctx, size_t bytes);   // gemm.hip: context-owned scratch
-}
-
 namespace {
 using namespace sa3k;
 using wattn::buffer_rsrc;
@@ -703,7 +699,7 @@ void fwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     // (if one operand is padded, both are: they share K)
     const size_t ox = s.take(px || pw ? (size_t)p.M * Kp * 2 : 0), ow = s.take(px || pw ? (size_t)p.N * Kp * 2 : 0);
     const size_t os = s.take(split_bytes(plan, p.M, p.N));
-    char* ws = s.need ? reinterpret_cast<char*>(gemm_workspace_bytes(ctx, s.need)) : nullptr;
+    char* ws = s.need ? reinterpret_cast<char*>(layer_workspace(ctx, s.need)) : nullptr;
     if (px || pw) {
         a.A = padded<T>(ctx, p.X, p.ldx, p.M, p.K, ws + ox);
         a.B = padded<T>(ctx, p.W, p.ldw, p.N, p.K, ws + ow);
@@ -736,7 +732,7 @@ void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     const size_t ow = s.take(pw ? (size_t)N * Kp * 2 : 0), ob = s.take(p.db && parts > 1 ? (size_t)parts * N * 4 : 0);
     const size_t sx = do_x ? split_bytes(plan.a, M, K) : 0, sw = do_w ? split_bytes(plan.b, N, K) : 0;
     const size_t osx = s.take(plan.together ? sx : std::max(sx, sw)), osw = plan.together ? s.take(sw) : osx;
-    char* ws = s.need ? reinterpret_cast<char*>(gemm_workspace_bytes(ctx, s.need)) : nullptr;
+    char* ws = s.need ? reinterpret_cast<char*>(layer_workspace(ctx, s.need)) : nullptr;
     T* dz = own_dz ? reinterpret_cast<T*>(ws + oz) : nullptr;
     float* part = !p.db ? nullptr : parts > 1 ? reinterpret_cast<float*>(ws + ob) : p.db;
     if (own_dz || p.db) {

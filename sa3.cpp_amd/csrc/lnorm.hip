@@ -17,10 +17,6 @@
 
 #include "layer_ops_dev.h"
 
-namespace sa3k {
-float* gemm_workspace_bytes(sa3k_ctx* ctx, size_t bytes);   // gemm.hip: context-owned scratch
-}
-
 namespace {
 using namespace sa3k;
 
@@ -257,7 +253,7 @@ void norm_launch(sa3k_ctx* ctx, const NormArgs& a, bool bwd) {
     // workgroups of the same number of rounds each
     const int64_t rounds = ceil_div(blocks, sums ? kNormBwdGroups : 1 << 20);
     const int grid = (int)ceil_div(blocks, rounds);
-    float* part = sums ? gemm_workspace_bytes(ctx, (size_t)grid * 2 * (size_t)a.cols * sizeof(float)) : nullptr;
+    float* part = sums ? layer_workspace(ctx, (size_t)grid * 2 * (size_t)a.cols * sizeof(float)) : nullptr;
     {
         KernelScope ks(ctx, "layer_norm_bwd");
         launch_k(ctx, !sums, norm_bwd_kernel<T, TG, CH>, dim3((unsigned)grid), thr, 0, a, part);

@@ -185,6 +185,7 @@ SA3K_API void sa3k_destroy(sa3k_ctx* ctx) {
     if (ctx->red_ws_side) (void)hipFree(ctx->red_ws_side);
     if (ctx->gemm_ws_quick) (void)hipFree(ctx->gemm_ws_quick);
     if (ctx->red_ws_quick) (void)hipFree(ctx->red_ws_quick);
+    if (ctx->layer_ws) (void)hipFree(ctx->layer_ws);
     for (hipEvent_t e : ctx->side_ev)
         if (e) (void)hipEventDestroy(e);
     if (ctx->block_tail_ev) (void)hipEventDestroy(ctx->block_tail_ev);

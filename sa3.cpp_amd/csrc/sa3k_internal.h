@@ -96,6 +96,8 @@ struct sa3k_ctx {
     size_t gemm_ws_quick_bytes = 0;
     void* red_ws_quick = nullptr;
     size_t red_ws_quick_bytes = 0;
+    void* layer_ws = nullptr;             // the layer operators' scratch (layer_ops_dev.h)
+    size_t layer_ws_bytes = 0;
     int gemm_fixup = 0;                   // split partials summed by the last split (no reduce launch):
                                           // 0 never, 1 always, 2 for small outputs only
     int* tile_counters = nullptr;         // [kMaxFixupTiles] arrival counters, zero between launches

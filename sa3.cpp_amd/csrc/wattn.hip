@@ -12,10 +12,6 @@
 
 #include "wattn.h"
 
-namespace sa3k {
-float* gemm_workspace_bytes(sa3k_ctx* ctx, size_t bytes);   // gemm.hip: context-owned scratch
-}
-
 namespace {
 using namespace sa3k;
 using namespace sa3k::wattn;
@@ -378,7 +374,7 @@ void fwd_run(sa3k_ctx* ctx, FwdArgs& a) {
         a.chunks = (int)ceil_div((int64_t)s.Sq * s.G, 32);
         a.splits = attn_splits(s, a.chunks);
         if (a.splits > 1)
-            a.part = gemm_workspace_bytes(ctx, (size_t)s.B * s.K * a.chunks * a.splits * 32 * (D + 2) * sizeof(float));
+            a.part = layer_workspace(ctx, (size_t)s.B * s.K * a.chunks * a.splits * 32 * (D + 2) * sizeof(float));
         {
             KernelScope ks(ctx, "window_attn_split");
             launch_k(ctx, a.splits == 1, wattn_split_kernel<T, D>, dim3((unsigned)(s.B * s.K) * a.chunks * a.splits),

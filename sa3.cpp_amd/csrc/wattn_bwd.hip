@@ -12,10 +12,6 @@
 
 #include "wattn.h"
 
-namespace sa3k {
-float* gemm_workspace_bytes(sa3k_ctx* ctx, size_t bytes);   // gemm.hip: context-owned scratch
-}
-
 namespace {
 using namespace sa3k;
 using namespace sa3k::wattn;
@@ -388,7 +384,7 @@ void bwd_run(sa3k_ctx* ctx, BwdArgs& a) {
     const int summed = a.split.rest > 1 ? a.split.tiles : a.split.first > 1 ? a.split.first_tiles : 0;
     const size_t nd = ((size_t)s.B * s.H * s.Sq + 63) / 64 * 64;
     const size_t np = summed ? (size_t)s.B * s.K * a.split.items() * 2 * kKeyTile * D : 0;
-    a.delta = gemm_workspace_bytes(ctx, (nd + np) * sizeof(float));
+    a.delta = layer_workspace(ctx, (nd + np) * sizeof(float));
     a.part = a.delta + nd;
     if (s.Sq > 0) {
         KernelScope ks(ctx, "window_attn_delta");
