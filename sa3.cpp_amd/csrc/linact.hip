@@ -270,7 +270,11 @@ __device__ __forceinline__ void finish_rows(const GemmArgs& a, const TilePlace& 
     }
 }
 
-// Tiles of 256 x 256: eight waves of 64 x 128, one workgroup a CU.
+// Tiles of 256 x 256: eight waves of 64 x 128, one workgroup a CU. Measured on MI355X: 8192^3 bf16 940 us (1170 TFLOP/s),
+// 8191 x 4096 x 8192 f16 512 us (1074) and with gelu_tanh and z stored 547. Bound by the operand loads and LDS reads beside
+// the MFMAs (busy for 54% of the time; with the loads left out 8192^3 takes 800 us). Not kept: four waves of 128 x 128 (579 us
+// against 530 for the last call: its epilogue stalls the only wave of a SIMD), fragments read a step ahead (520 against 512),
+// steps of 32 of K (527).
 template <class T, bool AK, bool BK, bool FWD>
 __global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
     typedef typename Vec<T>::x8 x8;
@@ -363,7 +367,9 @@ __global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
 // fed by itself: the fragments of K step ks + 1 are read between the products of ks. Before the last step's products every wave
 // has read the last of tile t and tile t + 1 has landed; the one barrier a tile is there, and behind it the first fragments of
 // t + 1 are read and the loads of tile t + STAGES begin to go out into t's piece, a quarter of them a K step. (Loads of tiles past
-// the end give zeros and touch no memory, so that every round has the same number under way.)
+// the end give zeros and touch no memory, so that every round has the same number under way.) Measured on MI355X: 2176 x 6144
+// x 1536 with bias and residual 56.7 us (724 TFLOP/s). A CU takes 0.55 us a tile and 64 of K, 0.42 with the loads left out; MFMA
+// busy for 38% of the time.
 template <class T, int STAGES, bool AK, bool BK, bool FWD>
 __device__ __forceinline__ void tile_body(const GemmArgs& a, int L, char* lds) {
     typedef typename Vec<T>::x8 x8;
@@ -506,7 +512,8 @@ __global__ __launch_bounds__(256) void prod_sum_kernel(GemmArgs a) {
 }
 
 // Few rows (at most 16): 16 columns of the output a workgroup, whose eight waves split K in steps of 32 and read W
-// straight from memory into the MFMA's registers (each element once); the waves' sums are joined in LDS.
+// straight from memory into the MFMA's registers (each element once); the waves' sums are joined in LDS. Bound by the latency
+// of a launch and a few rounds of loads: 1 x 1536 x 6144 bf16 7.2 us, 19 MB of W.
 template <class T>
 __global__ __launch_bounds__(512) void prod_few_kernel(GemmArgs a) {
     typedef typename Vec<T>::x8 x8;
@@ -576,6 +583,7 @@ __global__ __launch_bounds__(256) void prod_pad_kernel(const T* src, int64_t ld,
 
 // dz = dY act'(z) [M][pitch] (null: not stored) and its column sums over this workgroup's rows, part [gridDim.y][N] (null:
 // none; a single row of workgroups writes db itself). A workgroup takes 256 columns, 8 a thread, eight rows at a time.
+// Bound by HBM and, with gelu, its arithmetic: 2176 x 6144 bf16 gelu 22.3 us, 80 MB.
 template <class T>
 __global__ __launch_bounds__(256) void prod_dz_kernel(const T* dY, int64_t lddy, const T* Z, int64_t ldz, int64_t M, int64_t N,
                                                       int act, T* dz, int64_t pitch, float* part, int accumulate) {
