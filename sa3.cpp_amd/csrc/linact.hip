@@ -630,16 +630,22 @@ __global__ __launch_bounds__(512) void prod_few_kernel(GemmArgs a) {
     }
 }
 
-// rows [rows][cols] into rows of `pitch` (a multiple of 8), zeros behind them
+// rows [rows][cols] into rows of cols rounded up to a multiple of 8, zeros behind them; two operands in one launch (either may
+// have no rows)
+struct PadArgs {
+    const void* src[2];
+    int64_t ld[2], rows[2], cols;
+    void* dst[2];
+};
 template <class T>
-__global__ __launch_bounds__(256) void prod_pad_kernel(const T* src, int64_t ld, int64_t rows, int64_t cols, T* dst,
-                                                       int64_t pitch) {
-    const int64_t chunks = pitch / 8, n = rows * chunks;
+__global__ __launch_bounds__(256) void prod_pad_kernel(PadArgs a) {
+    const int64_t chunks = (a.cols + 7) / 8, n0 = a.rows[0] * chunks, n = n0 + a.rows[1] * chunks;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+        const int w = i >= n0;
+        const int64_t j = w ? i - n0 : i, r = j / chunks, c = (j - r * chunks) * 8;
         float v[8];
-        load8(src + r * ld, c, cols, v);
-        store8(dst + r * pitch, c, pitch, v);
+        load8(static_cast<const T*>(w ? a.src[1] : a.src[0]) + r * (w ? a.ld[1] : a.ld[0]), c, a.cols, v);
+        store8(static_cast<T*>(w ? a.dst[1] : a.dst[0]) + r * chunks * 8, c, chunks * 8, v);
     }
 }
 
@@ -707,13 +713,12 @@ struct Scratch {
 };
 
 template <class T>
-const T* padded(sa3k_ctx* ctx, const void* p, int64_t ld, int64_t rows, int64_t cols, char* to) {
+void pad(sa3k_ctx* ctx, const PadArgs& a) {
+    const int64_t n = (a.rows[0] + a.rows[1]) * (up8(a.cols) / 8);
+    if (n == 0) return;
     KernelScope ks(ctx, "linear_act_pad");
-    const int64_t n = rows * (up8(cols) / 8);
-    launch_k(ctx, false, prod_pad_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 65536)), dim3(256), 0,
-             static_cast<const T*>(p), ld, rows, cols, reinterpret_cast<T*>(to), up8(cols));
+    launch_k(ctx, false, prod_pad_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 65536)), dim3(256), 0, a);
     SA3K_LAUNCHED();
-    return reinterpret_cast<const T*>(to);
 }
 
 size_t split_bytes(const ProdPlan& p, int64_t M, int64_t N) {
@@ -771,8 +776,9 @@ void fwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     const size_t os = s.take(split_bytes(plan, p.M, p.N));
     char* ws = s.need ? reinterpret_cast<char*>(layer_workspace(ctx, s.need)) : nullptr;
     if (px || pw) {
-        a.A = padded<T>(ctx, p.X, p.ldx, p.M, p.K, ws + ox);
-        a.B = padded<T>(ctx, p.W, p.ldw, p.N, p.K, ws + ow);
+        pad<T>(ctx, PadArgs{{p.X, p.W}, {p.ldx, p.ldw}, {p.M, p.N}, p.K, {ws + ox, ws + ow}});
+        a.A = ws + ox;
+        a.B = ws + ow;
         a.lda = a.ldb = a.K = Kp;
     }
     tile_run<T, false, false, true>(ctx, a, plan, reinterpret_cast<float*>(ws + os), "linear_act_fwd");
@@ -820,16 +826,17 @@ void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     const void* g = own_dz ? dz : p.dY;
     const int64_t ldg = own_dz ? Np : p.lddy;
     GemmArgs x{}, w{};
+    pad<T>(ctx, PadArgs{{p.W, p.X}, {p.ldw, p.ldx}, {pw ? N : 0, px ? M : 0}, K, {ws + ow, ws + ox}});
     if (do_x) {   // [M][K] = dz [M][N] . W [N][K]
         x.A = g; x.lda = ldg;
-        x.B = pw ? padded<T>(ctx, p.W, p.ldw, N, K, ws + ow) : p.W;
+        x.B = pw ? ws + ow : p.W;
         x.ldb = pw ? Kp : p.ldw;
         x.M = M; x.N = K; x.K = N;
         x.C = p.dX; x.ldc = p.lddx;
     }
     if (do_w) {   // [N][K] = dz^T [N][M] . X [M][K]
         w.A = g; w.lda = ldg;
-        w.B = px ? padded<T>(ctx, p.X, p.ldx, M, K, ws + ox) : p.X;
+        w.B = px ? ws + ox : p.X;
         w.ldb = px ? Kp : p.ldx;
         w.M = N; w.N = K; w.K = M;
         w.C = p.dW; w.ldc = p.lddw;
