@@ -135,6 +135,21 @@ def test_backward_against_differences(ctx):
         assert abs(float(dw.numpy()[i, j]) - num) <= float(e[:, i] @ a[:, j].abs()) + 1e-5
 
 
+@pytest.mark.parametrize("odd", ["x", "w", "dy"])
+def test_one_operand_off_its_alignment(ctx, odd):
+    """only one operand has rows that the wide loads cannot take: exact on whole numbers, forward and backward"""
+    M, N, K = 140, 72, 104
+    x, w, dy = whole(1, (M, K), kind="f16"), whole(2, (N, K), kind="f16"), whole(3, (M, N), 2, "f16")
+    px, pw, pd = (Pitched(ctx, t, t.shape[1] + (3 if n == odd else 0), 1 if n == odd else 0)
+                  for n, t in (("x", x), ("w", w), ("dy", dy)))
+    y, dx, dw = (ctx.zeros(s, np.uint16) for s in ((M, N), (M, K), (N, K)))
+    sa3k.linear_act_fwd(ctx, TYPE["f16"], ACTS["none"], px, pw, M, N, K, y, ldx=px.ld, ldw=pw.ld)
+    sa3k.linear_act_bwd(ctx, TYPE["f16"], ACTS["none"], pd, px, pw, M, N, K, dx=dx, dw=dw, lddy=pd.ld, ldx=px.ld, ldw=pw.ld)
+    X, W, D = x.double(), w.double(), dy.double()
+    for got, want in ((y, X @ W.t()), (dx, D @ W), (dw, D.t() @ X)):
+        assert torch.equal(down(got, "f16"), want.to(torch.float16))
+
+
 def test_long_sums(ctx):
     """random values over a long K, split over workgroups: K U of the terms' absolute sum at most"""
     M, N, K = 70, 90, 20000
