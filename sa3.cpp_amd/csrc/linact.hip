@@ -274,7 +274,8 @@ __device__ __forceinline__ TilePlace tile_place(const GemmArgs& a, int L) {   //
 
 // The end of a tile: 64 rows of its sums at a time, staged in LDS as f32; a thread finishes 8 columns, the same in every
 // round, of four of the rows. The bias is read once, a round's residual before its sums are staged, so that the rounds do
-// not wait for memory one after the other (2176 x 6144 x 1536 with both read in place: 56.7 us).
+// not wait for memory one after the other (with both read in place and the activation branched on for each value, 8191 x 4096 x
+// 8192 f16 gelu_tanh with z took 547 us against 514, 2176 x 1536 x 6144 gelu 62.5 against 56.4).
 template <class T, bool FWD, int EDGE, int NT, int EROW>
 struct Finish {
     static constexpr int CPR = EDGE / 8, STEP = NT / CPR, ROUNDS = 64 / STEP;   // threads a row; rows a round
@@ -319,11 +320,11 @@ struct Finish {
     }
 };
 
-// Tiles of 256 x 256: eight waves of 64 x 128, one workgroup a CU. Measured on MI355X: 8192^3 bf16 940 us (1170 TFLOP/s),
-// 8191 x 4096 x 8192 f16 512 us (1074) and with gelu_tanh and z stored 547. Bound by the operand loads and LDS reads beside
-// the MFMAs (busy for 54% of the time; with the loads left out 8192^3 takes 800 us). Not kept: four waves of 128 x 128 (579 us
-// against 530 for the last call: its epilogue stalls the only wave of a SIMD), fragments read a step ahead (520 against 512),
-// steps of 32 of K (527).
+// Tiles of 256 x 256: eight waves of 64 x 128, one workgroup a CU. Measured on MI355X: 8192^3 bf16 925 us (1190 TFLOP/s),
+// 8191 x 4096 x 8192 bf16 463 us, f16 488 and with gelu_tanh and z stored 514. Bound by the operand loads and LDS reads beside
+// the MFMAs (busy for 54% of the time; with the loads left out 8192^3 takes 800 us). Not kept (f16, each against the kernel of its
+// time): four waves of 128 x 128, 579 us against 530 (its epilogue stalls the only wave of a SIMD); fragments read a step
+// ahead, 519 against 512; steps of 32 of K, 527 against 512.
 template <class T, bool AK, bool BK, bool FWD>
 __global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
     typedef typename Vec<T>::x8 x8;
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
 // has read the last of tile t and tile t + 1 has landed; the one barrier a tile is there, and behind it the first fragments of
 // t + 1 are read and the loads of tile t + STAGES begin to go out into t's piece, a quarter of them a K step. (Loads of tiles past
 // the end give zeros and touch no memory, so that every round has the same number under way.) Measured on MI355X: 2176 x 6144
-// x 1536 with bias and residual 56.7 us (724 TFLOP/s). A CU takes 0.55 us a tile and 64 of K, 0.42 with the loads left out; MFMA
+// x 1536 with bias and residual 54.1 us (759 TFLOP/s). A CU takes 0.55 us a tile and 64 of K, 0.42 with the loads left out; MFMA
 // busy for 38% of the time.
 template <class T, int STAGES, bool AK, bool BK, bool FWD>
 __device__ __forceinline__ void tile_body(const GemmArgs& a, int L, char* lds) {
@@ -536,7 +537,7 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void prod_tile_kernel(Gem
 }
 
 // dX (x_wgs workgroups, a multiple of 8) and dW in one launch: each alone leaves CUs empty in its last turn. Measured on MI355X
-// with the pass over dz: 2176 x 1536 x 6144 122 us against 137 one after the other, 1024 x 1024 x 4096 40 against 48,
+// with the pass over dz, as it was then: 2176 x 1536 x 6144 122 us (114 now) against 137 one after the other, 1024 x 1024 x 4096 40 against 48,
 // 64 x 1536 x 1536 18 against 23; from about 4096 x 2048 x 2048 on the 256 x 256 tiles' two launches are chosen.
 template <class T>
 __global__ __launch_bounds__(256, 2) void prod_pair_kernel(GemmArgs x, GemmArgs w, int x_wgs) {
@@ -651,7 +652,7 @@ __global__ __launch_bounds__(256) void prod_pad_kernel(PadArgs a) {
 
 // dz = dY act'(z) [M][pitch] (null: not stored) and its column sums over this workgroup's rows, part [gridDim.y][N] (null:
 // none; a single row of workgroups writes db itself). A workgroup takes 256 columns, 8 a thread, eight rows at a time.
-// Bound by HBM and, with gelu, its arithmetic: 2176 x 6144 bf16 gelu 22.3 us, 80 MB.
+// Bound by HBM: 2176 x 6144 bf16 gelu 17.2 us, 80 MB, 4.7 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void prod_dz_kernel(const T* dY, int64_t lddy, const T* Z, int64_t ldz, int64_t M, int64_t N,
                                                       int act, T* dz, int64_t pitch, float* part, int accumulate) {
