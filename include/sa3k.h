@@ -503,7 +503,8 @@ enum {
  *   z = X W^T + bias,  Y = act(z) + residual
  * X [M][K], W [N][K], residual, Y and z [M][N]; bias f32 [N]; bias, residual and z nullable. Activation and residual
  * apply to the f32 z; Y and z are each rounded once. Any M (0: nothing), N and K, row pitches below 2^22. Y may
- * be the residual itself (same pitch). */
+ * be the residual itself (same pitch). NaN and infinities go through the formulas as they stand: a NaN z gives NaN, z = -inf
+ * does with silu and the gelus (infinity times 0). */
 SA3K_API int sa3k_linear_act_fwd(sa3k_ctx* ctx, int type, int act, const void* X, int64_t ldx, const void* W, int64_t ldw,
                                  const float* bias, const void* residual, int64_t ldr, int64_t M, int64_t N, int64_t K,
                                  void* Y, int64_t ldy, void* Z, int64_t ldz);
@@ -511,7 +512,8 @@ SA3K_API int sa3k_linear_act_fwd(sa3k_ctx* ctx, int type, int act, const void* X
 /* Its backward from dY and the stored z (Z may be null without an activation): dz = dY act'(z),
  *   dX = dz W,  dW = dz^T X,  db = sum_rows dz    (each nullable; the residual's gradient is dY itself)
  * dz is rounded to `type` for the two products, not for db. dw_type: `type`, or f32; accumulate = 1 adds to dW
- * (f32 only) and db. relu's slope at 0 is 0. Sums run in a fixed order. */
+ * (f32 only) and db. relu's slope at 0 is 0. act' is NaN at a NaN z, and with silu and the gelus at an infinite one (0 times
+ * infinity). Sums run in a fixed order. */
 SA3K_API int sa3k_linear_act_bwd(sa3k_ctx* ctx, int type, int act, const void* dY, int64_t lddy, const void* Z, int64_t ldz,
                                  const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t M, int64_t N, int64_t K,
                                  void* dX, int64_t lddx, void* dW, int dw_type, int64_t lddw, float* db, int accumulate);

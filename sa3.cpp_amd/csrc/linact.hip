@@ -45,8 +45,8 @@ struct GemmArgs {
     int splits, per;
 };
 
-// The activations on the hardware's exp2 and reciprocal. For gelu_tanh, (1 + tanh u) / 2 = 1 / (1 + e^-2u); its argument is
-// held within +-10, where it is 0 or 1 in f32, so that a large z^3 does not overflow. For gelu, (1 + erf(z / sqrt 2)) / 2 by
+// The activations on the hardware's exp2 and reciprocal. For gelu_tanh, (1 + tanh u) / 2 = 1 / (1 + e^-2u), which is 0 or 1 where
+// a large z^3 overflows to an infinity. NaN and infinities go through the formulas as they stand. For gelu, (1 + erf(z / sqrt 2)) / 2 by
 // Abramowitz and Stegun's approximation 7.1.26 of erf (off by at most 1.5e-7): with x = |z| / sqrt 2 and t = 1 / (1 + 0.3275911 x),
 // 1 - erf x = (a1 t + .. + a5 t^5) e^-x^2, whose exponential is also the slope's. (The library's erff made the pass over dY and z
 // bound by its arithmetic.)
@@ -66,10 +66,9 @@ __device__ __forceinline__ float gelu(float z) {
     float bell;
     return z * normal_below(z, bell);
 }
-__device__ __forceinline__ float gelu_tanh(float z) {
-    const float y = fminf(fmaxf(z, -10.f), 10.f);
-    return z * sigmoid(1.5957691216057308f * (y + 0.044715f * y * y * y));
-}
+// (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2
+__device__ __forceinline__ float tanh_gate(float z) { return sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z)); }
+__device__ __forceinline__ float gelu_tanh(float z) { return z * tanh_gate(z); }
 // act of N values (one branch for all: their chains of dependent instructions run side by side)
 template <int N>
 __device__ __forceinline__ void act_values(float (&v)[N], int act) {
@@ -88,7 +87,7 @@ __device__ __forceinline__ void act_values(float (&v)[N], int act) {
     }
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
-    if (act == SA3K_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if (act == SA3K_ACT_RELU) return z <= 0.f ? 0.f : z > 0.f ? 1.f : z;   // (NaN stays NaN)
     if (act == SA3K_ACT_SILU) {
         const float g = sigmoid(z);
         return g * (1.f + z * (1.f - g));
@@ -99,9 +98,10 @@ __device__ __forceinline__ float act_slope(float z, int act) {
         return below + z * bell * 0.39894228040143268f;
     }
     if (act == SA3K_ACT_GELU_TANH) {
-        const float y = fminf(fmaxf(z, -10.f), 10.f);
-        const float g = sigmoid(1.5957691216057308f * (y + 0.044715f * y * y * y));
-        return g + y * g * (1.f - g) * 1.5957691216057308f * (1.f + 0.134145f * y * y);
+        // Past +-10 g (1 - g) is below 2^-125, and its factors need not grow on: z^2 of a finite z must not overflow. z times 0
+        // leaves a NaN or an infinite z a NaN, as the formula does.
+        const float g = tanh_gate(z), y = fminf(fmaxf(z, -10.f), 10.f);
+        return __builtin_fmaf(y * g * (1.f - g) * 1.5957691216057308f, 1.f + 0.134145f * y * y, g) + 0.f * z;
     }
     return 1.f;
 }
