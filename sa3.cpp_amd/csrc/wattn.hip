@@ -89,7 +89,8 @@ struct Running {
 #pragma unroll
             for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[h][v]);
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx > m + kLazy) != 0, 0)) {   // a maximum moved far
+        // a maximum moved far (the difference is exact where it matters; m + kLazy may round to m + 16 past 2^27)
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(mx - m > kLazy) != 0, 0)) {
             const float mn = fmaxf(m, mx);
             const float al = ex2(m - (mn == -INFINITY ? 0.f : mn));   // 0 when m was -inf
             m = mn;
