@@ -258,6 +258,8 @@ constexpr int kKeyTile = 128;
 struct KeySplit {
     int tiles, first_tiles, first, rest;   // first_tiles of the tiles hold first tokens
     SA3K_HD int items() const { return first_tiles * first + (tiles - first_tiles) * rest; }   // workgroups a k/v head
+    // those whose sums a second launch adds up, and which have a place in the scratch: they come first among the items
+    SA3K_HD int shares() const { return rest > 1 ? items() : first > 1 ? first_tiles * first : 0; }
 };
 inline KeySplit key_split(const AttnShape& s) {
     KeySplit r;

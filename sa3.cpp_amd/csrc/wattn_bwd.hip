@@ -29,7 +29,7 @@ struct BwdArgs {
     float* delta;   // [B][H][Sq]
     void *dq, *dk, *dv;
     KeySplit split;
-    float* part;    // per (sample, key/value head, item) dk [128][D] and dv [128][D], of tiles with more than one share
+    float* part;    // per (sample, key/value head, share) dk [128][D] and dv [128][D], of tiles with more than one share
 };
 
 template <class T>
@@ -319,7 +319,7 @@ __device__ __forceinline__ void dkdv_body(const BwdArgs& a, int index, char* lds
         store_row<T, D>(static_cast<T*>(a.dv) + voff, dv, 1.f, hl);
         return;
     }
-    float* pk = a.part + ((int64_t)bk * a.split.items() + item) * (2 * kKeyTile * D) + (wave * 32 + c32) * D;
+    float* pk = a.part + ((int64_t)bk * a.split.shares() + item) * (2 * kKeyTile * D) + (wave * 32 + c32) * D;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(kThreads) void wattn_dkdv_sum_kernel(BwdArgs a, int
     const bool first = tile < a.split.first_tiles;
     const int n = first ? a.split.first : a.split.rest;
     const int item = first ? tile * n : a.split.first_tiles * a.split.first + (tile - a.split.first_tiles) * n;
-    const float* p = a.part + ((int64_t)bk * a.split.items() + item) * (2 * kKeyTile * D) + (int64_t)r * D + d0;
+    const float* p = a.part + ((int64_t)bk * a.split.shares() + item) * (2 * kKeyTile * D) + (int64_t)r * D + d0;
     float x[2][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[0][e] = x[1][e] = 0.f;
@@ -391,7 +391,7 @@ void bwd_run(sa3k_ctx* ctx, BwdArgs& a) {
     // tiles whose shares a second launch adds up: those with first tokens only, or all
     const int summed = a.split.rest > 1 ? a.split.tiles : a.split.first > 1 ? a.split.first_tiles : 0;
     const size_t nd = ((size_t)s.B * s.H * s.Sq + 63) / 64 * 64;
-    const size_t np = summed ? (size_t)s.B * s.K * a.split.items() * 2 * kKeyTile * D : 0;
+    const size_t np = (size_t)s.B * s.K * a.split.shares() * 2 * kKeyTile * D;
     a.delta = layer_workspace(ctx, (nd + np) * sizeof(float));
     a.part = a.delta + nd;
     if (s.Sq > 0) {

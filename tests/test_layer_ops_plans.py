@@ -1,0 +1,58 @@
+"""What the layer operators' launches take (csrc/layer_ops.h, host arithmetic): the scratch of shared key tiles, and that the GPU
+tests' shapes reach the variants that they are there for."""
+import ctypes as C
+import os
+import random
+import subprocess
+
+import pytest
+
+from conftest import PKG, ROOT, sa3k
+from layer_ops_shapes import FIRST_SHARED
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("layer_ops_plans") / "liblayer_ops_plans.so")
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(ROOT, "include"),
+           "-I", os.path.join(PKG, "csrc"), os.path.join(ROOT, "tests", "host", "layer_ops_plan_shim.cpp"), "-o", out]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-4000:]
+    return C.CDLL(out)
+
+
+def shares(host, batch, heads, kv, dim, sq, sk, left=-1, right=-1, sinks=0, causal=True):
+    """tiles, tiles with first tokens, shares of those, shares of the others, workgroups, places in the scratch"""
+    out = (C.c_int * 6)()
+    host.key_shares((C.c_int * 11)(sa3k.TYPE_BF16, batch, heads, kv, dim, sq, sk, left, right, sinks, int(causal)), out)
+    return tuple(out)
+
+
+def test_scratch_holds_the_shares_and_no_more(host):
+    """a place for every workgroup of a tile that more than one takes, in the order of the workgroups, none for the others"""
+    r = random.Random(1)
+    seen = set()
+    for _ in range(3000):
+        K, s = r.choice([1, 2, 8]), int(2 ** r.uniform(0, 14))
+        tiles, first_tiles, first, rest, wgs, places = shares(
+            host, r.randint(1, 4), K * r.choice([1, 4]), K, r.choice([64, 128]), s, s, r.choice([-1, 16, 500, 4000]),
+            r.choice([-1, 16, 500]), r.choice([0, 4, 200]), r.random() < 0.5)
+        assert wgs == first_tiles * first + (tiles - first_tiles) * rest
+        split = [n > 1 for t in range(tiles) for n in [first if t < first_tiles else rest] for _ in range(n)]
+        assert places == sum(split) and all(split[:places])
+        seen.add((first_tiles > 0, first > 1, rest > 1))
+    assert {(True, True, False), (True, True, True), (False, False, True), (False, False, False)} <= seen
+
+
+@pytest.mark.parametrize("batch,s,left,most", [(2, 8192, 1023, 2), (4, 32768, 127, 3), (4, 131072, 127, 3)])
+def test_long_windows_with_first_tokens_take_little_scratch(host, batch, s, left, most):
+    """32 on 8 heads of 128, 4 first tokens: only their tile is shared out, whatever the length"""
+    tiles, first_tiles, first, rest, wgs, places = shares(host, batch, 32, 8, 128, s, s, left, 0, 4)
+    assert (first_tiles, rest) == (1, 1) and wgs >= s // 128 and places == first and 1 < places <= most
+
+
+@pytest.mark.parametrize("c", FIRST_SHARED, ids=[c["name"] for c in FIRST_SHARED])
+def test_shapes_share_first_tokens_only(host, c):
+    tiles, first_tiles, first, rest, _, _ = shares(host, c["batch"], c["heads"], c["kv"], c["dim"], c["sq"], c["sk"], c["left"],
+                                                   c["right"], c["sinks"], c["causal"])
+    assert first > 1 and rest == 1 and tiles > first_tiles > 0
