@@ -261,7 +261,7 @@ struct KeySplit {
     // those whose sums a second launch adds up, and which have a place in the scratch: they come first among the items
     SA3K_HD int shares() const { return rest > 1 ? items() : first > 1 ? first_tiles * first : 0; }
 };
-inline KeySplit key_split(const AttnShape& s) {
+inline KeySplit key_split(const AttnShape& s, int* priced = nullptr) {   // priced: the plans that were
     KeySplit r;
     r.tiles = (s.Sk + kKeyTile - 1) / kKeyTile;
     r.first_tiles = (s.sinks + kKeyTile - 1) / kKeyTile;
@@ -277,27 +277,39 @@ inline KeySplit key_split(const AttnShape& s) {
     const int64_t q_wgs = (int64_t)s.B * s.H * ((s.Sq + 127) / 128), k_all = (s.Sk + 63) / 64;
     const int64_t k_band = ((int64_t)128 + s.left + s.right + 62) / 64 + 1 + (s.sinks + 63) / 64;
     const double by_query = 0.85 * (double)q_wgs * (double)((k_band < k_all ? k_band : k_all) + 2);
+    // The work and the sums grow with either count: a plan that is dearer by these alone ends the search in that direction, and so
+    // does one whose first tiles' shares are no longer than the others'. (Priced one by one, the plans of 32 on 1 heads of 64 x 1024
+    // took 47 us of host time in every call, of 16 on 2 x 8192 with a window of 4096 105 us; now 0.4 and 0.1.)
     double least = 1e300;
+    int count = 0;
     r.first = r.rest = 1;
     for (int64_t n = 1; n <= 64 && (n == 1 || usual / n >= 4); ++n) {   // at least four blocks a workgroup
-        const int64_t len = (usual + n - 1) / n;
-        for (int64_t f = r.first_tiles > 0 ? n : 1; f <= 256 && (f == n || f == 1 || most / f >= 4); ++f) {
-            const int64_t flen = (most + f - 1) / f, longest = r.first_tiles > 0 && flen > len ? flen : later > 0 ? len : flen;
+        const int64_t len = (usual + n - 1) / n, f0 = r.first_tiles > 0 ? n : 1;
+        bool dearer = false;   // at f0: so is every larger n
+        for (int64_t f = f0; f <= 256 && (f == n || f == 1 || most / f >= 4); ++f) {
             const int64_t wgs = pairs * (r.first_tiles * f + later * n);
             const double work = (double)pairs * (double)(r.first_tiles * most + later * usual) + 2.0 * (double)wgs + by_query;
             const double all_of_it = work * block / 256.0;
+            const double sums = n > 1 ? 4.0 + (double)wgs * share
+                                : r.first_tiles > 0 && f > 1 ? 4.0 + (double)(pairs * r.first_tiles * f) * share : 0.0;
+            ++count;
+            if (all_of_it + sums >= least) {
+                dearer = f == f0;
+                break;
+            }
+            const int64_t flen = (most + f - 1) / f, longest = r.first_tiles > 0 && flen > len ? flen : later > 0 ? len : flen;
             const double last = (double)(longest + 2) * block * (wgs + q_wgs <= 256 ? 1.35 : 2.0);
-            double t = all_of_it > last ? all_of_it : last;
-            if (n > 1) t += 4.0 + (double)wgs * share;
-            else if (r.first_tiles > 0 && f > 1) t += 4.0 + (double)(pairs * r.first_tiles * f) * share;
+            const double t = (all_of_it > last ? all_of_it : last) + sums;
             if (t < least) {
                 least = t;
                 r.rest = (int)n;
                 r.first = (int)f;
             }
-            if (r.first_tiles == 0) break;
+            if (r.first_tiles == 0 || (later > 0 && flen <= len)) break;
         }
+        if (dearer || later == 0) break;   // (with no other tiles n says nothing)
     }
+    if (priced) *priced = count;
     return r;
 }
 struct KeyItem {

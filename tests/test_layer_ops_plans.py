@@ -56,3 +56,29 @@ def test_shapes_share_first_tokens_only(host, c):
     tiles, first_tiles, first, rest, _, _ = shares(host, c["batch"], c["heads"], c["kv"], c["dim"], c["sq"], c["sk"], c["left"],
                                                    c["right"], c["sinks"], c["causal"])
     assert first > 1 and rest == 1 and tiles > first_tiles > 0
+
+
+def search(host, batch, heads, kv, dim, sq, sk, left=-1, right=-1, sinks=0, causal=True):
+    """(shares of tiles with first tokens, of the others) as chosen, the plans priced for that, and the cheapest of all plans"""
+    out = (C.c_int * 5)()
+    host.key_search((C.c_int * 11)(sa3k.TYPE_BF16, batch, heads, kv, dim, sq, sk, left, right, sinks, int(causal)), out)
+    return (out[0], out[1]), out[2], (out[3], out[4])
+
+
+def test_key_split_finds_the_cheapest_plan(host):
+    r = random.Random(2)
+    for _ in range(4000):
+        K, sq = r.choice([1, 2, 4, 8]), int(2 ** r.uniform(0, 16))
+        sk = sq if r.random() < 0.7 else int(2 ** r.uniform(0, 16))
+        args = (r.randint(1, 8), K * r.choice([1, 2, 4, 8, 32]), K, r.choice([64, 128]), sq, sk, r.choice([-1, 0, 16, 1000]),
+                r.choice([-1, 0, 16, 500]), r.choice([0, 1, 4, 64, 200, 5000, 1 << 20]), r.random() < 0.5)
+        chosen, _, best = search(host, *args)
+        assert chosen == best, args
+
+
+@pytest.mark.parametrize("args", [(3, 16, 2, 128, 2049, 2049, 511, 0, 4), (1, 32, 8, 128, 8192, 8192, 1023, 0, 4),
+                                  (1, 32, 8, 128, 32768, 32768, 1023, 0, 4), (1, 32, 1, 64, 1024, 1024, -1, -1, 4),
+                                  (1, 16, 2, 128, 8192, 8192, 4095, 0, 4), (2, 24, 24, 64, 1088, 1088, 128, 128, 64, False)])
+def test_key_split_prices_few_plans(host, args):
+    """each call of the backward chooses anew: a plan takes about 8 ns to price, so that 64 of them are half a microsecond"""
+    assert search(host, *args)[1] <= 64
