@@ -133,12 +133,15 @@ struct Sa3kError : std::runtime_error {
 
 inline void sa3k_throw(int code, const std::string& msg) { throw Sa3kError(code, msg); }
 
+// (the runtime's own note of the failure is cleared: the next launch's check would find it and fail that call too)
 #define SA3K_HIP(call)                                                                            \
     do {                                                                                          \
         hipError_t e_ = (call);                                                                   \
-        if (e_ != hipSuccess)                                                                     \
+        if (e_ != hipSuccess) {                                                                   \
+            (void)hipGetLastError();                                                              \
             sa3k_throw(e_ == hipErrorOutOfMemory ? SA3K_ERR_NOMEM : SA3K_ERR_DEVICE,              \
                        std::string(#call) + ": " + hipGetErrorString(e_));                        \
+        }                                                                                         \
     } while (0)
 
 #define SA3K_REQUIRE(cond, msg)                                                                   \
