@@ -49,4 +49,17 @@ void key_search(const int* i, int* out) {
         }
 }
 
+// out: edge and splits of a product of M x N x K
+void product(int64_t M, int64_t N, int64_t K, int* out) {
+    const ProdPlan p = prod_plan(M, N, K);
+    out[0] = p.edge; out[1] = p.splits;
+}
+// a backward's dX [M][K] and dW [N][K]; out: together, then edge and splits of each
+void backward(int64_t M, int64_t N, int64_t K, int* out) {
+    const int64_t x[3] = {M, K, N}, w[3] = {N, K, M};
+    const ProdPair p = prod_pair(x, w);
+    out[0] = p.together;
+    out[1] = p.a.edge; out[2] = p.a.splits; out[3] = p.b.edge; out[4] = p.b.splits;
+}
+
 }  // extern "C"

@@ -8,7 +8,7 @@ import subprocess
 import pytest
 
 from conftest import PKG, ROOT, sa3k
-from layer_ops_shapes import FIRST_SHARED
+from layer_ops_shapes import BACKWARD, FIRST_SHARED, FORWARD
 
 
 @pytest.fixture(scope="module")
@@ -82,3 +82,44 @@ def test_key_split_finds_the_cheapest_plan(host):
 def test_key_split_prices_few_plans(host, args):
     """each call of the backward chooses anew: a plan takes about 8 ns to price, so that 64 of them are half a microsecond"""
     assert search(host, *args)[1] <= 64
+
+
+def product(host, M, N, K):
+    """edge of the tiles, splits of K"""
+    out, I = (C.c_int * 2)(), C.c_int64
+    host.product(I(M), I(N), I(K), out)
+    return tuple(out)
+
+
+def backward(host, M, N, K):
+    """dX and dW together, edge and splits of dX, of dW"""
+    out, I = (C.c_int * 5)(), C.c_int64
+    host.backward(I(M), I(N), I(K), out)
+    return tuple(out)
+
+
+@pytest.mark.parametrize("shape", list(FORWARD))
+def test_forward_shapes_reach_their_tiles(host, shape):
+    M, N, K = shape
+    for k in (K, -(-K // 8) * 8):   # as they are, and in padded rows
+        edge, splits = product(host, M, N, k)
+        assert (edge, splits > 1) == FORWARD[shape]
+    assert -(-K // 64) >= 6 or shape == (7563, 1048, 16)
+
+
+@pytest.mark.parametrize("shape", list(BACKWARD))
+def test_backward_shapes_reach_their_tiles(host, shape):
+    together, ex, sx, ew, sw = backward(host, *shape)
+    assert (bool(together), ex, sx > 1, ew, sw > 1) == BACKWARD[shape]
+
+
+def test_shapes_cover_every_variant(host):
+    """those of 4000 drawn shapes, of up to 2^13 rows, columns and length"""
+    assert set(FORWARD.values()) == {(128, False), (128, True), (256, False), (256, True)}
+    r, seen = random.Random(3), set()
+    for _ in range(4000):
+        together, ex, sx, ew, sw = backward(host, *(int(2 ** r.uniform(4, 13.2)) for _ in range(3)))
+        seen.add((bool(together), ex, sx > 1, ew, sw > 1))
+    assert seen <= set(BACKWARD.values()), seen - set(BACKWARD.values())
+    M, N, K = 1313, 1739, 9179   # its single gradients are there on 256 x 256 tiles, too
+    assert product(host, M, K, N)[0] == product(host, N, K, M)[0] == 256
