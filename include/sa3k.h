@@ -433,7 +433,8 @@ SA3K_API int sa3k_diff_attn_bwd(sa3k_ctx* ctx, const void* q1, const void* k1, c
 
 /* Layer norm of rows [rows][cols] (cols <= 16384), type f32, f16 or bf16, optionally of the sum with a
  * residual:
- *   s = x + residual, rounded to `type` (residual null: s = x), stored to sum when that is not null;
+ *   s = x + residual, rounded to `type`, stored to sum when that is not null; residual null: s = x, and sum must be
+ *       null too;
  *   mean = sum_c s / cols, rstd = 1 / sqrt(sum_c (s - mean)^2 / cols + eps)      (f32, nullable outputs [rows])
  *   y = (s - mean) rstd gamma + beta            (gamma null: 1, beta null: 0; f32 [cols])
  * y or sum may be x or residual itself (same pitch). */
@@ -485,7 +486,9 @@ SA3K_API int sa3k_window_attn_fwd(sa3k_ctx* ctx, const sa3k_window_attn* d, cons
  *   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij dO_i,
  * the sums of dk and dv also over the query heads of their group. Written, not added to, in a fixed order of
  * summation; rows past a sample's lengths stay as they were. p and ds are rounded to `type` for these products
- * (f16: gradients smaller than about 2^-24 a pair are lost, as in any f16 backward without loss scaling). */
+ * (f16: gradients smaller than about 2^-24 a pair are lost, as in any f16 backward without loss scaling). lse is f32: p is
+ * off by up to 2^-24 |lse| of itself. Within the lengths q, o and dO must be finite as k and v must: a hidden pair's p and
+ * ds are 0, but 0 times an infinite or NaN value is NaN. */
 SA3K_API int sa3k_window_attn_bwd(sa3k_ctx* ctx, const sa3k_window_attn* d, const void* q, const void* k, const void* v,
                                   const void* o, const float* lse, const void* dO, const int32_t* q_len,
                                   const int32_t* k_len, void* dq, void* dk, void* dv);

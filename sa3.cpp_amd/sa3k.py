@@ -665,7 +665,7 @@ def _p(a):
 
 def layer_norm_fwd(ctx, type, x, rows, cols, gamma, beta, eps, y, mean=None, rstd=None, residual=None, sum=None,
                    ldx=None, ldr=None, ldsum=None, ldy=None):
-    """y = layer norm of x (+ residual, the sum stored to `sum`); every argument with a `.ptr`, pitches in
+    """y = layer norm of x (+ residual, the sum stored to `sum`, which needs one); every argument with a `.ptr`, pitches in
     elements (None: cols)"""
     ctx.check(ctx.lib.sa3k_layer_norm_fwd(ctx.h, type, _p(x), cols if ldx is None else ldx, _p(residual),
                                           cols if ldr is None else ldr, rows, cols, _p(gamma), _p(beta), eps, _p(sum),
