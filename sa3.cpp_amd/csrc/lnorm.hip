@@ -284,7 +284,7 @@ void norm_run(sa3k_ctx* ctx, const NormArgs& a, bool bwd) {
     else if (ch <= 256) norm_launch<T, 64, 4>(ctx, a, bwd);
     else if (M > 4 && ch <= 64 * 6) norm_launch<T, 64, (M > 4 ? 6 : 4)>(ctx, a, bwd);
     else if (M > 4 && ch <= 64 * 8) norm_launch<T, 64, M>(ctx, a, bwd);
-    else if (ch <= 256 * 2) norm_launch<T, 256, 2>(ctx, a, bwd);
+    else if (M == 4 && ch <= 256 * 2) norm_launch<T, 256, (M == 4 ? 2 : 4)>(ctx, a, bwd);   // (f32: a wave takes these)
     else if (ch <= 256 * 4) norm_launch<T, 256, 4>(ctx, a, bwd);
     else if (M > 4 && ch <= 256 * 8) norm_launch<T, 256, M>(ctx, a, bwd);
     else norm_launch<T, 512, M>(ctx, a, bwd);

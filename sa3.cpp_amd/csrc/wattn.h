@@ -161,10 +161,6 @@ __device__ __forceinline__ void wait_tile(int later) {
     asm volatile("s_barrier" ::: "memory");
 }
 
-// this wave's LDS writes are done; then a barrier, past which the other waves see them (loads stay under way)
-__device__ __forceinline__ void wait_lds_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
 // The sums of a loop, after it, as the registers that the loop used. Without this the compiler takes the vectors apart for
 // the code behind the loop and copies every element to a register of its own in every round.
 template <int N>
