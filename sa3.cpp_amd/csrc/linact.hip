@@ -656,6 +656,8 @@ __global__ __launch_bounds__(256) void prod_pad_kernel(PadArgs a) {
     }
 }
 
+// dz is rounded to the tensors' type, which the matrix units read and which halves its way through memory: against 64 bits dX and dW are
+// off by 2.3e-3 of their norm in bf16, where their own rounding alone gives 1.7e-3; db is of dz before that.
 // dz = dY act'(z) [M][pitch] (null: not stored) and its column sums over this workgroup's rows, part [gridDim.y][N] (null:
 // none; a single row of workgroups writes db itself). A workgroup takes 256 columns, 8 a thread, eight rows at a time.
 // Bound by HBM: 2176 x 6144 bf16 gelu 17.2 us, 80 MB, 4.7 TB/s.

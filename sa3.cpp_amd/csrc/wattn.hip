@@ -9,6 +9,11 @@
 // 32-key half; O^T += V^T P^T (A: V read transposed from LDS, B: P^T as the lane holds it) leaves it with its own query's
 // dims, so neither maximum, sum nor rescale needs another lane than l ^ 32.
 //
+// Weights are rounded to the tensors' type for the product with V, whose operands the matrix units take in 16 bits; their sum l is
+// of the weights before that, in f32. That adds half a step a weight to o: against 64 bits o is off by 2.3e-3 of its norm in
+// bf16 and 2.8e-4 in f16, where rounding o alone gives 1.7e-3 and 2.1e-4. (Both halves of a weight, high and low, would be exact at
+// twice the products with V.)
+//
 // Measured on MI355X: 2 x 24 heads of 64 x 1088, window 128 both ways, 64 first tokens, bf16 14.7 us (270 TFLOP/s of visible
 // pairs); 32 heads of 128 on 8 x 8192, causal window of 1024, 169 us (760 TFLOP/s); one query of each of 8 samples, 32 heads on 8,
 // a window of 4096 keys, 32.4 us (4.1 TB/s of keys and values).

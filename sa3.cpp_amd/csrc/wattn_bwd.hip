@@ -3,7 +3,9 @@
 //   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij dO_i
 // Two passes, each over the scores of every visible block, so that no sum is shared between workgroups (no atomics:
 // the same bits in every run): one by queries (dq), one by keys (dk, dv, over all the query heads of a group). Seven
-// products of 2 D a pair where five would do with dq summed by atomics.
+// products of 2 D a pair where five would do with dq summed by atomics. p and ds are rounded to the tensors' type for the products
+// that take them, as the matrix units read 16 bits: against 64 bits the gradients are off by 2.4e-3 of their norm in bf16 and
+// 3.0e-4 in f16, where their own rounding alone gives 1.7e-3 and 2.1e-4.
 //
 // Measured on MI355X (whole calls): 2 x 24 heads of 64 x 1088, window 128 both ways, 64 first tokens, bf16 41 us; 3 x 16 heads of
 // 128 on 2, up to 2049 tokens, causal window of 512, 4 first tokens, f16 124 to 131 us (350 TFLOP/s of five products). Bound by the work
