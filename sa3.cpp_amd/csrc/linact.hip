@@ -281,7 +281,7 @@ __device__ __forceinline__ TilePlace tile_place(const GemmArgs& a, int L) {   //
 // The end of a tile: 64 rows of its sums at a time, staged in LDS as f32; a thread finishes 8 columns, the same in every
 // round, of four of the rows. The bias is read once, a round's residual before its sums are staged, so that the rounds do
 // not wait for memory one after the other (with both read in place and the activation branched on for each value, 8191 x 4096 x
-// 8192 f16 gelu_tanh with z took 547 us against 514, 2176 x 1536 x 6144 gelu 62.5 against 56.4).
+// 8192 f16 gelu_tanh with z took 546 us against 513, 2176 x 1536 x 6144 gelu with z 62.5 against 56.2, in turn on one box).
 template <class T, bool FWD, int EDGE, int NT, int EROW>
 struct Finish {
     static constexpr int CPR = EDGE / 8, STEP = NT / CPR, ROUNDS = 64 / STEP;   // threads a row; rows a round
@@ -326,9 +326,10 @@ struct Finish {
     }
 };
 
-// Tiles of 256 x 256: eight waves of 64 x 128, one workgroup a CU. Measured on MI355X: 8192^3 bf16 925 us (1190 TFLOP/s),
-// 8191 x 4096 x 8192 bf16 463 us, f16 488 and with gelu_tanh and z stored 514. Bound by the operand loads and LDS reads beside
-// the MFMAs (busy for 54% of the time; with the loads left out 8192^3 takes 800 us). Not kept (f16, each against the kernel of its
+// Tiles of 256 x 256: eight waves of 64 x 128, one workgroup a CU. Measured on MI355X: 8192^3 bf16 872 us (1260 TFLOP/s),
+// 8191 x 4096 x 8192 bf16 460 us, f16 486 and with gelu_tanh and z stored 510 to 518 (in the first calls after a pause 575). Bound by
+// the operand loads and LDS reads beside the MFMAs (busy for 58% of the time; without the loads 8192^3 took 800 us against 925, as they
+// were then). Not kept (f16, each against the kernel of its
 // time): four waves of 128 x 128, 579 us against 530 (its epilogue stalls the only wave of a SIMD); fragments read a step
 // ahead, 519 against 512; steps of 32 of K, 527 against 512.
 template <class T, bool AK, bool BK, bool FWD>
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
 // t + 1 are read and the loads of tile t + STAGES begin to go out into t's piece, a quarter of them a K step. (Loads of tiles past
 // the end give zeros and touch no memory, so that every round has the same number under way.) Measured on MI355X: 2176 x 6144
 // x 1536 with bias and residual 54.1 us (759 TFLOP/s). A CU takes 0.55 us a tile and 64 of K, 0.42 with the loads left out; MFMA
-// busy for 38% of the time.
+// busy for 40% of the time.
 template <class T, int STAGES, bool AK, bool BK, bool FWD>
 __device__ __forceinline__ void tile_body(const GemmArgs& a, int L, char* lds) {
     typedef typename Vec<T>::x8 x8;
@@ -542,9 +543,9 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void prod_tile_kernel(Gem
     tile_body<T, STAGES, AK, BK, FWD>(a, blockIdx.x, lds);
 }
 
-// dX (x_wgs workgroups, a multiple of 8) and dW in one launch: each alone leaves CUs empty in its last turn. Measured on MI355X
-// with the pass over dz, as it was then: 2176 x 1536 x 6144 122 us (114 now) against 137 one after the other, 1024 x 1024 x 4096 40 against 48,
-// 64 x 1536 x 1536 18 against 23; from about 4096 x 2048 x 2048 on the 256 x 256 tiles' two launches are chosen.
+// dX (x_wgs workgroups, a multiple of 8) and dW in one launch: each alone leaves CUs empty in its last turn. Measured on MI355X:
+// 2176 x 1536 -> 6144 bf16 103 us (797 TFLOP/s) against 113 one after the other; prod_pair has more shapes. Large ones run on the 256 x
+// 256 tiles' two launches (4096 x 4096 -> 4096 236 us, 1163 TFLOP/s).
 template <class T>
 __global__ __launch_bounds__(256, 2) void prod_pair_kernel(GemmArgs x, GemmArgs w, int x_wgs) {
     __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * 128 * 128];
@@ -656,10 +657,10 @@ __global__ __launch_bounds__(256) void prod_pad_kernel(PadArgs a) {
     }
 }
 
-// dz is rounded to the tensors' type, which the matrix units read and which halves its way through memory: against 64 bits dX and dW are
-// off by 2.3e-3 of their norm in bf16, where their own rounding alone gives 1.7e-3; db is of dz before that.
 // dz = dY act'(z) [M][pitch] (null: not stored) and its column sums over this workgroup's rows, part [gridDim.y][N] (null:
 // none; a single row of workgroups writes db itself). A workgroup takes 256 columns, 8 a thread, eight rows at a time.
+// dz is rounded to the tensors' type, as the matrix units read 16 bits; db is of dz before that. Against 64 bits dX and dW are off by
+// 2.3e-3 of their norm in bf16, where their own rounding alone gives 1.7e-3.
 // Bound by HBM: 2176 x 6144 bf16 gelu 17.2 us, 80 MB, 4.7 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void prod_dz_kernel(const T* dY, int64_t lddy, const T* Z, int64_t ldz, int64_t M, int64_t N,

@@ -15,8 +15,8 @@
 // twice the products with V.)
 //
 // Measured on MI355X: 2 x 24 heads of 64 x 1088, window 128 both ways, 64 first tokens, bf16 14.7 us (270 TFLOP/s of visible
-// pairs); 32 heads of 128 on 8 x 8192, causal window of 1024, 169 us (760 TFLOP/s); one query of each of 8 samples, 32 heads on 8,
-// a window of 4096 keys, 32.4 us (4.1 TB/s of keys and values).
+// pairs); 32 heads of 128 on 8 x 8192, causal window of 1024, 166 to 172 us (750 to 778 TFLOP/s); one query of each of 8 samples, 32 heads on 8,
+// a window of 4096 keys, 32.0 us (4.2 TB/s of keys and values).
 #include <algorithm>
 
 #include "wattn.h"
@@ -127,7 +127,7 @@ struct Running {
 };
 
 // 128 queries of one head a workgroup, 32 a wave; tiles of 64 keys, whose loads run STAGES - 1 tiles ahead (three or four
-// stages gained nothing). Bound by the work of a block on its SIMD: of a block's time the matrix units are busy for 43% with heads
+// stages gained nothing). Bound by the work of a block on its SIMD: of a block's time the matrix units are busy for 42% with heads
 // of 128 and 18% with heads of 64, the rest are the exponentials, the conversions and the reads of K and V, which the two waves
 // of a SIMD hide in each other only partly. A grid that passes over the chip little more than once, as 2 x 24 x 1088 does, lasts
 // as long as its eight blocks one after the other, 1.3 us each. Two heads of a group a workgroup, which halves the loads of

@@ -8,7 +8,7 @@
 // 3.0e-4 in f16, where their own rounding alone gives 1.7e-3 and 2.1e-4.
 //
 // Measured on MI355X (whole calls): 2 x 24 heads of 64 x 1088, window 128 both ways, 64 first tokens, bf16 41 us; 3 x 16 heads of
-// 128 on 2, up to 2049 tokens, causal window of 512, 4 first tokens, f16 124 to 131 us (350 TFLOP/s of five products). Bound by the work
+// 128 on 2, up to 2049 tokens, causal window of 512, 4 first tokens, f16 131 us (350 TFLOP/s of five products). Bound by the work
 // of a block on its SIMD, as the forward: the matrix units are busy for 37% of the time with heads of 128 and 22% with heads of
 // 64; the sums fill a lane's registers, so that two waves a SIMD is all there is. Not kept: pairs of waves that share a tile,
 // one for dk and one for dv (dK/dV pass 116 us against 78), three waves a SIMD with heads of 64 (47 us against 40).
