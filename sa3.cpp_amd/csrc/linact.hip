@@ -281,7 +281,7 @@ __device__ __forceinline__ TilePlace tile_place(const GemmArgs& a, int L) {   //
 // The end of a tile: 64 rows of its sums at a time, staged in LDS as f32; a thread finishes 8 columns, the same in every
 // round, of four of the rows. The bias is read once, a round's residual before its sums are staged, so that the rounds do
 // not wait for memory one after the other (with both read in place and the activation branched on for each value, 8191 x 4096 x
-// 8192 f16 gelu_tanh with z took 546 us against 513, 2176 x 1536 x 6144 gelu with z 62.5 against 56.2, in turn on one box).
+// 8192 f16 gelu_tanh with z took 546 us against 513, 2176 x 1536 x 6144 gelu with z 62.5 against 56.2, in turn on one card).
 template <class T, bool FWD, int EDGE, int NT, int EROW>
 struct Finish {
     static constexpr int CPR = EDGE / 8, STEP = NT / CPR, ROUNDS = 64 / STEP;   // threads a row; rows a round
