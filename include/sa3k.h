@@ -521,6 +521,45 @@ SA3K_API int sa3k_linear_act_bwd(sa3k_ctx* ctx, int type, int act, const void* d
                                  const void* X, int64_t ldx, const void* W, int64_t ldw, int64_t M, int64_t N, int64_t K,
                                  void* dX, int64_t lddx, void* dW, int dw_type, int64_t lddw, float* db, int accumulate);
 
+/* RMS norm of the heads of q and k with the position rotation in the same pass, between a projection and an attention. */
+typedef struct {
+    int type;             /* SA3K_TYPE_F32, _F16 or _BF16, of every tensor */
+    int batch, tokens;
+    int heads, kv_heads;  /* of q; of k and v */
+    int head_dim;         /* a multiple of 8, at most 256 */
+    int rope_dims;        /* the first elements of a head, which are rotated: a multiple of 16 (0: none) */
+    int neighbours;       /* the pairs: 0 (i, i + rope_dims / 2), 1 (2i, 2i + 1) */
+    int cache_tokens;     /* rows a sample of k_out and v_out has, where slots are given */
+    float eps;
+    float rope_base;      /* >= 1 */
+    /* distances in elements between samples, tokens and heads; a head's elements lie together. Inputs may repeat (0);
+     * an output's rows lie apart. */
+    int64_t q_stride[3], k_stride[3], v_stride[3], q_out_stride[3], k_out_stride[3], v_out_stride[3];
+} sa3k_head_norm;
+
+/* For each head x of q and of k, of token t of sample b:
+ *   n = x / sqrt(mean x^2 + eps) * gain,  y = n with pair i of its first rope_dims elements turned by
+ *   pos rope_base^(-2i / rope_dims) radians: (a, c) -> (a cos - c sin, c cos + a sin)
+ * q_gain and k_gain f32 [head_dim] (null: ones). pos device int32 [batch][tokens] (null: t; any value, the angles are exact
+ * modulo a turn to 2^-33 turns). q, k and v with their outputs are each nullable; v is copied. slot device int32 [batch][tokens] (nullable): the
+ * row of k_out and v_out that a token's k and v go to, else row t; a slot outside 0 .. cache_tokens - 1 is not stored, and the
+ * slots of a sample that are must differ. len device int32 [batch] (nullable): tokens past a sample's length are not read, and
+ * their outputs stay as they were. q_out may be q with the same strides; k_out and v_out likewise without slots. Sums and angles f32,
+ * outputs rounded once. Tensors need only be aligned to their elements. */
+SA3K_API int sa3k_head_norm_fwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const void* q, const void* k, const void* v,
+                                const float* q_gain, const float* k_gain, const int32_t* pos, const int32_t* slot,
+                                const int32_t* len, void* q_out, void* k_out, void* v_out);
+
+/* Its backward from the outputs' gradients, which lie as q_out and k_out do (row t; there are no slots): with w the gradient
+ * turned back and h = w gain, r = 1 / sqrt(mean x^2 + eps),
+ *   dx = r (h - x r mean(h x r)),  dgain = sum over tokens and heads of w x r
+ * dq and dk lie as q and k do and may be dq_out and dk_out themselves (same strides). q and k (with their gradients) and the gains'
+ * gradients (f32 [head_dim]) are each nullable; accumulate = 1 adds to the latter. Tokens past a sample's length are not read, add nothing,
+ * and their gradients stay as they were. Sums run in a fixed order. */
+SA3K_API int sa3k_head_norm_bwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const void* q, const void* k, const void* dq_out,
+                                const void* dk_out, const float* q_gain, const float* k_gain, const int32_t* pos,
+                                const int32_t* len, void* dq, void* dk, float* dq_gain, float* dk_gain, int accumulate);
+
 /* ---------------------------------------------------------------- C3: one DiT block */
 
 /* Shape of a (differential) DiT block, the DitConfig fields dit_block reads (src/dit.h:20-46). */

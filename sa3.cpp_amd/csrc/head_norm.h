@@ -1,0 +1,112 @@
+// Host-side arithmetic of the head norms with rotation: the checks of their arguments, the frequencies and the shape of
+// the launches. No HIP in here: compiled with g++ in the CPU tests too.
+#pragma once
+
+#include <cmath>
+
+#include "layer_ops.h"
+
+namespace sa3k {
+
+constexpr int kHeadMaxDim = 256;
+constexpr int kHeadMaxTokens = 1 << 28;
+
+struct HeadPtrs {
+    const void *q = nullptr, *k = nullptr, *v = nullptr;      // the projections
+    const void *dqo = nullptr, *dko = nullptr;                // backward: the outputs' gradients
+    const void *q_gain = nullptr, *k_gain = nullptr, *pos = nullptr, *slot = nullptr, *len = nullptr;
+    void *qo = nullptr, *ko = nullptr, *vo = nullptr;         // forward: the outputs; backward: dq and dk in qo and ko
+    void *dq_gain = nullptr, *dk_gain = nullptr;
+    int accumulate = 0;
+};
+
+// one tensor's strides over (samples, tokens, heads) and its address; out: it is written
+inline const char* head_tensor_check(const void* p, const int64_t* st, const int64_t* n, int dim, int bytes, bool out) {
+    if (!elem_aligned(p, bytes)) return "a tensor is not aligned to its elements";
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && (st[i] < 0 || st[i] >= kMaxStride)) return "a stride is negative or out of range";
+    if (out && !rows_apart(st, n, dim)) return "the rows of an output overlap";
+    return nullptr;
+}
+// x and y may be the same tensor, not two views of one address
+inline bool same_place(const void* x, const void* y, const int64_t* sx, const int64_t* sy, const int64_t* n) {
+    if (!x || x != y) return true;
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && sx[i] != sy[i]) return false;
+    return true;
+}
+
+inline const char* head_norm_check(const sa3k_head_norm* d, const HeadPtrs& p, bool bwd, int* code) {
+    *code = SA3K_ERR_INVALID;
+    if (!d) return "null shape";
+    if (d->type != SA3K_TYPE_F32 && d->type != SA3K_TYPE_F16 && d->type != SA3K_TYPE_BF16) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "type must be f32, f16 or bf16";
+    }
+    if (d->head_dim <= 0 || d->head_dim > kHeadMaxDim || d->head_dim % 8 != 0) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "head_dim must be a multiple of 8, at most 256";
+    }
+    if (d->rope_dims < 0 || d->rope_dims > d->head_dim) return "rope_dims must lie within head_dim";
+    if (d->rope_dims % 16 != 0) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "rope_dims must be a multiple of 16";
+    }
+    if (d->neighbours != 0 && d->neighbours != 1) return "neighbours must be 0 or 1";
+    if (d->batch < 0 || d->batch > 65535 || d->tokens < 0 || d->tokens >= kHeadMaxTokens) return "batch or tokens out of range";
+    if ((int64_t)d->batch * d->tokens >= kMaxExtent) return "batch x tokens out of range";
+    if (d->heads <= 0 || d->heads > 65535 || d->kv_heads <= 0 || d->kv_heads > 65535) return "heads or kv_heads out of range";
+    // ranges are written so that a NaN fails them
+    if (!(d->eps >= 0.f && d->eps <= 3.0e38f)) return "eps must be finite and not negative";
+    if (!(d->rope_base >= 1.f && d->rope_base <= 3.0e38f)) return "rope_base must be finite and at least 1";
+    if (d->cache_tokens < 0 || d->cache_tokens >= kHeadMaxTokens) return "cache_tokens out of range";
+    if (p.slot && d->cache_tokens == 0) return "slots need cache_tokens";
+    if (bwd && p.accumulate != 0 && p.accumulate != 1) return "accumulate must be 0 or 1";
+    const void* f[7] = {p.q_gain, p.k_gain, p.pos, p.slot, p.len, p.dq_gain, p.dk_gain};
+    for (const void* x : f)
+        if (!elem_aligned(x, 4)) return "gains, positions, slots and lengths must be 4-byte aligned";
+    if (d->batch == 0 || d->tokens == 0) return nullptr;   // nothing is read or written but the gains' gradients
+    const int eb = elem_bytes(d->type), D = d->head_dim;
+    const int64_t nq[3] = {d->batch, d->tokens, d->heads}, nk[3] = {d->batch, d->tokens, d->kv_heads};
+    const int64_t nc[3] = {d->batch, p.slot ? d->cache_tokens : d->tokens, d->kv_heads};
+    if (!p.q && !p.k && !p.v) return "q, k and v are all null";
+    if (!p.q != !p.qo || !p.k != !p.ko || !p.v != !p.vo) return "q, k and v need an output each, and an output its input";
+    if (bwd && ((p.q && !p.dqo) || (p.k && !p.dko))) return "q and k need their outputs' gradients";
+    if (bwd && ((p.dq_gain && !p.q) || (p.dk_gain && !p.k))) return "a gain's gradient needs its heads";
+    const char* m = nullptr;
+    // backward: dqo and dko lie as the outputs do, dq and dk as q and k do
+    const struct { const void* p; const int64_t *st, *n; bool out; } t[8] = {
+        {p.q, d->q_stride, nq, false}, {p.k, d->k_stride, nk, false}, {p.v, d->v_stride, nk, false},
+        {p.qo, bwd ? d->q_stride : d->q_out_stride, nq, true}, {p.ko, bwd ? d->k_stride : d->k_out_stride, bwd ? nk : nc, true},
+        {p.vo, d->v_out_stride, nc, true}, {p.dqo, d->q_out_stride, nq, false}, {p.dko, d->k_out_stride, nk, false}};
+    for (const auto& x : t)
+        if (x.p && (m = head_tensor_check(x.p, x.st, x.n, D, eb, x.out))) return m;
+    if (!bwd && p.slot && ((p.ko && p.ko == p.k) || (p.vo && p.vo == p.v))) return "k and v cannot move within themselves";
+    if (!same_place(bwd ? p.dqo : p.q, p.qo, bwd ? d->q_out_stride : d->q_stride, bwd ? d->q_stride : d->q_out_stride, nq) ||
+        !same_place(bwd ? p.dko : p.k, p.ko, bwd ? d->k_out_stride : d->k_stride, bwd ? d->k_stride : d->k_out_stride, nk) ||
+        !same_place(p.v, p.vo, d->v_stride, d->v_out_stride, nk))
+        return "a tensor written in place keeps its strides";
+    return nullptr;
+}
+
+// Pair i turns by pos base^(-2i / dims) radians. A position is a whole number, so only the fraction of a turn that one
+// position makes matters: as 64 bits behind the point, pos times it is exact modulo a turn, and off by at most
+// |pos| 2^-65 turns of the real number (2^-34 at the furthest position) whatever the position. Powers by repeated
+// products in 80 bits: the error of the last, 127 half steps of 2^-64, is below that of one rounding to 64 bits behind the point.
+inline void head_turns(int dims, float base, uint64_t* turn) {
+    const long double step = dims > 0 ? powl((long double)base, -2.0L / (long double)dims) : 0.0L;
+    long double f = 1.0L / 6.283185307179586476925286766559L;   // turns a position, pair 0
+    for (int i = 0; i < dims / 2; ++i, f *= step) turn[i] = (uint64_t)(f * 18446744073709551616.0L);
+}
+
+// Rows (token of a sample) that a workgroup of 256 threads takes at once: their angles, one a thread, are worked out together. Four
+// where that leaves 1024 workgroups or more (four a CU), else fewer, so that few rows use more of the chip.
+inline int head_rows(int64_t rows, int pairs) {
+    int n = rows >= 4096 ? 4 : rows >= 2048 ? 2 : 1;
+    while (n > 1 && n * pairs > 256) n /= 2;
+    return n;
+}
+// lanes that share a head, eight of its elements each
+inline int head_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+
+}  // namespace sa3k

@@ -63,6 +63,13 @@ class WindowAttnShape(C.Structure):
                [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride")]
 
 
+class HeadNormShape(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("type", "batch", "tokens", "heads", "kv_heads", "head_dim", "rope_dims", "neighbours",
+                                       "cache_tokens")] + [("eps", C.c_float), ("rope_base", C.c_float)] + \
+               [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride",
+                                             "v_out_stride")]
+
+
 class DitTrain(C.Structure):
     _fields_ = [("rank", C.c_int), ("alpha", C.c_float), ("dora", C.c_int), ("scope", C.c_int), ("batch", C.c_int),
                 ("frames", C.c_int), ("ctx_tokens", C.c_int), ("recompute", C.c_int)]
@@ -127,6 +134,8 @@ def _declare(lib):
         "sa3k_lora_chain_constants": (I, [P, P, P, P, C.POINTER(I)]),
         "sa3k_diff_attn_fwd": (I, [P, P, P, P, P, P, I, I, I, I, I, I, F, P, P, P, P, P]),
         "sa3k_diff_attn_bwd": (I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, P, P, P, P, P, P, P]),
+        "sa3k_head_norm_fwd": (I, [P, P] + [P] * 11),
+        "sa3k_head_norm_bwd": (I, [P, P] + [P] * 12 + [I]),
         "sa3k_layer_norm_fwd": (I, [P, I, P, I64, P, I64, I64, I64, P, P, F, P, I64, P, I64, P, P]),
         "sa3k_layer_norm_bwd": (I, [P, I, P, I64, P, I64, P, I64, I64, I64, P, P, P, P, I64, P, P, I]),
         "sa3k_window_attn_fwd": (I, [P, C.POINTER(WindowAttnShape), P, P, P, P, P, P, P]),
@@ -708,6 +717,37 @@ class WindowAttn:
         c = self.ctx
         c.check(c.lib.sa3k_window_attn_bwd(c.h, C.byref(self.shape), _p(q), _p(k), _p(v), _p(o), _p(lse), _p(dO), _p(q_len),
                                            _p(k_len), _p(dq), _p(dk), _p(dv)))
+
+
+class HeadNorm:
+    """RMS norm of the heads of q and k with the position rotation of their first `rope_dims` elements. Strides: (sample,
+    token, head) in elements; None: [batch][tokens][heads][head_dim] without gaps, k and v outputs of `cache_tokens` tokens
+    where that is given."""
+
+    def __init__(self, ctx, type, batch, tokens, heads, kv_heads, head_dim, rope_dims, neighbours=False, eps=1e-6, rope_base=1e4,
+                 cache_tokens=0, q_strides=None, k_strides=None, v_strides=None, q_out_strides=None, k_out_strides=None,
+                 v_out_strides=None):
+        self.ctx = ctx
+        dense = lambda n, h: (n * h * head_dim, h * head_dim, head_dim)  # noqa: E731
+        out = cache_tokens or tokens
+        st = [s if s is not None else dense(n, h) for s, n, h in
+              ((q_strides, tokens, heads), (k_strides, tokens, kv_heads), (v_strides, tokens, kv_heads),
+               (q_out_strides, tokens, heads), (k_out_strides, out, kv_heads), (v_out_strides, out, kv_heads))]
+        self.shape = HeadNormShape(type, batch, tokens, heads, kv_heads, head_dim, rope_dims, int(neighbours), cache_tokens, eps,
+                                   rope_base, *[(C.c_int64 * 3)(*s) for s in st])
+
+    def forward(self, q, k, q_gain, k_gain, q_out, k_out, v=None, v_out=None, pos=None, slot=None, len=None):
+        """k and v go to row `slot` of their outputs where slots are given"""
+        c = self.ctx
+        c.check(c.lib.sa3k_head_norm_fwd(c.h, C.byref(self.shape), _p(q), _p(k), _p(v), _p(q_gain), _p(k_gain), _p(pos),
+                                         _p(slot), _p(len), _p(q_out), _p(k_out), _p(v_out)))
+
+    def backward(self, q, k, dq_out, dk_out, q_gain, k_gain, dq, dk, dq_gain=None, dk_gain=None, pos=None, len=None,
+                 accumulate=False):
+        """dq and dk lie as q and k do, dq_out and dk_out as the outputs do"""
+        c = self.ctx
+        c.check(c.lib.sa3k_head_norm_bwd(c.h, C.byref(self.shape), _p(q), _p(k), _p(dq_out), _p(dk_out), _p(q_gain), _p(k_gain),
+                                         _p(pos), _p(len), _p(dq), _p(dk), _p(dq_gain), _p(dk_gain), int(accumulate)))
 
 
 def linear_act_fwd(ctx, type, act, x, w, M, N, K, y, bias=None, residual=None, z=None, ldx=None, ldw=None, ldr=None,
