@@ -560,6 +560,31 @@ SA3K_API int sa3k_head_norm_bwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const vo
                                 const void* dk_out, const float* q_gain, const float* k_gain, const int32_t* pos,
                                 const int32_t* len, void* dq, void* dk, float* dq_gain, float* dk_gain, int accumulate);
 
+/* Global norm and clip of gradients that lie in many tensors, of several types: sa3k_average_and_clip for gradients that are not
+ * one f32 arena, and the way into one (outputs in f32, end to end). */
+typedef struct {
+    void* grad;       /* device, n elements of `type`; only read where there is an output */
+    void* out;        /* device, n elements of `out_type`, or null: in place */
+    int64_t n;        /* >= 0 */
+    int type;         /* SA3K_TYPE_F32, _F16 or _BF16 */
+    int out_type;     /* `type`, or SA3K_TYPE_F32 */
+} sa3k_tensor;
+typedef struct sa3k_tensors sa3k_tensors;   /* a list of them, cut into pieces, on the device */
+
+/* A list of `count` tensors (0: none). It keeps their addresses, not their memory, which has to outlive its calls. An output must not
+ * meet another tensor's gradient or output, nor its own gradient but in place; gradients may repeat. Tensors need only be
+ * aligned to their elements. Synchronises the stream. */
+SA3K_API int sa3k_tensors_create(sa3k_ctx* ctx, const sa3k_tensor* tensors, int64_t count, sa3k_tensors** out);
+SA3K_API int sa3k_tensors_destroy(sa3k_ctx* ctx, sa3k_tensors* t);
+/* Over all of them, as sa3k_average_and_clip does over an arena:
+ *   s = g (1/count) if count > 1, else g               (float)
+ *   norm = sqrt(sum (double)s^2)                       (double, in a fixed order)
+ *   out = s (float)(max_norm / (norm + 1e-6)) if max_norm > 0 and norm > max_norm, else s     (rounded once to out_type)
+ * In place without average or clip nothing is written. A norm that is NaN clips nothing; an infinite one clips by 0, which leaves
+ * NaN in the place of infinities. stat (device double [2], nullable): norm, and the factor (1 without a clip). norm_out (host,
+ * nullable) receives the norm; passing it synchronises the stream. */
+SA3K_API int sa3k_tensors_clip(sa3k_ctx* ctx, sa3k_tensors* t, int count, float max_norm, double* stat, double* norm_out);
+
 /* ---------------------------------------------------------------- C3: one DiT block */
 
 /* Shape of a (differential) DiT block, the DitConfig fields dit_block reads (src/dit.h:20-46). */

@@ -70,6 +70,10 @@ class HeadNormShape(C.Structure):
                                              "v_out_stride")]
 
 
+class TensorEntry(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("n", C.c_int64), ("type", C.c_int), ("out_type", C.c_int)]
+
+
 class DitTrain(C.Structure):
     _fields_ = [("rank", C.c_int), ("alpha", C.c_float), ("dora", C.c_int), ("scope", C.c_int), ("batch", C.c_int),
                 ("frames", C.c_int), ("ctx_tokens", C.c_int), ("recompute", C.c_int)]
@@ -136,6 +140,9 @@ def _declare(lib):
         "sa3k_diff_attn_bwd": (I, [P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, P, P, P, P, P, P, P]),
         "sa3k_head_norm_fwd": (I, [P, P] + [P] * 11),
         "sa3k_head_norm_bwd": (I, [P, P] + [P] * 12 + [I]),
+        "sa3k_tensors_create": (I, [P, C.POINTER(TensorEntry), I64, C.POINTER(P)]),
+        "sa3k_tensors_destroy": (I, [P, P]),
+        "sa3k_tensors_clip": (I, [P, P, I, F, P, C.POINTER(D)]),
         "sa3k_layer_norm_fwd": (I, [P, I, P, I64, P, I64, I64, I64, P, P, F, P, I64, P, I64, P, P]),
         "sa3k_layer_norm_bwd": (I, [P, I, P, I64, P, I64, P, I64, I64, I64, P, P, P, P, I64, P, P, I]),
         "sa3k_window_attn_fwd": (I, [P, C.POINTER(WindowAttnShape), P, P, P, P, P, P, P]),
@@ -748,6 +755,29 @@ class HeadNorm:
         c = self.ctx
         c.check(c.lib.sa3k_head_norm_bwd(c.h, C.byref(self.shape), _p(q), _p(k), _p(dq_out), _p(dk_out), _p(q_gain), _p(k_gain),
                                          _p(pos), _p(len), _p(dq), _p(dk), _p(dq_gain), _p(dk_gain), int(accumulate)))
+
+
+class Tensors:
+    """A list of gradients: (device address, elements, type, output's address or None: in place, output's type)"""
+
+    def __init__(self, ctx, entries):
+        self.ctx, self.h = ctx, None
+        arr = (TensorEntry * max(1, len(entries)))(*[TensorEntry(g, o, n, t, ot) for g, n, t, o, ot in entries])
+        h = C.c_void_p()
+        ctx.check(ctx.lib.sa3k_tensors_create(ctx.h, arr, len(entries), C.byref(h)))
+        self.h = h.value
+
+    def clip(self, count, max_norm, stat=None, want_norm=False):
+        """average over `count`, clip to the global norm; stat: device f64 [2] (norm, factor)"""
+        norm = C.c_double()
+        self.ctx.check(self.ctx.lib.sa3k_tensors_clip(self.ctx.h, self.h, int(count), float(max_norm), _p(stat),
+                                                      C.byref(norm) if want_norm else None))
+        return norm.value if want_norm else None
+
+    def destroy(self):
+        if self.h and self.ctx.h:
+            self.ctx.check(self.ctx.lib.sa3k_tensors_destroy(self.ctx.h, self.h))
+        self.h = None
 
 
 def linear_act_fwd(ctx, type, act, x, w, M, N, K, y, bias=None, residual=None, z=None, ldx=None, ldw=None, ldr=None,
