@@ -143,6 +143,8 @@ def _declare(lib):
         "sa3k_tensors_create": (I, [P, C.POINTER(TensorEntry), I64, C.POINTER(P)]),
         "sa3k_tensors_destroy": (I, [P, P]),
         "sa3k_tensors_clip": (I, [P, P, I, F, P, C.POINTER(D)]),
+        "sa3k_gated_linear_fwd": (I, [P, I, I, P, I64, P, P, I64, P, P, I64, I64, I64, P, I64, P, P, I64]),
+        "sa3k_gated_linear_bwd": (I, [P, I, I, P, I64, P, P, I64, P, I64, P, P, I64, I64, I64, I64, P, I64, P, P, I, I64, P, P, I]),
         "sa3k_layer_norm_fwd": (I, [P, I, P, I64, P, I64, I64, I64, P, P, F, P, I64, P, I64, P, P]),
         "sa3k_layer_norm_bwd": (I, [P, I, P, I64, P, I64, P, I64, I64, I64, P, P, P, P, I64, P, P, I]),
         "sa3k_window_attn_fwd": (I, [P, C.POINTER(WindowAttnShape), P, P, P, P, P, P, P]),
@@ -795,3 +797,21 @@ def linear_act_bwd(ctx, type, act, dy, x, w, M, N, K, z=None, dx=None, dw=None, 
     ctx.check(ctx.lib.sa3k_linear_act_bwd(ctx.h, type, act, _p(dy), d(lddy, N), _p(z), d(ldz, N), _p(x), d(ldx, K), _p(w),
                                           d(ldw, K), M, N, K, _p(dx), d(lddx, K), _p(dw), d(dw_type, type), d(lddw, K),
                                           _p(db), int(accumulate)))
+
+
+def gated_linear_fwd(ctx, type, act, x, w_gate, w_up, M, N, K, y, gate_bias=None, up_bias=None, gate=None, up=None, ldx=None,
+                     ldw=None, ldy=None, ldz=None):
+    """y [M][N] = act(g) u, g = x [M][K] . w_gate [N][K]^T + gate_bias, u of w_up likewise (stored to `gate` and `up` when
+    given); pitches in elements"""
+    d = lambda v, n: n if v is None else v  # noqa: E731
+    ctx.check(ctx.lib.sa3k_gated_linear_fwd(ctx.h, type, act, _p(x), d(ldx, K), _p(w_gate), _p(w_up), d(ldw, K), _p(gate_bias),
+                                            _p(up_bias), M, N, K, _p(y), d(ldy, N), _p(gate), _p(up), d(ldz, N)))
+
+
+def gated_linear_bwd(ctx, type, act, dy, gate, up, x, w_gate, w_up, M, N, K, dx=None, dw_gate=None, dw_up=None, db_gate=None,
+                     db_up=None, dw_type=None, accumulate=False, lddy=None, ldz=None, ldx=None, ldw=None, lddx=None, lddw=None):
+    """dx, the weights' gradients (of `type`, or dw_type) and the biases' of gated_linear_fwd"""
+    d = lambda v, n: n if v is None else v  # noqa: E731
+    ctx.check(ctx.lib.sa3k_gated_linear_bwd(ctx.h, type, act, _p(dy), d(lddy, N), _p(gate), _p(up), d(ldz, N), _p(x), d(ldx, K),
+                                            _p(w_gate), _p(w_up), d(ldw, K), M, N, K, _p(dx), d(lddx, K), _p(dw_gate), _p(dw_up),
+                                            d(dw_type, type), d(lddw, K), _p(db_gate), _p(db_up), int(accumulate)))

@@ -1,0 +1,31 @@
+// The gated products' argument checks and plans (csrc/gated.h) for the CPU tests.
+#include "gated.h"
+
+using namespace sa3k;
+
+static void* at(int64_t v) { return reinterpret_cast<void*>((uintptr_t)v); }
+
+extern "C" {
+
+// p: X, Wg, Wu, dY, G, U, Y, g output, u output, dX, dWg, dWu, bg, bu, dbg, dbu as addresses; ld: x, w, dy, z, y, dx, dw
+int gated(int type, int act, const int64_t* mnk, const int64_t* p, const int64_t* ld, int dw_type, int accumulate, int bwd) {
+    GatedArgs a;
+    a.type = type; a.act = act; a.M = mnk[0]; a.N = mnk[1]; a.K = mnk[2];
+    a.X = at(p[0]); a.Wg = at(p[1]); a.Wu = at(p[2]); a.dY = at(p[3]); a.G = at(p[4]); a.U = at(p[5]); a.Y = at(p[6]);
+    a.Go = at(p[7]); a.Uo = at(p[8]); a.dX = at(p[9]); a.dWg = at(p[10]); a.dWu = at(p[11]);
+    a.bg = (const float*)at(p[12]); a.bu = (const float*)at(p[13]); a.dbg = (float*)at(p[14]); a.dbu = (float*)at(p[15]);
+    a.ldx = ld[0]; a.ldw = ld[1]; a.lddy = ld[2]; a.ldz = ld[3]; a.ldy = ld[4]; a.lddx = ld[5]; a.lddw = ld[6];
+    a.dw_type = dw_type; a.accumulate = accumulate;
+    int code = -1;
+    return gated_check(a, bwd != 0, &code) ? code : 0;
+}
+// forward: edge, splits; backward: together, edge and splits of dX, of dW
+void plans(int64_t M, int64_t N, int64_t K, int* out) {
+    const int64_t h = 2 * gated_half(N), Kp = (K + 7) / 8 * 8;
+    const ProdPlan f = prod_plan(M, 2 * N, Kp);
+    const ProdPair p = prod_pair({M, K, h}, {h, K, M});
+    out[0] = f.edge; out[1] = f.splits;
+    out[2] = p.together; out[3] = p.a.edge; out[4] = p.a.splits; out[5] = p.b.edge; out[6] = p.b.splits;
+}
+
+}  // extern "C"
