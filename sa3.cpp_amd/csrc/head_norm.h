@@ -99,14 +99,13 @@ inline void head_turns(int dims, float base, uint64_t* turn) {
     for (int i = 0; i < dims / 2; ++i, f *= step) turn[i] = (uint64_t)(f * 18446744073709551616.0L);
 }
 
-// Rows (token of a sample) that a workgroup of 256 threads takes at once: their angles, one a thread, are worked out together. Four
-// where that leaves 1024 workgroups or more (four a CU), else fewer, so that few rows use more of the chip.
-inline int head_rows(int64_t rows, int pairs) {
-    int n = rows >= 4096 ? 4 : rows >= 2048 ? 2 : 1;
-    while (n > 1 && n * pairs > 256) n /= 2;
-    return n;
-}
 // lanes that share a head, eight of its elements each
 inline int head_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+// a wave takes this many groups of 64 / lanes heads at the most, and a tensor's heads are that many waves' to a row
+constexpr int kGroups = 3;
+inline int head_parts(int heads, int dim) {
+    const int per = kGroups * (64 / head_lanes(dim));
+    return (heads + per - 1) / per;
+}
 
 }  // namespace sa3k

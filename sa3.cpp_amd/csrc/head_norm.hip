@@ -5,27 +5,32 @@
 //   backward   w = R^T dy, dgain = sum over tokens and heads w x r, h = w gain, dx = r (h - x r mean(h x r))
 // The statistics are worked out again in the backward, from the x it reads anyway. All arithmetic in f32, each output rounded once.
 //
-// Eight elements of a head a lane, 4 to 32 lanes a head, several heads a wave; a wave's heads are all q, all k or all v, so that
-// pointers, strides and gains are the wave's own. A workgroup takes whole rows (tokens): their sines and cosines, shared by all heads,
-// go through LDS once. Angles are exact modulo a turn (head_turns), so a position a million tokens out is as good as the first.
+// Eight elements of a head a lane, 4 to 32 lanes a head, several heads a wave. A wave takes up to four such groups of heads of one row
+// (token) and one tensor, so that nothing but the lane's own head is chosen inside it; the row's sines and cosines, which the heads share,
+// are worked out a pair a lane while the loads are under way. Angles are exact modulo a turn (head_turns), so a position a million tokens out is as good as the first.
 #include <algorithm>
 
 #include "head_norm.h"
+#include "headprep.h"
 #include "layer_ops_dev.h"
 
 namespace {
 using namespace sa3k;
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kFwdWaves = 4, kBwdWaves = 8;   // of a workgroup
 
+struct HeadTensor {   // q, k or v
+    const void *x, *dy;
+    void* y;
+    const float* gain;
+    int64_t xs[3], ys[3], dys[3];   // strides of samples, tokens, heads
+    int heads, first;               // first: of the workgroups' parts (blockIdx.y)
+};
 struct HeadArgs {
-    const void *x[3], *dy[2];
-    void* y[3];
-    int64_t xs[3][3], ys[3][3], dys[2][3];   // strides of samples, tokens, heads
-    const float* gain[2];
+    HeadTensor t[3];
     const int32_t *pos, *slot, *len;
-    int batch, tokens, heads[3], groups[3];   // of q, k, v; groups: of as many heads as a wave takes
-    int dim, rope, near, cache, rows;         // rows: a workgroup takes at once
+    int batch, tokens, dim, rope, near, cache, kinds;   // kinds: tensors there are, one after the other in t
+    int kind[3];                                        // which each is: 0 q, 1 k, 2 v
     float eps;
     uint64_t turn[kHeadMaxDim / 2];
 };
@@ -56,304 +61,330 @@ __device__ __forceinline__ float inverse_root(float v) {
     else return __builtin_amdgcn_rsqf(v);   // off by 2^-23, against the 2^-9 or 2^-12 of the output's rounding
 }
 
-// the angles' cos and sin of `n` rows from row0 on into tab [n][rope / 2]
-__device__ __forceinline__ void fill_turns(const HeadArgs& a, int64_t row0, int n, float2* tab) {
-    const int pairs = a.rope >> 1;
-    for (int i = threadIdx.x; i < n * pairs; i += kThreads) {
-        const int r = i / pairs, p = i - r * pairs;
-        const uint32_t row = (uint32_t)row0 + (uint32_t)r;
-        const int64_t pos = a.pos ? a.pos[row] : (int64_t)(row % (uint32_t)a.tokens);
-        tab[i] = cos_sin((uint32_t)(((uint64_t)pos * a.turn[p]) >> 32));
-    }
-}
-
-// One wave's share of a row's group of heads: which tensor, and where this lane's eight elements lie
-struct Item {
-    int kind, b, t, slot;   // 0 q, 1 k, 2 v
-    int row;                // of the workgroup's
-    int64_t head;
-    bool on;                // the lane has elements of a head, and the token is in its sequence
-    bool store;             // and they have a place to go to
+// The row (a token of a sample) of a wave
+struct Row {
+    int64_t row;
+    int b, t;
+    bool on;   // the token is in its sequence
 };
-template <int LPH>
-__device__ __forceinline__ Item item_of(const HeadArgs& a, int64_t row0, int n, int i, int lane) {
-    constexpr int HPW = 64 / LPH;
-    const int groups = a.groups[0] + a.groups[1] + a.groups[2];
-    Item m;
-    m.row = __builtin_amdgcn_readfirstlane(i / groups);
-    int g = __builtin_amdgcn_readfirstlane(i - m.row * groups);
-    m.kind = g < a.groups[0] ? 0 : g < a.groups[0] + a.groups[1] ? 1 : 2;
-    g -= m.kind > 0 ? a.groups[0] : 0;
-    g -= m.kind > 1 ? a.groups[1] : 0;
-    const bool in = m.row < n;
-    const uint32_t row = (uint32_t)row0 + (uint32_t)(in ? m.row : 0);   // (batch x tokens stays below 2^31)
-    m.b = (int)(row / (uint32_t)a.tokens);
-    m.t = (int)(row - (uint32_t)m.b * (uint32_t)a.tokens);
-    m.head = g * HPW + lane / LPH;
-    m.on = in && m.head < a.heads[m.kind] && (lane % LPH) * 8 < a.dim && !(a.len && m.t >= a.len[m.b]);
-    m.slot = a.slot && m.kind > 0 && in ? a.slot[row] : m.t;
-    m.store = m.on && !(a.slot && m.kind > 0 && (m.slot < 0 || m.slot >= a.cache));
-    return m;
+__device__ __forceinline__ Row row_of(const HeadArgs& a, int64_t row) {
+    Row r;
+    r.row = row;
+    r.b = __builtin_amdgcn_readfirstlane((int)((uint32_t)row / (uint32_t)a.tokens));   // (batch x tokens stays below 2^31)
+    r.t = (int)((uint32_t)row - (uint32_t)r.b * (uint32_t)a.tokens);
+    r.on = !(a.len && r.t >= a.len[r.b]);
+    return r;
 }
-__device__ __forceinline__ int64_t place(const int64_t* s, int b, int t, int64_t head, int lane_off) {
-    return b * s[0] + t * s[1] + head * s[2] + lane_off;
+// cos and sin of the row's angles for this lane's eight elements (with neighbours four pairs, else eight): each pair's by one lane of
+// the wave, exchanged through `tab`, this wave's place in LDS (kTab long: lanes whose elements are not turned read on)
+constexpr int kTab = kHeadMaxDim / 2 + 8;
+__device__ __forceinline__ void row_turns(const HeadArgs& a, const Row& r, int c, int lane, float2* tab, float2 (&w)[8]) {
+    if (a.rope == 0) return;   // (uniform)
+    const int pairs = a.rope >> 1;
+    const int64_t pos = a.pos ? a.pos[r.row] : (int64_t)r.t;
+    for (int p = lane; p < pairs; p += 64) tab[p] = cos_sin((uint32_t)(((uint64_t)pos * a.turn[p]) >> 32));
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int h = a.rope >> 4;   // lanes of half the turned elements
+    const int at = 8 * c >= a.rope ? 0 : a.near ? 4 * c : 8 * (c < h ? c : c - h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = tab[at + e];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();   // (the next row's angles come after these reads)
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// which tensor a workgroup's part is of
+__device__ __forceinline__ int tensor_of(const HeadArgs& a, int part) {
+    int i = 0;
+    if (a.kinds > 1 && part >= a.t[1].first) i = 1;
+    if (a.kinds > 2 && part >= a.t[2].first) i = 2;
+    return i;
+}
+// eight elements of a head, from element `at` on
+template <class T>
+struct Eight {
+    u32x4a r[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const void* p, int64_t at) {
+        const SA3K_GLOBAL T* q = (const SA3K_GLOBAL T*)p + at;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = load16(q + i * (16 / sizeof(T)));
+    }
+    __device__ __forceinline__ void store(void* p, int64_t at) const {
+        SA3K_GLOBAL T* q = (SA3K_GLOBAL T*)p + at;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) store16(q + i * (16 / sizeof(T)), r[i]);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const Pack<T, 8> q = __builtin_bit_cast(Pack<T, 8>, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)q.v[e];
+    }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+        Pack<T, 8> q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q.v[e] = (T)v[e];
+        *this = __builtin_bit_cast(Eight, q);
+    }
+};
+
+// over the lanes of a head, the same bits in each
 template <int LPH>
 __device__ __forceinline__ float head_sum(float v) {
-#pragma unroll
-    for (int o = 1; o < LPH; o <<= 1) v += __shfl_xor(v, o, 64);
+    v = dpp_add<0xB1>(v);                                    // lane ^ 1
+    v = dpp_add<0x4E>(v);                                    // lane ^ 2
+    if constexpr (LPH > 4) v = dpp_add<0x141>(v);            // the mirrored lane of eight
+    if constexpr (LPH > 8) v = dpp_add<0x140>(v);            // of sixteen
+    if constexpr (LPH > 16) v += __shfl_xor(v, 16, 64);
     return v;
 }
 
-// y's pairs turned by the angles in tab (sign -1: back). Elements 8c .. 8c + 7 of the head; rope and its half are
-// multiples of eight, so a lane's elements are all turned or none, and the partners of (i, i + rope / 2) are one lane's.
-template <int LPH>
-__device__ __forceinline__ void rotate(const HeadArgs& a, const float2* tab, int c, int lane, float sign, float (&y)[8]) {
+// y's pairs turned by w (sign -1: back). Elements 8c .. 8c + 7 of the head; rope and its half are multiples of eight, so a
+// lane's elements are all turned or none, and the partners of (i, i + rope / 2) are one lane's.
+__device__ __forceinline__ void rotate(const HeadArgs& a, const float2 (&w)[8], int c, int lane, float sign, float (&y)[8]) {
     if (a.rope == 0) return;   // (uniform)
     const bool turned = 8 * c < a.rope;
     if (a.near) {
-        if (!turned) return;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-            const float2 w = tab[4 * c + e / 2];
-            const float p = y[e], q = y[e + 1], s = sign * w.y;
-            y[e] = __builtin_fmaf(p, w.x, -q * s);
-            y[e + 1] = __builtin_fmaf(q, w.x, p * s);
+            const float p = y[e], q = y[e + 1], s = sign * w[e / 2].y;
+            y[e] = turned ? __builtin_fmaf(p, w[e / 2].x, -q * s) : p;
+            y[e + 1] = turned ? __builtin_fmaf(q, w[e / 2].x, p * s) : q;
         }
         return;
     }
-    const int h = a.rope >> 4;   // lanes of half the turned elements
+    const int h = a.rope >> 4;
     const bool first = c < h;
     const int from = !turned ? lane : first ? lane + h : lane - h;
-    float o[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = __shfl(y[e], from, 64);
-    if (!turned) return;
     const float sg = first ? -sign : sign;
-    const float2* w = tab + 8 * (first ? c : c - h);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(y[e], w[e].x, o[e] * (sg * w[e].y));
-}
-
-template <int LPH>
-__device__ __forceinline__ void load_gain(const HeadArgs& a, int c, float (&g)[2][8]) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[k][e] = a.gain[k] && 8 * c < a.dim ? a.gain[k][8 * c + e] : 1.f;
-}
-
-template <class T, int LPH>
-__global__ __launch_bounds__(kThreads) void head_norm_fwd_kernel(HeadArgs a) {
-    constexpr int U = 4;   // groups of heads whose loads a wave has under way
-    __shared__ float2 tab[kThreads];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane % LPH;
-    const int64_t rows = (int64_t)a.batch * a.tokens;
-    float gain[2][8];
-    load_gain<LPH>(a, c, gain);
-    const float inv = 1.f / (float)a.dim;
-    for (int64_t row0 = (int64_t)blockIdx.x * a.rows; row0 < rows; row0 += (int64_t)gridDim.x * a.rows) {
-        const int n = (int)min((int64_t)a.rows, rows - row0), items = n * (a.groups[0] + a.groups[1] + a.groups[2]);
-        if (row0 != (int64_t)blockIdx.x * a.rows) __syncthreads();   // (the rows before are done with the table)
-        fill_turns(a, row0, n, tab);
-        __syncthreads();
-        for (int i0 = wave; i0 < items; i0 += kWaves * U) {
-            Pack<T, 8> x[U];
-            Item m[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                m[u] = item_of<LPH>(a, row0, n, i0 + u * kWaves, lane);
-                if (m[u].on) {
-                    x[u] = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.x[m[u].kind]) +
-                                                               place(a.xs[m[u].kind], m[u].b, m[u].t, m[u].head, 8 * c));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[u].v[e] = (T)0.f;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (i0 + u * kWaves >= items) break;   // (uniform)
-                T* out = static_cast<T*>(a.y[m[u].kind]) + place(a.ys[m[u].kind], m[u].b, m[u].slot, m[u].head, 8 * c);
-                if (m[u].kind == 2) {   // (uniform)
-                    if (m[u].store) *reinterpret_cast<Pack<T, 8>*>(out) = x[u];
-                    continue;
-                }
-                float y[8], s = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    y[e] = (float)x[u].v[e];
-                    s = __builtin_fmaf(y[e], y[e], s);
-                }
-                const float r = inverse_root<T>(__builtin_fmaf(head_sum<LPH>(s), inv, a.eps));
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] *= r * (m[u].kind ? gain[1][e] : gain[0][e]);
-                rotate<LPH>(a, tab + m[u].row * (a.rope >> 1), c, lane, 1.f, y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[u].v[e] = (T)y[e];
-                if (m[u].store) *reinterpret_cast<Pack<T, 8>*>(out) = x[u];
-            }
-        }
+    for (int e = 0; e < 8; ++e) {
+        const float o = __shfl(y[e], from, 64);
+        y[e] = turned ? __builtin_fmaf(y[e], w[e].x, o * (sg * w[e].y)) : y[e];
     }
 }
 
-// part [gridDim.x][2][dim]: this workgroup's sums of the gains' gradients (null: none)
+__device__ __forceinline__ void load_gain(const HeadArgs& a, const float* p, int c, float (&g)[8]) {
+    if (p && 8 * c < a.dim) {
+        const SA3K_GLOBAL float* q = (const SA3K_GLOBAL float*)p + 8 * c;
+        const u32x4a lo = load16(q), hi = load16(q + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            g[e] = __uint_as_float(lo[e]);
+            g[4 + e] = __uint_as_float(hi[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = 1.f;
+    }
+}
+
+// A wave takes kGroups groups of heads of one row and tensor at the most, whose loads are all under way at once. A lane past the last
+// head, or past a head's elements, reads the last ones and stores nothing.
 template <class T, int LPH>
-__global__ __launch_bounds__(kThreads) void head_norm_bwd_kernel(HeadArgs a, float* part) {
-    constexpr int U = 2;
-    __shared__ float2 tab[kThreads];
-    __shared__ float sums[kWaves][2][LPH * 8];
+__global__ __launch_bounds__(64 * kFwdWaves) void head_norm_fwd_kernel(HeadArgs a) {
+    __shared__ float2 tabs[kFwdWaves][kTab];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane % LPH;
+    const int64_t row = (int64_t)blockIdx.x * kFwdWaves + wave;
+    if (row >= (int64_t)a.batch * a.tokens) return;
+    const int part = blockIdx.y, ti = tensor_of(a, part), kind = a.kind[ti];
+    const HeadTensor& tn = a.t[ti];
+    const Row r = row_of(a, row);
+    if (!r.on) return;
+    const int h0 = (part - tn.first) * kGroups * (64 / LPH) + lane / LPH, e0 = min(8 * c, a.dim - 8), heads = tn.heads;
+    const int64_t from = r.b * tn.xs[0] + r.t * tn.xs[1] + e0, xh = tn.xs[2];
+    Eight<T> x[kGroups];
+#pragma unroll
+    for (int u = 0; u < kGroups; ++u) x[u].load(tn.x, from + min(h0 + u * (64 / LPH), heads - 1) * xh);
+    const int slot = a.slot && kind ? a.slot[row] : r.t;
+    const bool kept = !(a.slot && kind) || (slot >= 0 && slot < a.cache);
+    float2 w[8];
+    float gain[8];
+    if (kind < 2) {   // (uniform)
+        load_gain(a, tn.gain, c, gain);
+        row_turns(a, r, c, lane, tabs[wave], w);   // (while the loads are under way)
+    }
+    if (!kept) return;   // (uniform)
+    const float inv = 1.f / (float)a.dim;
+    const int64_t to = r.b * tn.ys[0] + slot * tn.ys[1] + e0, yh = tn.ys[2];
+#pragma unroll
+    for (int u = 0; u < kGroups; ++u) {
+        const int h = h0 + u * (64 / LPH);
+        if (u && h - lane / LPH >= heads) break;   // (uniform)
+        if (kind < 2) {   // (uniform)
+            float y[8], s = 0.f;
+            x[u].get(y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[e] = 8 * c < a.dim ? y[e] : 0.f;
+                s = __builtin_fmaf(y[e], y[e], s);
+            }
+            const float rt = inverse_root<T>(__builtin_fmaf(head_sum<LPH>(s), inv, a.eps));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] *= rt * gain[e];
+            rotate(a, w, c, lane, 1.f, y);
+            x[u].set(y);
+        }
+        if (h < heads && 8 * c < a.dim) x[u].store(tn.y, to + h * yh);
+    }
+}
+
+// part [gridDim.y][gridDim.x][dim]: each workgroup's sums of its gain's gradient (null: none)
+template <class T, int LPH>
+__global__ __launch_bounds__(64 * kBwdWaves, 4) void head_norm_bwd_kernel(HeadArgs a, float* part) {
+    __shared__ union {
+        float2 tabs[kBwdWaves][kTab];
+        float sums[kBwdWaves][LPH * 8];
+    } lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane % LPH;
     const int64_t rows = (int64_t)a.batch * a.tokens;
-    float gain[2][8], dg[2][8];
-    load_gain<LPH>(a, c, gain);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dg[0][e] = dg[1][e] = 0.f;
+    const HeadTensor& tn = a.t[tensor_of(a, blockIdx.y)];
+    const int h0 = ((int)blockIdx.y - tn.first) * kGroups * (64 / LPH) + lane / LPH, e0 = min(8 * c, a.dim - 8), heads = tn.heads;
     const float inv = 1.f / (float)a.dim;
-    for (int64_t row0 = (int64_t)blockIdx.x * a.rows; row0 < rows; row0 += (int64_t)gridDim.x * a.rows) {
-        const int n = (int)min((int64_t)a.rows, rows - row0), items = n * (a.groups[0] + a.groups[1]);
-        __syncthreads();   // (the rows before are done with the table)
-        fill_turns(a, row0, n, tab);
-        __syncthreads();
-        for (int i0 = wave; i0 < items; i0 += kWaves * U) {
-            Pack<T, 8> x[U], dy[U];
-            Item m[U];
+    float gain[8], dg[8];
+    load_gain(a, tn.gain, c, gain);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                m[u] = item_of<LPH>(a, row0, n, i0 + u * kWaves, lane);
-                const int k = m[u].kind;
-                if (m[u].on) {
-                    x[u] = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.x[k]) +
-                                                               place(a.xs[k], m[u].b, m[u].t, m[u].head, 8 * c));
-                    dy[u] = *reinterpret_cast<const Pack<T, 8>*>(static_cast<const T*>(a.dy[k]) +
-                                                                place(a.dys[k], m[u].b, m[u].t, m[u].head, 8 * c));
-                } else {
+    for (int e = 0; e < 8; ++e) dg[e] = 0.f;
+    for (int64_t row = (int64_t)blockIdx.x * kBwdWaves + wave; row < rows; row += (int64_t)gridDim.x * kBwdWaves) {
+        const Row r = row_of(a, row);
+        if (!r.on) continue;   // (uniform)
+        const int64_t xat = r.b * tn.xs[0] + r.t * tn.xs[1] + e0, dat = r.b * tn.dys[0] + r.t * tn.dys[1] + e0;
+        const int64_t yat = r.b * tn.ys[0] + r.t * tn.ys[1] + e0;
+        Eight<T> x[kGroups], dy[kGroups];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[u].v[e] = dy[u].v[e] = (T)0.f;
-                }
+        for (int u = 0; u < kGroups; ++u) {
+            const int h = min(h0 + u * (64 / LPH), heads - 1);
+            x[u].load(tn.x, xat + h * tn.xs[2]);
+            dy[u].load(tn.dy, dat + h * tn.dys[2]);
+        }
+        float2 w[8];
+        row_turns(a, r, c, lane, lds.tabs[wave], w);   // (while the loads are under way)
+#pragma unroll
+        for (int u = 0; u < kGroups; ++u) {
+            const int hd = h0 + u * (64 / LPH);
+            if (u && hd - lane / LPH >= heads) break;   // (uniform)
+            const bool on = hd < heads && 8 * c < a.dim;
+            float d[8], xf[8], h[8], s = 0.f, t = 0.f;
+            dy[u].get(d);
+            x[u].get(xf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                d[e] = on ? d[e] : 0.f;
+                xf[e] = on ? xf[e] : 0.f;
             }
+            rotate(a, w, c, lane, -1.f, d);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (i0 + u * kWaves >= items) break;   // (uniform)
-                const int k = m[u].kind;
-                float w[8], xf[8], s = 0.f, t = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    w[e] = (float)dy[u].v[e];
-                    xf[e] = (float)x[u].v[e];
-                }
-                rotate<LPH>(a, tab + m[u].row * (a.rope >> 1), c, lane, -1.f, w);
-                float h[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h[e] = w[e] * (k ? gain[1][e] : gain[0][e]);
-                    s = __builtin_fmaf(xf[e], xf[e], s);
-                    t = __builtin_fmaf(h[e], xf[e], t);
-                }
-                const float r = inverse_root<T>(__builtin_fmaf(head_sum<LPH>(s), inv, a.eps));
-                const float mean = head_sum<LPH>(t) * r * inv;
-                if (m[u].on) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float xh = xf[e] * r;
-                        if (k) dg[1][e] = __builtin_fmaf(w[e], xh, dg[1][e]);
-                        else dg[0][e] = __builtin_fmaf(w[e], xh, dg[0][e]);
-                        x[u].v[e] = (T)(r * (h[e] - xh * mean));
-                    }
-                    *reinterpret_cast<Pack<T, 8>*>(static_cast<T*>(a.y[k]) + place(a.ys[k], m[u].b, m[u].t, m[u].head, 8 * c)) = x[u];
-                }
+            for (int e = 0; e < 8; ++e) {
+                h[e] = d[e] * gain[e];
+                s = __builtin_fmaf(xf[e], xf[e], s);
+                t = __builtin_fmaf(h[e], xf[e], t);
             }
+            s = head_sum<LPH>(s);
+            const float rt = on ? inverse_root<T>(__builtin_fmaf(s, inv, a.eps)) : 0.f;
+            const float mean = head_sum<LPH>(t) * rt * inv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float xh = xf[e] * rt;
+                dg[e] = __builtin_fmaf(d[e], xh, dg[e]);
+                h[e] = rt * (h[e] - xh * mean);
+            }
+            x[u].set(h);
+            if (on) x[u].store(tn.y, yat + hd * tn.ys[2]);
         }
     }
     if (!part) return;
     // over the wave's heads, then the waves in their order
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float v = dg[k][e];
-#pragma unroll
-            for (int o = LPH; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-            if (lane < LPH) sums[wave][k][8 * c + e] = v;
-        }
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * a.dim; i += kThreads) {
-        const int k = i >= a.dim, d = k ? i - a.dim : i;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v = dg[e];
+#pragma unroll
+        for (int o = LPH; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+        if (lane < LPH) lds.sums[wave][8 * c + e] = v;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.dim; i += 64 * kBwdWaves) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) v += sums[w][k][d];
-        part[(int64_t)blockIdx.x * 2 * a.dim + i] = v;
+        for (int n = 0; n < kBwdWaves; ++n) v += lds.sums[n][i];
+        part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.dim + i] = v;
     }
 }
 
-// the gains' gradients from the workgroups' sums
-__global__ __launch_bounds__(kColumnSumThreads) void head_norm_sum_kernel(const float* __restrict__ part, int parts, int dim,
+// the gains' gradients from the workgroups' sums: of q (blockIdx.y 0) the first nq rows, of k the nk after them
+__global__ __launch_bounds__(kColumnSumThreads) void head_norm_sum_kernel(const float* __restrict__ part, int nq, int nk, int dim,
                                                                           float* dq, float* dk, int accumulate) {
-    column_sums(part, parts, 2 * (int64_t)dim, [&](int64_t i, float t) {
-        float* d = i < dim ? dq : dk;
-        const int64_t e = i < dim ? i : i - dim;
-        if (d) d[e] = accumulate ? d[e] + t : t;
-    });
+    float* d = blockIdx.y ? dk : dq;
+    if (!d) return;
+    column_sums(blockIdx.y ? part + (int64_t)nq * dim : part, blockIdx.y ? nk : nq, dim,
+                [&](int64_t i, float t) { d[i] = accumulate ? d[i] + t : t; });
 }
 
-// Workgroups of the backward with gains' gradients, at the most: each writes 8 dim bytes that the second launch reads again.
-constexpr int kHeadBwdGroups = 1024;
-
-void copy3(int64_t (&to)[3], const int64_t* from) {
-    for (int i = 0; i < 3; ++i) to[i] = from[i];
-}
+// Workgroups of the backward with gains' gradients, at the most: each writes 4 dim bytes that the second launch reads again.
+constexpr int kHeadBwdGroups = 512;
 
 HeadArgs head_args(const sa3k_head_norm& d, const HeadPtrs& p, bool bwd) {
     HeadArgs a{};
-    a.x[0] = p.q; a.x[1] = p.k; a.x[2] = p.v;
-    a.y[0] = p.qo; a.y[1] = p.ko; a.y[2] = p.vo;
-    a.dy[0] = p.dqo; a.dy[1] = p.dko;
-    copy3(a.xs[0], d.q_stride); copy3(a.xs[1], d.k_stride); copy3(a.xs[2], d.v_stride);
-    copy3(a.ys[0], bwd ? d.q_stride : d.q_out_stride); copy3(a.ys[1], bwd ? d.k_stride : d.k_out_stride);
-    copy3(a.ys[2], d.v_out_stride);
-    copy3(a.dys[0], d.q_out_stride); copy3(a.dys[1], d.k_out_stride);
-    a.gain[0] = static_cast<const float*>(p.q_gain);
-    a.gain[1] = static_cast<const float*>(p.k_gain);
+    const void *x[3] = {p.q, p.k, p.v}, *dy[3] = {p.dqo, p.dko, nullptr}, *gain[3] = {p.q_gain, p.k_gain, nullptr};
+    void* y[3] = {p.qo, p.ko, p.vo};
+    const int64_t *xs[3] = {d.q_stride, d.k_stride, d.v_stride}, *os[3] = {d.q_out_stride, d.k_out_stride, d.v_out_stride};
+    int parts = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (!x[i]) continue;
+        HeadTensor& t = a.t[a.kinds];
+        a.kind[a.kinds++] = i;
+        t.x = x[i];
+        t.dy = dy[i];
+        t.y = y[i];
+        t.gain = static_cast<const float*>(gain[i]);
+        for (int n = 0; n < 3; ++n) {
+            t.xs[n] = xs[i][n];
+            t.ys[n] = (bwd ? xs : os)[i][n];
+            t.dys[n] = os[i][n];
+        }
+        t.heads = i == 0 ? d.heads : d.kv_heads;
+        t.first = parts;
+        parts += head_parts(t.heads, d.head_dim);
+    }
     a.pos = static_cast<const int32_t*>(p.pos);
     a.slot = static_cast<const int32_t*>(p.slot);
     a.len = static_cast<const int32_t*>(p.len);
     a.batch = d.batch; a.tokens = d.tokens;
-    const int per_wave = 64 / head_lanes(d.head_dim);
-    for (int i = 0; i < 3; ++i) {
-        a.heads[i] = !a.x[i] ? 0 : i == 0 ? d.heads : d.kv_heads;
-        a.groups[i] = (int)ceil_div(a.heads[i], per_wave);
-    }
     a.dim = d.head_dim; a.rope = d.rope_dims; a.near = d.neighbours; a.cache = d.cache_tokens; a.eps = d.eps;
-    a.rows = head_rows((int64_t)d.batch * d.tokens, d.rope_dims / 2);
     head_turns(d.rope_dims, d.rope_base, a.turn);
     return a;
 }
 
+void head_sums(sa3k_ctx* ctx, const HeadPtrs& p, const float* part, int nq, int nk, int dim) {
+    KernelScope ks(ctx, "head_norm_bwd_sum");
+    launch_k(ctx, true, head_norm_sum_kernel, dim3((unsigned)ceil_div(dim, 64), 2), dim3(kColumnSumThreads), 0, part, nq, nk, dim,
+             static_cast<float*>(p.dq_gain), static_cast<float*>(p.dk_gain), p.accumulate);
+    SA3K_LAUNCHED();
+}
+
 template <class T, int LPH>
 void head_launch(sa3k_ctx* ctx, const HeadArgs& a, const HeadPtrs& p, bool bwd) {
-    const int64_t blocks = ceil_div((int64_t)a.batch * a.tokens, a.rows);
+    const int64_t rows = (int64_t)a.batch * a.tokens;
+    int of[3] = {0, 0, 0}, parts = 0;   // parts of each
+    for (int i = 0; i < a.kinds; ++i) parts += of[a.kind[i]] = head_parts(a.t[i].heads, a.dim);
     if (!bwd) {
         KernelScope ks(ctx, "head_norm_fwd");
-        launch_k(ctx, true, head_norm_fwd_kernel<T, LPH>, dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), dim3(kThreads), 0, a);
+        launch_k(ctx, true, head_norm_fwd_kernel<T, LPH>, dim3((unsigned)ceil_div(rows, kFwdWaves), (unsigned)parts),
+                 dim3(64 * kFwdWaves), 0, a);
         SA3K_LAUNCHED();
         return;
     }
     const bool sums = p.dq_gain || p.dk_gain;
-    const int64_t rounds = ceil_div(blocks, sums ? kHeadBwdGroups : 1 << 20);
-    const int grid = (int)ceil_div(blocks, rounds);   // workgroups of the same number of rounds each
-    float* part = sums ? layer_workspace(ctx, (size_t)grid * 2 * (size_t)a.dim * sizeof(float)) : nullptr;
+    const int64_t blocks = ceil_div(rows, kBwdWaves), most = sums ? std::max<int64_t>(1, kHeadBwdGroups / parts) : 1 << 20;
+    const int grid = (int)ceil_div(blocks, ceil_div(blocks, most));   // workgroups of the same number of rounds each
+    float* part = sums ? layer_workspace(ctx, (size_t)grid * parts * (size_t)a.dim * sizeof(float)) : nullptr;
     {
         KernelScope ks(ctx, "head_norm_bwd");
-        launch_k(ctx, !sums, head_norm_bwd_kernel<T, LPH>, dim3((unsigned)grid), dim3(kThreads), 0, a, part);
+        launch_k(ctx, !sums, head_norm_bwd_kernel<T, LPH>, dim3((unsigned)grid, (unsigned)parts), dim3(64 * kBwdWaves), 0, a, part);
         SA3K_LAUNCHED();
     }
-    if (sums) {
-        KernelScope ks(ctx, "head_norm_bwd_sum");
-        launch_k(ctx, true, head_norm_sum_kernel, dim3((unsigned)ceil_div(2 * a.dim, 64)), dim3(kColumnSumThreads), 0, part, grid,
-                 a.dim, static_cast<float*>(p.dq_gain), static_cast<float*>(p.dk_gain), p.accumulate);
-        SA3K_LAUNCHED();
-    }
+    if (sums) head_sums(ctx, p, part, of[0] * grid, of[1] * grid, a.dim);
 }
 template <class T>
 void head_run(sa3k_ctx* ctx, const HeadArgs& a, const HeadPtrs& p, bool bwd) {
@@ -367,11 +398,7 @@ void head_run(sa3k_ctx* ctx, const HeadArgs& a, const HeadPtrs& p, bool bwd) {
 void head_dispatch(sa3k_ctx* ctx, const sa3k_head_norm& d, const HeadPtrs& p, bool bwd) {
     DeviceScope dev(ctx);
     if (d.batch == 0 || d.tokens == 0) {
-        if (bwd && !p.accumulate && (p.dq_gain || p.dk_gain)) {   // sums over nothing
-            head_norm_sum_kernel<<<(unsigned)ceil_div(2 * d.head_dim, 64), kColumnSumThreads, 0, ctx->stream>>>(
-                nullptr, 0, d.head_dim, static_cast<float*>(p.dq_gain), static_cast<float*>(p.dk_gain), 0);
-            SA3K_LAUNCHED();
-        }
+        if (bwd && !p.accumulate && (p.dq_gain || p.dk_gain)) head_sums(ctx, p, nullptr, 0, 0, d.head_dim);   // over nothing
         return;
     }
     const HeadArgs a = head_args(d, p, bwd);

@@ -55,6 +55,28 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T v[N];
 };
 
+// Where addresses come from memory, the compiler has to be told that they are of global memory. 16 bytes at a time, at an address
+// that is aligned to an element (elements of T, two or four bytes); store16_past goes past the caches.
+#define SA3K_GLOBAL __attribute__((address_space(1)))
+typedef unsigned u32x4a __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x4at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <class T>
+__device__ __forceinline__ u32x4a load16(const SA3K_GLOBAL T* p) {
+    if constexpr (sizeof(T) == 4) return *(const SA3K_GLOBAL u32x4at4*)p;
+    else return *(const SA3K_GLOBAL u32x4at2*)p;
+}
+template <class T>
+__device__ __forceinline__ void store16(SA3K_GLOBAL T* p, u32x4a v) {
+    if constexpr (sizeof(T) == 4) *(SA3K_GLOBAL u32x4at4*)p = u32x4at4(v);
+    else *(SA3K_GLOBAL u32x4at2*)p = u32x4at2(v);
+}
+template <class T>
+__device__ __forceinline__ void store16_past(SA3K_GLOBAL T* p, u32x4a v) {
+    if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(u32x4at4(v), (SA3K_GLOBAL u32x4at4*)p);
+    else __builtin_nontemporal_store(u32x4at2(v), (SA3K_GLOBAL u32x4at2*)p);
+}
+
 // The sums of `parts` workspace rows of n floats each: a workgroup takes 64 columns, a sixteenth of the rows a wave, eight
 // rows in flight; added in row order within a wave, then wave by wave. Calls store(i, sum) for column i. (With four waves a
 // workgroup 512 rows of 2050 columns took 9.4 us.)

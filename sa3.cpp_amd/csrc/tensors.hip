@@ -28,23 +28,6 @@ constexpr int kMostGroups = 2048;                         // eight workgroups a 
 template <class T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
-// Addresses come from memory here, so the compiler has to be told that they are of global memory. 16 bytes at a time, at an address that is
-// aligned to an element; the results past the caches.
-#define SA3K_GLOBAL __attribute__((address_space(1)))
-typedef unsigned u32x4a __attribute__((ext_vector_type(4)));
-typedef unsigned u32x4at2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef unsigned u32x4at4 __attribute__((ext_vector_type(4), aligned(4)));
-template <class T>
-__device__ __forceinline__ u32x4a load16(const SA3K_GLOBAL T* p) {
-    if constexpr (sizeof(T) == 4) return *(const SA3K_GLOBAL u32x4at4*)p;
-    else return *(const SA3K_GLOBAL u32x4at2*)p;
-}
-template <class T>
-__device__ __forceinline__ void store16(SA3K_GLOBAL T* p, u32x4a v) {
-    if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(u32x4at4(v), (SA3K_GLOBAL u32x4at4*)p);
-    else __builtin_nontemporal_store(u32x4at2(v), (SA3K_GLOBAL u32x4at2*)p);
-}
-
 // Whole pieces keep all of a thread's loads in registers, kThreads apart; shorter ones go load by load.
 template <class T>
 __device__ __forceinline__ bool whole(const TensorPiece& p) { return p.n == kPieceBytes / (int)sizeof(T); }
@@ -100,7 +83,7 @@ __device__ __forceinline__ void scale_store(const TensorPiece& p, int i, u32x4a 
     }
     if (WHOLE || i + V <= p.n) {
 #pragma unroll
-        for (int w = 0; w < V / W; ++w) store16(o + i + w * W, __builtin_bit_cast(u32x4a, r[w]));
+        for (int w = 0; w < V / W; ++w) store16_past(o + i + w * W, __builtin_bit_cast(u32x4a, r[w]));
     } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)

@@ -27,7 +27,7 @@ int head_norm_null() {
     return head_norm_check(nullptr, HeadPtrs(), false, &code) ? code : 0;
 }
 void turns(int dims, float base, uint64_t* out) { head_turns(dims, base, out); }
-int rows(int64_t n, int pairs) { return head_rows(n, pairs); }
+int parts(int heads, int dim) { return head_parts(heads, dim); }
 int lanes(int dim) { return head_lanes(dim); }
 
 }  // extern "C"

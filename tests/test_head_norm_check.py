@@ -110,14 +110,11 @@ def test_turns(host, dims, base):
 
 
 def test_launch_shapes(host):
-    host.rows.argtypes = [C.c_int64, C.c_int]
-    for rows in (1, 2047, 2048, 5000, 1 << 20):
-        for pairs in (0, 8, 64, 128):
-            n = host.rows(rows, pairs)
-            assert 1 <= n <= 4 and n * pairs <= 256 and (n == 1 or rows // n >= 1024)
     for dim in range(8, 257, 8):
         n = host.lanes(dim)
         assert 64 % n == 0 and n * 8 >= dim
+        for heads in (1, 2, 7, 24, 65535):
+            assert heads <= host.parts(heads, dim) * (64 // n) * 4 and host.parts(heads, dim) <= 65535 // 2
 
 
 def test_angles_are_exact_modulo_a_turn():
