@@ -17,7 +17,7 @@
 namespace {
 using namespace sa3k;
 
-constexpr int kFwdWaves = 4, kBwdWaves = 8;   // of a workgroup
+constexpr int kFwdWaves = 4, kBwdWaves = 4;   // of a workgroup
 
 struct HeadTensor {   // q, k or v
     const void *x, *dy;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kColumnSumThreads) void head_norm_sum_kernel(const 
 }
 
 // Workgroups of the backward with gains' gradients, at the most: each writes 4 dim bytes that the second launch reads again.
-constexpr int kHeadBwdGroups = 512;
+constexpr int kHeadBwdGroups = 1024;
 
 HeadArgs head_args(const sa3k_head_norm& d, const HeadPtrs& p, bool bwd) {
     HeadArgs a{};
