@@ -10,13 +10,6 @@
 
 namespace {
 
-// act(z) and its slope
-__device__ __forceinline__ float2 act_and_slope(float z, int act) {
-    float v[1] = {z};
-    act_values(v, act);
-    return make_float2(v[0], act_slope(z, act));
-}
-
 // Few rows (at most 16): 16 columns of the output a workgroup, whose eight waves split K in steps of 32 and read both weights
 // straight from memory into the MFMA's registers (each element once); the waves' sums are joined in LDS. Bound by HBM and the
 // latency of a launch.
@@ -89,23 +82,30 @@ __global__ __launch_bounds__(512) void gated_few_kernel(GemmArgs a) {
 struct DzArgs {
     const void *dY, *G, *U;
     int64_t lddy, ldz, M, N, half;
-    int act;
-    void* dz;            // [M][2 half]: dg, then du, zeros behind each (null: not stored)
-    float* part;         // [gridDim.y][2][N] column sums of this workgroup's rows (null: none, or a single row of workgroups)
-    float *dbg, *dbu;    // a single row of workgroups writes these itself (each may be null)
+    int act, cols, rows;   // cols: workgroups that share the columns; rows: that share the rows
+    void* dz;              // [M][2 half]: dg, then du, zeros behind each (null: not stored)
+    float* part;           // [rows][2][N] column sums of this workgroup's rows (null: none, or a single row of workgroups)
+    float *dbg, *dbu;      // a single row of workgroups writes these itself (each may be null)
     int accumulate;
 };
-// A workgroup takes 256 columns, 8 a thread, eight rows at a time. Bound by HBM.
-template <class T>
-__global__ __launch_bounds__(256) void gated_dz_kernel(DzArgs a) {
-    __shared__ float red[2][8][256 + 8];
-    const int c = (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
-    const int64_t n = (int64_t)blockIdx.x * 256 + c;
+// dg and du of COLS columns a workgroup, 8 a thread, 2048 / COLS rows at a time. Bound by HBM: 2176 x 6144 bf16 silu, 134 MB, 26 us.
+// The workgroups behind those pad the products' operands, which need nothing of this pass: a launch less.
+template <class T, int COLS>
+__global__ __launch_bounds__(256) void gated_dz_kernel(DzArgs a, PadArgs pads) {
+    constexpr int TPR = COLS / 8, ROWS = 256 / TPR;   // threads a row, rows at a time
+    if ((int)blockIdx.x >= a.cols * a.rows) {
+        pad_body<T>(pads, (int)blockIdx.x - a.cols * a.rows, (int)gridDim.x - a.cols * a.rows);
+        return;
+    }
+    __shared__ float red[2][ROWS][COLS + 8];
+    const int by = (int)blockIdx.x / a.cols, bx = (int)blockIdx.x - by * a.cols;
+    const int c = ((int)threadIdx.x % TPR) * 8, rl = (int)threadIdx.x / TPR;
+    const int64_t n = (int64_t)bx * COLS + c;
     float sg[8], su[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) sg[e] = su[e] = 0.f;
     // (lanes past the last column go along, as zeros: a run of such instructions with few lanes enabled takes longer)
-    for (int64_t m = (int64_t)blockIdx.y * 8 + rl; m < a.M; m += (int64_t)gridDim.y * 8) {
+    for (int64_t m = (int64_t)by * ROWS + rl; m < a.M; m += (int64_t)a.rows * ROWS) {
         float d[8], g[8], u[8];
         load8(static_cast<const T*>(a.dY) + m * a.lddy, n, a.N, d);
         load8(static_cast<const T*>(a.G) + m * a.ldz, n, a.N, g);
@@ -134,32 +134,62 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(DzArgs a) {
         red[1][rl][c + e] = su[e];
     }
     __syncthreads();
-    const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (j >= a.N) return;
-    float t[2] = {0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        t[0] += red[0][w][threadIdx.x];
-        t[1] += red[1][w][threadIdx.x];
-    }
-    if (a.part) {
-        float* p = a.part + (int64_t)blockIdx.y * 2 * a.N + j;
-        p[0] = t[0];
-        p[a.N] = t[1];
-    } else {
-        if (a.dbg) a.dbg[j] = a.accumulate ? a.dbg[j] + t[0] : t[0];
-        if (a.dbu) a.dbu[j] = a.accumulate ? a.dbu[j] + t[1] : t[1];
+    for (int i = (int)threadIdx.x; i < 2 * COLS; i += 256) {
+        const int w = i / COLS, k = i % COLS;
+        const int64_t j = (int64_t)bx * COLS + k;
+        if (j >= a.N) continue;
+        float t = 0.f;
+#pragma unroll 8
+        for (int r = 0; r < ROWS; ++r) t += red[w][r][k];
+        if (a.part) {
+            a.part[((int64_t)by * 2 + w) * a.N + j] = t;
+        } else {
+            float* d = w ? a.dbu : a.dbg;
+            if (d) d[j] = a.accumulate ? d[j] + t : t;
+        }
     }
 }
 
-// the biases' gradients from the workgroups' sums
-__global__ __launch_bounds__(kColumnSumThreads) void gated_db_kernel(const float* __restrict__ part, int parts, int64_t N, float* dbg,
-                                                                     float* dbu, int accumulate) {
-    column_sums(part, parts, 2 * N, [&](int64_t i, float t) {
-        float* d = i < N ? dbg : dbu;
-        const int64_t c = i < N ? i : i - N;
-        if (d) d[c] = accumulate ? d[c] + t : t;
-    });
+// The biases' gradients from the workgroups' sums: 16 columns a workgroup, a sixteenth of the rows a thread, eight in flight; added in
+// row order within a thread, then thread by thread
+struct DbArgs {
+    const float* part;
+    int parts, accumulate;
+    int64_t N;
+    float *dbg, *dbu;
+};
+__device__ __forceinline__ void db_body(const DbArgs& a, int64_t block) {
+    __shared__ float s[16][17];
+    const int k = threadIdx.x & 15, w = threadIdx.x >> 4, per = (a.parts + 15) / 16;
+    const int lo = min(a.parts, w * per), hi = min(a.parts, lo + per);
+    const int64_t i = block * 16 + k;
+    float t = 0.f;
+    if (i < 2 * a.N)
+        for (int r = lo; r < hi; r += 8) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = a.part[(int64_t)min(r + u, hi - 1) * 2 * a.N + i];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (r + u < hi) t += v[u];
+        }
+    s[w][k] = t;
+    __syncthreads();
+    if (w || i >= 2 * a.N) return;
+    t = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t += s[r][k];
+    float* d = i < a.N ? a.dbg : a.dbu;
+    const int64_t c = i < a.N ? i : i - a.N;
+    if (d) d[c] = a.accumulate ? d[c] + t : t;
+}
+// what is left to add up after a backward's products, in one launch: dX's splits (x_wgs workgroups), dW's (w_wgs), the biases' gradients
+template <class T>
+__global__ __launch_bounds__(256) void gated_sums_kernel(GemmArgs x, GemmArgs w, DbArgs db, int64_t x_wgs, int64_t w_wgs) {
+    const int64_t b = blockIdx.x;
+    if (b < x_wgs) sum_body<T, kGatedInput>(x, b);
+    else if (b < x_wgs + w_wgs) sum_body<T, kGatedWeight>(w, b - x_wgs);
+    else db_body(db, b - x_wgs - w_wgs);
 }
 
 template <class T>
@@ -183,8 +213,8 @@ void fwd_run(sa3k_ctx* ctx, const GatedArgs& p) {
     const size_t ou = s.take(padded ? (size_t)p.N * Kp * 2 : 0), os = s.take(split_bytes(plan, p.M, 2 * up8(p.N)));
     char* ws = s.need ? reinterpret_cast<char*>(layer_workspace(ctx, s.need)) : nullptr;
     if (padded) {
-        pad<T>(ctx, PadArgs{{p.X, p.Wg}, {p.ldx, p.ldw}, {p.M, p.N}, p.K, {ws + ox, ws + og}}, "gated_linear_pad");
-        pad<T>(ctx, PadArgs{{p.Wu, nullptr}, {p.ldw, 0}, {p.N, 0}, p.K, {ws + ou, nullptr}}, "gated_linear_pad");
+        pad<T>(ctx, PadArgs{{p.X, p.Wg, p.Wu}, {p.ldx, p.ldw, p.ldw}, {p.M, p.N, p.N}, p.K, {ws + ox, ws + og, ws + ou}},
+               "gated_linear_pad");
         a.A = ws + ox;
         a.B = ws + og;
         a.B2 = ws + ou;
@@ -193,12 +223,17 @@ void fwd_run(sa3k_ctx* ctx, const GatedArgs& p) {
     tile_run<T, kGatedForward>(ctx, a, plan, reinterpret_cast<float*>(ws + os), "gated_linear_fwd", "gated_linear_sum");
 }
 
-// Row shares of the pass over dY, g and u: one for up to 64 rows (which saves the launch that adds up shares), else about 128,
-// each of the same number of rounds of eight rows.
-int dz_parts(int64_t M) {
-    if (M <= 64) return 1;
-    const int64_t groups = std::max<int64_t>(1, ceil_div(M, 8)), rounds = ceil_div(groups, 128);
-    return (int)ceil_div(groups, rounds);
+// The pass over dY, g and u: 256 columns a workgroup; 64, and four times the rows at a time, for up to 64 rows, whose column sums one
+// row of workgroups then adds up itself without a launch for the shares. Row shares: all there are rounds for where no column sums are
+// asked for, else about 128, each of the same number of rounds.
+struct DzPlan {
+    int cols, rows;   // columns a workgroup, row shares
+};
+DzPlan dz_plan(int64_t M, int64_t half, bool sums) {
+    if (M <= 64) return DzPlan{64, sums ? 1 : (int)std::max<int64_t>(1, ceil_div(M, 32))};
+    const int64_t groups = ceil_div(M, 8), most = sums ? 128 : std::min<int64_t>(4096, (1 << 22) / ceil_div(half, 256));
+    const int64_t rounds = ceil_div(groups, most);
+    return DzPlan{256, (int)ceil_div(groups, rounds)};
 }
 
 template <class T>
@@ -209,30 +244,25 @@ void bwd_run(sa3k_ctx* ctx, const GatedArgs& p) {
     const bool pw = do_x && (!loads16(p.Wg, p.ldw, K) || !loads16(p.Wu, p.ldw, K));
     ProdPair plan{false, prod_plan(M > 0 ? M : 1, K, 2 * half), prod_plan(2 * half, K, M > 0 ? M : 1)};
     if (do_x && do_w) plan = prod_pair({M, K, 2 * half}, {2 * half, K, M});
-    const int parts = dz_parts(M);
+    const DzPlan dz = dz_plan(M, half, sums);
     Scratch s;
     const size_t oz = s.take(products ? (size_t)M * 2 * half * 2 : 0), ox = s.take(px ? (size_t)M * Kp * 2 : 0);
     const size_t og = s.take(pw ? (size_t)N * Kp * 2 : 0), ou = s.take(pw ? (size_t)N * Kp * 2 : 0);
-    const size_t ob = s.take(sums && parts > 1 ? (size_t)parts * 2 * N * 4 : 0);
+    const size_t ob = s.take(sums && dz.rows > 1 ? (size_t)dz.rows * 2 * N * 4 : 0);
     const size_t sx = do_x ? split_bytes(plan.a, M, Kp) : 0, sw = do_w ? split_bytes(plan.b, 2 * half, Kp) : 0;
-    const size_t osx = s.take(plan.together ? sx : std::max(sx, sw)), osw = plan.together ? s.take(sw) : osx;
+    const size_t osx = s.take(sx), osw = s.take(sw);
     char* ws = s.need ? reinterpret_cast<char*>(layer_workspace(ctx, s.need)) : nullptr;
-    float* part = sums && parts > 1 ? reinterpret_cast<float*>(ws + ob) : nullptr;
+    float* part = sums && dz.rows > 1 ? reinterpret_cast<float*>(ws + ob) : nullptr;
     if (products || sums) {
-        DzArgs z{p.dY, p.G, p.U, p.lddy, p.ldz, M, N, half, p.act, products && M > 0 ? ws + oz : nullptr, part,
-                 part ? nullptr : p.dbg, part ? nullptr : p.dbu, p.accumulate};
+        const DzArgs z{p.dY, p.G, p.U, p.lddy, p.ldz, M, N, half, p.act, (int)ceil_div(half, dz.cols), dz.rows,
+                       products && M > 0 ? ws + oz : nullptr, part, part ? nullptr : p.dbg, part ? nullptr : p.dbu, p.accumulate};
+        const PadArgs pads{{p.Wg, p.Wu, p.X}, {p.ldw, p.ldw, p.ldx}, {pw ? N : 0, pw ? N : 0, px ? M : 0}, K, {ws + og, ws + ou, ws + ox}};
+        const int64_t grid = (int64_t)z.cols * z.rows + pad_blocks(pads);
         KernelScope ks(ctx, "gated_linear_dz");
-        launch_k(ctx, !products && !part, gated_dz_kernel<T>, dim3((unsigned)ceil_div(half, 256), (unsigned)parts), dim3(256), 0, z);
+        launch_k(ctx, !products && !part, dz.cols == 64 ? gated_dz_kernel<T, 64> : gated_dz_kernel<T, 256>, dim3((unsigned)grid), dim3(256),
+                 0, z, pads);
         SA3K_LAUNCHED();
     }
-    if (part) {
-        KernelScope ks(ctx, "gated_linear_db");
-        launch_k(ctx, !products, gated_db_kernel, dim3((unsigned)ceil_div(2 * N, 64)), dim3(kColumnSumThreads), 0, part, parts, N,
-                 p.dbg, p.dbu, p.accumulate);
-        SA3K_LAUNCHED();
-    }
-    pad<T>(ctx, PadArgs{{p.Wg, p.Wu}, {p.ldw, p.ldw}, {pw ? N : 0, pw ? N : 0}, K, {ws + og, ws + ou}}, "gated_linear_pad");
-    pad<T>(ctx, PadArgs{{p.X, nullptr}, {p.ldx, 0}, {px ? M : 0, 0}, K, {ws + ox, nullptr}}, "gated_linear_pad");
     GemmArgs x{}, w{};
     x.half = w.half = half;
     x.each = w.each = N;
@@ -254,20 +284,24 @@ void bwd_run(sa3k_ctx* ctx, const GatedArgs& p) {
         w.accumulate = p.accumulate;
     }
     float *part_x = reinterpret_cast<float*>(ws + osx), *part_w = reinterpret_cast<float*>(ws + osw);
-    if (plan.together) {
+    const bool pair = plan.together && products;
+    if (pair) {
         const int64_t nx = plan_into<kGatedInput>(x, plan.a, part_x), nw = plan_into<kGatedWeight>(w, plan.b, part_w);
-        {
-            KernelScope ks(ctx, "gated_linear_dx_dw", 8.0 * (double)M * (double)N * (double)K);
-            launch_k(ctx, x.splits == 1 && w.splits == 1, prod_pair_kernel<T, kGatedInput, kGatedWeight>, dim3((unsigned)(nx + nw)),
-                     dim3(256), 0, x, w, (int)nx);
-            SA3K_LAUNCHED();
-        }
-        sum_splits<T, kGatedInput>(ctx, x, "gated_linear_sum");
-        sum_splits<T, kGatedWeight>(ctx, w, "gated_linear_sum");
-        return;
+        KernelScope ks(ctx, "gated_linear_dx_dw", 8.0 * (double)M * (double)N * (double)K);
+        launch_k(ctx, x.splits == 1 && w.splits == 1 && !part, prod_pair_kernel<T, kGatedInput, kGatedWeight>, dim3((unsigned)(nx + nw)),
+                 dim3(256), 0, x, w, (int)nx);
+        SA3K_LAUNCHED();
+    } else {
+        if (do_x) tile_launch<T, kGatedInput>(ctx, x, plan.a, part_x, "gated_linear_dx");
+        if (do_w) tile_launch<T, kGatedWeight>(ctx, w, plan.b, part_w, "gated_linear_dw");
     }
-    if (do_x) tile_run<T, kGatedInput>(ctx, x, plan.a, part_x, "gated_linear_dx", "gated_linear_sum");
-    if (do_w) tile_run<T, kGatedWeight>(ctx, w, plan.b, part_w, "gated_linear_dw", "gated_linear_sum");
+    const int64_t x_wgs = do_x && x.splits > 1 ? ceil_div(M * (x.pitch / 8), 256) : 0;
+    const int64_t w_wgs = do_w && w.splits > 1 ? ceil_div(2 * half * (w.pitch / 8), 256) : 0, db_wgs = part ? ceil_div(2 * N, 16) : 0;
+    if (x_wgs + w_wgs + db_wgs == 0) return;
+    const DbArgs db{part, dz.rows, p.accumulate, N, p.dbg, p.dbu};
+    KernelScope ks(ctx, "gated_linear_sum");
+    launch_k(ctx, true, gated_sums_kernel<T>, dim3((unsigned)(x_wgs + w_wgs + db_wgs)), dim3(256), 0, x, w, db, x_wgs, w_wgs);
+    SA3K_LAUNCHED();
 }
 
 }  // namespace

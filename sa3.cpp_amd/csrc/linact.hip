@@ -132,7 +132,7 @@ void fwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     const size_t os = s.take(split_bytes(plan, p.M, up8(p.N)));
     char* ws = s.need ? reinterpret_cast<char*>(layer_workspace(ctx, s.need)) : nullptr;
     if (px || pw) {
-        pad<T>(ctx, PadArgs{{p.X, p.W}, {p.ldx, p.ldw}, {p.M, p.N}, p.K, {ws + ox, ws + ow}}, "linear_act_pad");
+        pad<T>(ctx, PadArgs{{p.X, p.W, nullptr}, {p.ldx, p.ldw, 0}, {p.M, p.N, 0}, p.K, {ws + ox, ws + ow, nullptr}}, "linear_act_pad");
         a.A = ws + ox;
         a.B = ws + ow;
         a.lda = a.ldb = a.K = Kp;
@@ -182,7 +182,7 @@ void bwd_run(sa3k_ctx* ctx, const ProdArgs& p) {
     const void* g = own_dz ? dz : p.dY;
     const int64_t ldg = own_dz ? Np : p.lddy;
     GemmArgs x{}, w{};
-    pad<T>(ctx, PadArgs{{p.W, p.X}, {p.ldw, p.ldx}, {pw ? N : 0, px ? M : 0}, K, {ws + ow, ws + ox}}, "linear_act_pad");
+    pad<T>(ctx, PadArgs{{p.W, p.X, nullptr}, {p.ldw, p.ldx, 0}, {pw ? N : 0, px ? M : 0, 0}, K, {ws + ow, ws + ox, nullptr}}, "linear_act_pad");
     if (do_x) {   // [M][K] = dz [M][N] . W [N][K]
         x.A = g; x.lda = ldg;
         x.B = pw ? ws + ow : p.W;

@@ -132,6 +132,24 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     return 1.f;
 }
 
+// act(z) and its slope, as act_values and act_slope give them, from one exponential
+__device__ __forceinline__ float2 act_and_slope(float z, int act) {
+    if (act == SA3K_ACT_SILU) {
+        const float g = sigmoid(z);
+        return make_float2(z * g, g * (1.f + z * (1.f - g)));
+    }
+    if (act == SA3K_ACT_GELU) {
+        float bell;
+        const float below = normal_below(z, bell);
+        return make_float2(z * below, below + z * bell * 0.39894228040143268f);
+    }
+    if (act == SA3K_ACT_GELU_TANH) {
+        const float g = tanh_gate(z), y = fminf(fmaxf(z, -10.f), 10.f);
+        return make_float2(z * g, __builtin_fmaf(y * g * (1.f - g) * 1.5957691216057308f, 1.f + 0.134145f * y * y, g) + 0.f * z);
+    }
+    return make_float2(act == SA3K_ACT_RELU && z <= 0.f ? 0.f : z, act_slope(z, act));
+}
+
 // n .. n + 7 of a row of `cols` elements, zeros past its end
 template <class S>
 __device__ __forceinline__ void load8(const S* p, int64_t n, int64_t cols, float (&v)[8]) {
@@ -687,8 +705,8 @@ __global__ __launch_bounds__(256, 2) void prod_pair_kernel(GemmArgs x, GemmArgs 
 
 // the K splits' sums in their order, then the epilogue
 template <class T, int P>
-__global__ __launch_bounds__(256) void prod_sum_kernel(GemmArgs a) {
-    const int64_t chunks = a.pitch / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / chunks, n = (i - m * chunks) * 8;
+__device__ __forceinline__ void sum_body(const GemmArgs& a, int64_t block) {
+    const int64_t chunks = a.pitch / 8, i = block * 256 + threadIdx.x, m = i / chunks, n = (i - m * chunks) * 8;
     if (m >= a.M) return;
     float v[8], b[8];
     Pack<T, 8> r;
@@ -709,6 +727,10 @@ __global__ __launch_bounds__(256) void prod_sum_kernel(GemmArgs a) {
             v[e + 3] += x.w;
         }
     finish8<T, P>(a, m, n, v, b, r, true);
+}
+template <class T, int P>
+__global__ __launch_bounds__(256) void prod_sum_kernel(GemmArgs a) {
+    sum_body<T, P>(a, blockIdx.x);
 }
 template <class T>
 __global__ __launch_bounds__(256) void gated_sum_kernel(GemmArgs a) {
@@ -734,23 +756,30 @@ __global__ __launch_bounds__(256) void gated_sum_kernel(GemmArgs a) {
     finish_gated8<T>(a, m, n, v[0], v[1], bg, bu, true);
 }
 
-// rows [rows][cols] into rows of cols rounded up to a multiple of 8, zeros behind them; two operands in one launch (either may
+// rows [rows][cols] into rows of cols rounded up to a multiple of 8, zeros behind them; up to three operands in one launch (each may
 // have no rows)
 struct PadArgs {
-    const void* src[2];
-    int64_t ld[2], rows[2], cols;
-    void* dst[2];
+    const void* src[3];
+    int64_t ld[3], rows[3], cols;
+    void* dst[3];
 };
+inline int64_t pad_chunks(const PadArgs& a) { return (a.rows[0] + a.rows[1] + a.rows[2]) * ((a.cols + 7) / 8); }
+template <class T>
+__device__ __forceinline__ void pad_body(const PadArgs& a, int64_t block, int64_t blocks) {
+    const int64_t chunks = (a.cols + 7) / 8, n0 = a.rows[0] * chunks, n1 = n0 + a.rows[1] * chunks, n = n1 + a.rows[2] * chunks;
+    for (int64_t i = block * 256 + threadIdx.x; i < n; i += blocks * 256) {
+        const int w = i >= n1 ? 2 : i >= n0 ? 1 : 0;
+        const int64_t j = i - (w == 2 ? n1 : w == 1 ? n0 : 0), r = j / chunks, c = (j - r * chunks) * 8;
+        const void* src = w == 2 ? a.src[2] : w == 1 ? a.src[1] : a.src[0];
+        void* dst = w == 2 ? a.dst[2] : w == 1 ? a.dst[1] : a.dst[0];
+        float v[8];
+        load8(static_cast<const T*>(src) + r * (w == 2 ? a.ld[2] : w == 1 ? a.ld[1] : a.ld[0]), c, a.cols, v);
+        store8(static_cast<T*>(dst) + r * chunks * 8, c, chunks * 8, v);
+    }
+}
 template <class T>
 __global__ __launch_bounds__(256) void prod_pad_kernel(PadArgs a) {
-    const int64_t chunks = (a.cols + 7) / 8, n0 = a.rows[0] * chunks, n = n0 + a.rows[1] * chunks;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int w = i >= n0;
-        const int64_t j = w ? i - n0 : i, r = j / chunks, c = (j - r * chunks) * 8;
-        float v[8];
-        load8(static_cast<const T*>(w ? a.src[1] : a.src[0]) + r * (w ? a.ld[1] : a.ld[0]), c, a.cols, v);
-        store8(static_cast<T*>(w ? a.dst[1] : a.dst[0]) + r * chunks * 8, c, chunks * 8, v);
-    }
+    pad_body<T>(a, blockIdx.x, gridDim.x);
 }
 
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
@@ -771,12 +800,12 @@ struct Scratch {
     }
 };
 
+inline int64_t pad_blocks(const PadArgs& a) { return std::min<int64_t>(ceil_div(pad_chunks(a), 256), 65536); }
 template <class T>
 void pad(sa3k_ctx* ctx, const PadArgs& a, const char* name) {
-    const int64_t n = (a.rows[0] + a.rows[1]) * (up8(a.cols) / 8);
-    if (n == 0) return;
+    if (pad_chunks(a) == 0) return;
     KernelScope ks(ctx, name);
-    launch_k(ctx, false, prod_pad_kernel<T>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 256), 65536)), dim3(256), 0, a);
+    launch_k(ctx, false, prod_pad_kernel<T>, dim3((unsigned)pad_blocks(a)), dim3(256), 0, a);
     SA3K_LAUNCHED();
 }
 
@@ -804,18 +833,21 @@ void sum_splits(sa3k_ctx* ctx, const GemmArgs& a, const char* name) {
     else launch_k(ctx, true, prod_sum_kernel<T, P>, dim3((unsigned)ceil_div(a.M * (a.pitch / 8), 256)), dim3(256), 0, a);
     SA3K_LAUNCHED();
 }
+// the products alone, splits not added up
+template <class T, int P>
+void tile_launch(sa3k_ctx* ctx, GemmArgs& a, const ProdPlan& p, float* part, const char* name) {
+    const int64_t wgs = plan_into<P>(a, p, part);
+    const dim3 grid((unsigned)wgs);
+    KernelScope ks(ctx, name, (Is<P>::gated_fwd ? 4.0 : 2.0) * (double)a.M * (double)a.N * (double)a.K);
+    if (p.edge == 256) launch_k(ctx, a.splits == 1, prod_big_kernel<T, P>, grid, dim3(512), 0, a);
+    else if (wgs <= 256)   // one workgroup a CU at the most: deeper stages
+        launch_k(ctx, a.splits == 1, prod_tile_kernel<T, 4, P>, grid, dim3(256), 0, a);
+    else launch_k(ctx, a.splits == 1, prod_tile_kernel<T, 2, P>, grid, dim3(256), 0, a);
+    SA3K_LAUNCHED();
+}
 template <class T, int P>
 void tile_run(sa3k_ctx* ctx, GemmArgs& a, const ProdPlan& p, float* part, const char* name, const char* sum_name) {
-    const int64_t wgs = plan_into<P>(a, p, part);
-    {
-        const dim3 grid((unsigned)wgs);
-        KernelScope ks(ctx, name, (Is<P>::gated_fwd ? 4.0 : 2.0) * (double)a.M * (double)a.N * (double)a.K);
-        if (p.edge == 256) launch_k(ctx, a.splits == 1, prod_big_kernel<T, P>, grid, dim3(512), 0, a);
-        else if (wgs <= 256)   // one workgroup a CU at the most: deeper stages
-            launch_k(ctx, a.splits == 1, prod_tile_kernel<T, 4, P>, grid, dim3(256), 0, a);
-        else launch_k(ctx, a.splits == 1, prod_tile_kernel<T, 2, P>, grid, dim3(256), 0, a);
-        SA3K_LAUNCHED();
-    }
+    tile_launch<T, P>(ctx, a, p, part, name);
     sum_splits<T, P>(ctx, a, sum_name);
 }
 
