@@ -525,7 +525,8 @@ SA3K_API int sa3k_linear_act_bwd(sa3k_ctx* ctx, int type, int act, const void* d
  *   g = X Wg^T + bg,  u = X Wu^T + bu,  Y = act(g) u
  * X [M][K], Wg and Wu [N][K] (two tensors, or halves of one), Y, G and U [M][N]; biases f32 [N]; biases, G and U (g and u,
  * for the backward) nullable. Activation and product apply to the f32 g and u; every output is rounded once. Any M
- * (0: nothing), N below 2^21 - 63 and K below 2^22, row pitches below 2^22. NaN and infinities go through the formulas as they stand. */
+ * (0: nothing), N below 2^21 - 63 and K below 2^22, row pitches below 2^22. Outputs overlap no other tensor. NaN and infinities go
+ * through the formulas as they stand. */
 SA3K_API int sa3k_gated_linear_fwd(sa3k_ctx* ctx, int type, int act, const void* X, int64_t ldx, const void* Wg, const void* Wu,
                                    int64_t ldw, const float* bg, const float* bu, int64_t M, int64_t N, int64_t K, void* Y,
                                    int64_t ldy, void* G, void* U, int64_t ldz);
@@ -533,7 +534,8 @@ SA3K_API int sa3k_gated_linear_fwd(sa3k_ctx* ctx, int type, int act, const void*
 /* Its backward from dY and the stored g and u: dg = dY u act'(g), du = dY act(g),
  *   dX = dg Wg + du Wu,  dWg = dg^T X,  dWu = du^T X (both or neither),  dbg and dbu = column sums of dg and du
  * (each nullable). dg and du are rounded to `type` for the products, not for the biases' gradients. dw_type: `type`, or f32;
- * accumulate = 1 adds to dWg and dWu (f32 only), dbg and dbu. act' as in sa3k_linear_act_bwd. Sums run in a fixed order. */
+ * accumulate = 1 adds to dWg and dWu (f32 only), dbg and dbu. Outputs overlap no other tensor. act' as in sa3k_linear_act_bwd; in f16
+ * a dg or du past 65504 is an infinity, as in any f16 backward without loss scaling. Sums run in a fixed order. */
 SA3K_API int sa3k_gated_linear_bwd(sa3k_ctx* ctx, int type, int act, const void* dY, int64_t lddy, const void* G, const void* U,
                                    int64_t ldz, const void* X, int64_t ldx, const void* Wg, const void* Wu, int64_t ldw, int64_t M,
                                    int64_t N, int64_t K, void* dX, int64_t lddx, void* dWg, void* dWu, int dw_type, int64_t lddw,
@@ -562,8 +564,9 @@ typedef struct {
  * modulo a turn to 2^-33 turns). q, k and v with their outputs are each nullable; v is copied. slot device int32 [batch][tokens] (nullable): the
  * row of k_out and v_out that a token's k and v go to, else row t; a slot outside 0 .. cache_tokens - 1 is not stored, and the
  * slots of a sample that are must differ. len device int32 [batch] (nullable): tokens past a sample's length are not read, and
- * their outputs stay as they were. q_out may be q with the same strides; k_out and v_out likewise without slots. Sums and angles f32,
- * outputs rounded once. Tensors need only be aligned to their elements. */
+ * their outputs stay as they were. q_out may be q with the same strides; k_out and v_out likewise without slots; outputs overlap
+ * nothing else. Sums and angles f32 (a head whose squares pass 3e38 gives 0), outputs rounded once. Tensors need only be aligned to
+ * their elements. */
 SA3K_API int sa3k_head_norm_fwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const void* q, const void* k, const void* v,
                                 const float* q_gain, const float* k_gain, const int32_t* pos, const int32_t* slot,
                                 const int32_t* len, void* q_out, void* k_out, void* v_out);
@@ -591,7 +594,7 @@ typedef struct sa3k_tensors sa3k_tensors;   /* a list of them, cut into pieces, 
 
 /* A list of `count` tensors (0: none). It keeps their addresses, not their memory, which has to outlive its calls. An output must not
  * meet another tensor's gradient or output, nor its own gradient but in place; gradients may repeat. Tensors need only be
- * aligned to their elements. Synchronises the stream. */
+ * aligned to their elements. It belongs to the context that made it. Synchronises the stream. */
 SA3K_API int sa3k_tensors_create(sa3k_ctx* ctx, const sa3k_tensor* tensors, int64_t count, sa3k_tensors** out);
 SA3K_API int sa3k_tensors_destroy(sa3k_ctx* ctx, sa3k_tensors* t);
 /* Over all of them, as sa3k_average_and_clip does over an arena:

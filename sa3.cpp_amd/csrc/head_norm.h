@@ -36,6 +36,15 @@ inline bool same_place(const void* x, const void* y, const int64_t* sx, const in
     return true;
 }
 
+// lanes that share a head, eight of its elements each
+inline int head_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+// a wave takes this many groups of 64 / lanes heads at the most, and a tensor's heads are that many waves' to a row
+constexpr int kGroups = 3;
+inline int head_parts(int heads, int dim) {
+    const int per = kGroups * (64 / head_lanes(dim));
+    return (heads + per - 1) / per;
+}
+
 inline const char* head_norm_check(const sa3k_head_norm* d, const HeadPtrs& p, bool bwd, int* code) {
     *code = SA3K_ERR_INVALID;
     if (!d) return "null shape";
@@ -73,6 +82,12 @@ inline const char* head_norm_check(const sa3k_head_norm* d, const HeadPtrs& p, b
     if (!p.q != !p.qo || !p.k != !p.ko || !p.v != !p.vo) return "q, k and v need an output each, and an output its input";
     if (bwd && ((p.q && !p.dqo) || (p.k && !p.dko))) return "q and k need their outputs' gradients";
     if (bwd && ((p.dq_gain && !p.q) || (p.dk_gain && !p.k))) return "a gain's gradient needs its heads";
+    // four rows a workgroup, a launch of fewer than 2^24 workgroups
+    const int64_t parts = head_parts(d->heads, D) + 2 * (int64_t)head_parts(d->kv_heads, D);
+    if (((int64_t)d->batch * d->tokens / 4 + 1) * parts >= ((int64_t)1 << 24)) {
+        *code = SA3K_ERR_UNSUPPORTED;
+        return "batch x tokens x heads is too large for one launch";
+    }
     const char* m = nullptr;
     // backward: dqo and dko lie as the outputs do, dq and dk as q and k do
     const struct { const void* p; const int64_t *st, *n; bool out; } t[8] = {
@@ -97,15 +112,6 @@ inline void head_turns(int dims, float base, uint64_t* turn) {
     const long double step = dims > 0 ? powl((long double)base, -2.0L / (long double)dims) : 0.0L;
     long double f = 1.0L / 6.283185307179586476925286766559L;   // turns a position, pair 0
     for (int i = 0; i < dims / 2; ++i, f *= step) turn[i] = (uint64_t)(f * 18446744073709551616.0L);
-}
-
-// lanes that share a head, eight of its elements each
-inline int head_lanes(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
-// a wave takes this many groups of 64 / lanes heads at the most, and a tensor's heads are that many waves' to a row
-constexpr int kGroups = 3;
-inline int head_parts(int heads, int dim) {
-    const int per = kGroups * (64 / head_lanes(dim));
-    return (heads + per - 1) / per;
 }
 
 }  // namespace sa3k

@@ -74,13 +74,13 @@ def test_forward_on_every_tile(ctx, shape):
 
 
 def backward_case(ctx, kind, M, N, K, variant):
-    """variant 0: plain and aligned; 1: relu, odd pitches, f32 dW added to; 2: dX and one bias' gradient only"""
+    """variant 0: plain and aligned; 1: relu, odd pitches, f32 dW added to; 2: dX and one bias' gradient only; 3: the products only"""
     act = "relu" if variant == 1 else "none"
     x, w, dy = whole(1, (M, K), 2, kind), whole(2, (2 * N, K), 2, kind), whole(5, (M, N), 1, kind)
     g, u = whole(6, (M, N), 2, kind), whole(7, (M, N), 2, kind)
     f, s = (torch.relu(g.float()), (g > 0).float()) if variant == 1 else (g.float(), 1.0)
     dg, du = dy.float() * u.float() * s, dy.float() * f
-    odd, some = variant == 1, variant == 2
+    odd, some, bare = variant == 1, variant == 2, variant == 3
     pad, off = ((1, 3, 2, 5, 1, 2), 1) if odd else ((0,) * 6, 0)
     ddy, dG, dU, dxx = (Pitched(ctx, t, t.shape[1] + p, off) for t, p in ((dy, pad[0]), (g, pad[1]), (u, pad[1]), (x, pad[2])))
     dw = [Pitched(ctx, t, K + pad[3], off) for t in (w[:N], w[N:])]
@@ -90,13 +90,13 @@ def backward_case(ctx, kind, M, N, K, variant):
     ow = [Pitched(ctx, t if odd else torch.zeros((N, K), dtype=TORCH[kind]), K + pad[5], off) for t in old]
     ob = [up(ctx, t) for t in oldb]
     sa3k.gated_linear_bwd(ctx, TYPE[kind], ACTS[act], ddy, dG, dU, None if some else dxx, dw[0], dw[1], M, N, K, dx=ox,
-                          dw_gate=None if some else ow[0], dw_up=None if some else ow[1], db_gate=None if some else ob[0],
-                          db_up=ob[1], dw_type=TYPE["f32"] if odd else None, accumulate=odd, lddy=ddy.ld, ldz=dG.ld, ldx=dxx.ld,
+                          dw_gate=None if some else ow[0], dw_up=None if some else ow[1], db_gate=None if some or bare else ob[0],
+                          db_up=None if bare else ob[1], dw_type=TYPE["f32"] if odd else None, accumulate=odd, lddy=ddy.ld, ldz=dG.ld, ldx=dxx.ld,
                           ldw=dw[0].ld, lddx=ox.ld, lddw=ow[0].ld)
     same(ox.get(), dg @ w[:N].float() + du @ w[N:].float())
     for i, d in enumerate((dg, du)):
-        if some and i == 0:
-            assert np.array_equal(ob[0].numpy(), oldb[0].numpy())
+        if bare or (some and i == 0):
+            assert np.array_equal(ob[i].numpy(), oldb[i].numpy())
         else:
             assert np.array_equal(ob[i].numpy(), (d.double().sum(0) + (oldb[i].double() if odd else 0)).float().numpy())
         if some:
@@ -108,8 +108,14 @@ def backward_case(ctx, kind, M, N, K, variant):
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 @pytest.mark.parametrize("M,N,K", SHAPES)
 def test_backward_is_exact_on_whole_numbers(ctx, kind, M, N, K):
-    for variant in range(3):
+    for variant in range(4):
         backward_case(ctx, kind, M, N, K, variant)
+
+
+def test_backward_of_many_rows(ctx):
+    """more rows than the pass over dY, g and u has shares for, with and without column sums"""
+    for variant in (0, 3):
+        backward_case(ctx, "bf16", 40003, 24, 16, variant)
 
 
 @pytest.mark.parametrize("shape", list(BACKWARD), ids=lambda s: "x".join(map(str, s)))

@@ -61,7 +61,7 @@ def test_accepts(host):
 
 @pytest.mark.parametrize("want,change", [
     (UNSUPPORTED, dict(type=sa3k.TYPE_Q8_0)), (UNSUPPORTED, dict(head_dim=264)), (UNSUPPORTED, dict(head_dim=60)),
-    (UNSUPPORTED, dict(head_dim=0)), (UNSUPPORTED, dict(head_dim=-8)), (UNSUPPORTED, dict(rope_dims=8)), (UNSUPPORTED, dict(rope_dims=40)),
+    (UNSUPPORTED, dict(batch=60, tokens=1 << 20, heads=64)), (UNSUPPORTED, dict(head_dim=0)), (UNSUPPORTED, dict(head_dim=-8)), (UNSUPPORTED, dict(rope_dims=8)), (UNSUPPORTED, dict(rope_dims=40)),
     (INVALID, dict(rope_dims=80)), (INVALID, dict(rope_dims=-16)), (INVALID, dict(neighbours=2)), (INVALID, dict(batch=-1)),
     (INVALID, dict(batch=65536)), (INVALID, dict(tokens=-1)), (INVALID, dict(tokens=1 << 28)), (INVALID, dict(batch=60000, tokens=1 << 20)),
     (INVALID, dict(heads=0)), (INVALID, dict(kv_heads=0)), (INVALID, dict(heads=65536)), (INVALID, dict(eps=-1e-6)),
