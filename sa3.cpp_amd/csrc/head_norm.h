@@ -111,7 +111,7 @@ inline const char* head_norm_check(const sa3k_head_norm* d, const HeadPtrs& p, b
 inline void head_turns(int dims, float base, uint64_t* turn) {
     const long double step = dims > 0 ? powl((long double)base, -2.0L / (long double)dims) : 0.0L;
     long double f = 1.0L / 6.283185307179586476925286766559L;   // turns a position, pair 0
-    for (int i = 0; i < dims / 2; ++i, f *= step) turn[i] = (uint64_t)(f * 18446744073709551616.0L);
+    for (int i = 0; i < dims / 2; ++i, f *= step) turn[i] = (uint64_t)(int64_t)(f * 18446744073709551616.0L);   // (below 2^62)
 }
 
 }  // namespace sa3k

@@ -24,12 +24,13 @@ struct HeadTensor {   // q, k or v
     void* y;
     const float* gain;
     int64_t xs[3], ys[3], dys[3];   // strides of samples, tokens, heads
-    int heads, first;               // first: of the workgroups' parts (blockIdx.y)
+    int heads, first;               // first: of the workgroups' parts
 };
 struct HeadArgs {
     HeadTensor t[3];
     const int32_t *pos, *slot, *len;
-    int batch, tokens, dim, rope, near, cache, kinds;   // kinds: tensors there are, one after the other in t
+    int batch, tokens, dim, rope, near, cache;
+    int kinds, parts;                                   // tensors there are, one after the other in t; parts of a row
     int kind[3];                                        // which each is: 0 q, 1 k, 2 v
     float eps;
     uint64_t turn[kHeadMaxDim / 2];
@@ -78,7 +79,8 @@ __device__ __forceinline__ Row row_of(const HeadArgs& a, int64_t row) {
 // cos and sin of the row's angles for this lane's eight elements (with neighbours four pairs, else eight): each pair's by one lane of
 // the wave, exchanged through `tab`, this wave's place in LDS (kTab long: lanes whose elements are not turned read on)
 constexpr int kTab = kHeadMaxDim / 2 + 8;
-__device__ __forceinline__ void row_turns(const HeadArgs& a, const Row& r, int c, int lane, float2* tab, float2 (&w)[8]) {
+// The sines come with the sign of the lane's share: w[e] turns (y, partner's y) to y w.x + partner's w.y. back: the other way round.
+__device__ __forceinline__ void row_turns(const HeadArgs& a, const Row& r, int c, int lane, bool back, float2* tab, float2 (&w)[8]) {
     if (a.rope == 0) return;   // (uniform)
     const int pairs = a.rope >> 1;
     const int64_t pos = a.pos ? a.pos[r.row] : (int64_t)r.t;
@@ -89,7 +91,10 @@ __device__ __forceinline__ void row_turns(const HeadArgs& a, const Row& r, int c
     const int h = a.rope >> 4;   // lanes of half the turned elements
     const int at = 8 * c >= a.rope ? 0 : a.near ? 4 * c : 8 * (c < h ? c : c - h);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = tab[at + e];
+    for (int e = 0; e < 8; ++e) {
+        w[e] = tab[at + e];
+        w[e].y = back != (!a.near && c < h) ? -w[e].y : w[e].y;
+    }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();   // (the next row's angles come after these reads)
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -140,15 +145,15 @@ __device__ __forceinline__ float head_sum(float v) {
     return v;
 }
 
-// y's pairs turned by w (sign -1: back). Elements 8c .. 8c + 7 of the head; rope and its half are multiples of eight, so a
-// lane's elements are all turned or none, and the partners of (i, i + rope / 2) are one lane's.
-__device__ __forceinline__ void rotate(const HeadArgs& a, const float2 (&w)[8], int c, int lane, float sign, float (&y)[8]) {
+// y's pairs turned by w. Elements 8c .. 8c + 7 of the head; rope and its half are multiples of eight, so a lane's elements are all
+// turned or none, and the partners of (i, i + rope / 2) are one lane's.
+__device__ __forceinline__ void rotate(const HeadArgs& a, const float2 (&w)[8], int c, int lane, float (&y)[8]) {
     if (a.rope == 0) return;   // (uniform)
     const bool turned = 8 * c < a.rope;
     if (a.near) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-            const float p = y[e], q = y[e + 1], s = sign * w[e / 2].y;
+            const float p = y[e], q = y[e + 1], s = w[e / 2].y;
             y[e] = turned ? __builtin_fmaf(p, w[e / 2].x, -q * s) : p;
             y[e + 1] = turned ? __builtin_fmaf(q, w[e / 2].x, p * s) : q;
         }
@@ -157,11 +162,10 @@ __device__ __forceinline__ void rotate(const HeadArgs& a, const float2 (&w)[8], 
     const int h = a.rope >> 4;
     const bool first = c < h;
     const int from = !turned ? lane : first ? lane + h : lane - h;
-    const float sg = first ? -sign : sign;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float o = __shfl(y[e], from, 64);
-        y[e] = turned ? __builtin_fmaf(y[e], w[e].x, o * (sg * w[e].y)) : y[e];
+        y[e] = turned ? __builtin_fmaf(y[e], w[e].x, o * w[e].y) : y[e];
     }
 }
 
@@ -180,15 +184,21 @@ __device__ __forceinline__ void load_gain(const HeadArgs& a, const float* p, int
     }
 }
 
+__device__ __forceinline__ void clear(float (&v)[8], bool keep) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = keep ? v[e] : 0.f;
+}
+
 // A wave takes kGroups groups of heads of one row and tensor at the most, whose loads are all under way at once. A lane past the last
 // head, or past a head's elements, reads the last ones and stores nothing.
 template <class T, int LPH>
 __global__ __launch_bounds__(64 * kFwdWaves) void head_norm_fwd_kernel(HeadArgs a) {
     __shared__ float2 tabs[kFwdWaves][kTab];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane % LPH;
-    const int64_t row = (int64_t)blockIdx.x * kFwdWaves + wave;
+    const int part = (int)(blockIdx.x % (uint32_t)a.parts);
+    const int64_t row = (int64_t)(blockIdx.x / (uint32_t)a.parts) * kFwdWaves + wave;
     if (row >= (int64_t)a.batch * a.tokens) return;
-    const int part = blockIdx.y, ti = tensor_of(a, part), kind = a.kind[ti];
+    const int ti = tensor_of(a, part), kind = a.kind[ti];
     const HeadTensor& tn = a.t[ti];
     const Row r = row_of(a, row);
     if (!r.on) return;
@@ -203,10 +213,11 @@ __global__ __launch_bounds__(64 * kFwdWaves) void head_norm_fwd_kernel(HeadArgs 
     float gain[8];
     if (kind < 2) {   // (uniform)
         load_gain(a, tn.gain, c, gain);
-        row_turns(a, r, c, lane, tabs[wave], w);   // (while the loads are under way)
+        row_turns(a, r, c, lane, false, tabs[wave], w);   // (while the loads are under way)
     }
     if (!kept) return;   // (uniform)
     const float inv = 1.f / (float)a.dim;
+    const bool tail = a.dim < 8 * LPH;   // (uniform) lanes past a head's elements, which hold a copy of its last
     const int64_t to = r.b * tn.ys[0] + slot * tn.ys[1] + e0, yh = tn.ys[2];
 #pragma unroll
     for (int u = 0; u < kGroups; ++u) {
@@ -215,22 +226,20 @@ __global__ __launch_bounds__(64 * kFwdWaves) void head_norm_fwd_kernel(HeadArgs 
         if (kind < 2) {   // (uniform)
             float y[8], s = 0.f;
             x[u].get(y);
+            if (tail) clear(y, 8 * c < a.dim);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                y[e] = 8 * c < a.dim ? y[e] : 0.f;
-                s = __builtin_fmaf(y[e], y[e], s);
-            }
+            for (int e = 0; e < 8; ++e) s = __builtin_fmaf(y[e], y[e], s);
             const float rt = inverse_root<T>(__builtin_fmaf(head_sum<LPH>(s), inv, a.eps));
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] *= rt * gain[e];
-            rotate(a, w, c, lane, 1.f, y);
+            rotate(a, w, c, lane, y);
             x[u].set(y);
         }
         if (h < heads && 8 * c < a.dim) x[u].store(tn.y, to + h * yh);
     }
 }
 
-// part [gridDim.y][gridDim.x][dim]: each workgroup's sums of its gain's gradient (null: none)
+// part [parts][workgroups of a part][dim]: each workgroup's sums of its gain's gradient (null: none)
 template <class T, int LPH>
 __global__ __launch_bounds__(64 * kBwdWaves, 4) void head_norm_bwd_kernel(HeadArgs a, float* part) {
     __shared__ union {
@@ -239,14 +248,17 @@ __global__ __launch_bounds__(64 * kBwdWaves, 4) void head_norm_bwd_kernel(HeadAr
     } lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane % LPH;
     const int64_t rows = (int64_t)a.batch * a.tokens;
-    const HeadTensor& tn = a.t[tensor_of(a, blockIdx.y)];
-    const int h0 = ((int)blockIdx.y - tn.first) * kGroups * (64 / LPH) + lane / LPH, e0 = min(8 * c, a.dim - 8), heads = tn.heads;
+    const int mine = (int)(blockIdx.x % (uint32_t)a.parts), block = (int)(blockIdx.x / (uint32_t)a.parts);
+    const int blocks = (int)(gridDim.x / (uint32_t)a.parts);
+    const HeadTensor& tn = a.t[tensor_of(a, mine)];
+    const int h0 = (mine - tn.first) * kGroups * (64 / LPH) + lane / LPH, e0 = min(8 * c, a.dim - 8), heads = tn.heads;
     const float inv = 1.f / (float)a.dim;
+    const bool tail = a.dim < 8 * LPH;   // (uniform) lanes past a head's elements, which hold a copy of its last
     float gain[8], dg[8];
     load_gain(a, tn.gain, c, gain);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dg[e] = 0.f;
-    for (int64_t row = (int64_t)blockIdx.x * kBwdWaves + wave; row < rows; row += (int64_t)gridDim.x * kBwdWaves) {
+    for (int64_t row = (int64_t)block * kBwdWaves + wave; row < rows; row += (int64_t)blocks * kBwdWaves) {
         const Row r = row_of(a, row);
         if (!r.on) continue;   // (uniform)
         const int64_t xat = r.b * tn.xs[0] + r.t * tn.xs[1] + e0, dat = r.b * tn.dys[0] + r.t * tn.dys[1] + e0;
@@ -259,7 +271,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 4) void head_norm_bwd_kernel(HeadAr
             dy[u].load(tn.dy, dat + h * tn.dys[2]);
         }
         float2 w[8];
-        row_turns(a, r, c, lane, lds.tabs[wave], w);   // (while the loads are under way)
+        row_turns(a, r, c, lane, true, lds.tabs[wave], w);   // (while the loads are under way)
 #pragma unroll
         for (int u = 0; u < kGroups; ++u) {
             const int hd = h0 + u * (64 / LPH);
@@ -268,21 +280,20 @@ __global__ __launch_bounds__(64 * kBwdWaves, 4) void head_norm_bwd_kernel(HeadAr
             float d[8], xf[8], h[8], s = 0.f, t = 0.f;
             dy[u].get(d);
             x[u].get(xf);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                d[e] = on ? d[e] : 0.f;
-                xf[e] = on ? xf[e] : 0.f;
+            if (tail) {
+                clear(d, 8 * c < a.dim);
+                clear(xf, 8 * c < a.dim);
             }
-            rotate(a, w, c, lane, -1.f, d);
+            rotate(a, w, c, lane, d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 h[e] = d[e] * gain[e];
                 s = __builtin_fmaf(xf[e], xf[e], s);
                 t = __builtin_fmaf(h[e], xf[e], t);
             }
-            s = head_sum<LPH>(s);
-            const float rt = on ? inverse_root<T>(__builtin_fmaf(s, inv, a.eps)) : 0.f;
+            const float rt = inverse_root<T>(__builtin_fmaf(head_sum<LPH>(s), inv, a.eps));
             const float mean = head_sum<LPH>(t) * rt * inv;
+            if (hd - lane / LPH + 64 / LPH > heads) clear(d, on);   // (uniform) the group's last heads are a copy: of no gradient to the gain
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float xh = xf[e] * rt;
@@ -308,7 +319,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 4) void head_norm_bwd_kernel(HeadAr
         float v = 0.f;
 #pragma unroll
         for (int n = 0; n < kBwdWaves; ++n) v += lds.sums[n][i];
-        part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.dim + i] = v;
+        part[((int64_t)mine * blocks + block) * a.dim + i] = v;
     }
 }
 
@@ -347,6 +358,7 @@ HeadArgs head_args(const sa3k_head_norm& d, const HeadPtrs& p, bool bwd) {
         t.first = parts;
         parts += head_parts(t.heads, d.head_dim);
     }
+    a.parts = parts;
     a.pos = static_cast<const int32_t*>(p.pos);
     a.slot = static_cast<const int32_t*>(p.slot);
     a.len = static_cast<const int32_t*>(p.len);
@@ -366,22 +378,22 @@ void head_sums(sa3k_ctx* ctx, const HeadPtrs& p, const float* part, int nq, int 
 template <class T, int LPH>
 void head_launch(sa3k_ctx* ctx, const HeadArgs& a, const HeadPtrs& p, bool bwd) {
     const int64_t rows = (int64_t)a.batch * a.tokens;
-    int of[3] = {0, 0, 0}, parts = 0;   // parts of each
-    for (int i = 0; i < a.kinds; ++i) parts += of[a.kind[i]] = head_parts(a.t[i].heads, a.dim);
+    int of[3] = {0, 0, 0};   // parts of each
+    for (int i = 0; i < a.kinds; ++i) of[a.kind[i]] = head_parts(a.t[i].heads, a.dim);
     if (!bwd) {
         KernelScope ks(ctx, "head_norm_fwd");
-        launch_k(ctx, true, head_norm_fwd_kernel<T, LPH>, dim3((unsigned)ceil_div(rows, kFwdWaves), (unsigned)parts),
+        launch_k(ctx, true, head_norm_fwd_kernel<T, LPH>, dim3((unsigned)(ceil_div(rows, kFwdWaves) * a.parts)),
                  dim3(64 * kFwdWaves), 0, a);
         SA3K_LAUNCHED();
         return;
     }
     const bool sums = p.dq_gain || p.dk_gain;
-    const int64_t blocks = ceil_div(rows, kBwdWaves), most = sums ? std::max<int64_t>(1, kHeadBwdGroups / parts) : 1 << 20;
+    const int64_t blocks = ceil_div(rows, kBwdWaves), most = sums ? std::max<int64_t>(1, kHeadBwdGroups / a.parts) : 1 << 20;
     const int grid = (int)ceil_div(blocks, ceil_div(blocks, most));   // workgroups of the same number of rounds each
-    float* part = sums ? layer_workspace(ctx, (size_t)grid * parts * (size_t)a.dim * sizeof(float)) : nullptr;
+    float* part = sums ? layer_workspace(ctx, (size_t)grid * a.parts * (size_t)a.dim * sizeof(float)) : nullptr;
     {
         KernelScope ks(ctx, "head_norm_bwd");
-        launch_k(ctx, !sums, head_norm_bwd_kernel<T, LPH>, dim3((unsigned)grid, (unsigned)parts), dim3(64 * kBwdWaves), 0, a, part);
+        launch_k(ctx, !sums, head_norm_bwd_kernel<T, LPH>, dim3((unsigned)(grid * a.parts)), dim3(64 * kBwdWaves), 0, a, part);
         SA3K_LAUNCHED();
     }
     if (sums) head_sums(ctx, p, part, of[0] * grid, of[1] * grid, a.dim);
