@@ -1,5 +1,5 @@
-// Host-side arithmetic of the gated products: the checks of their arguments. No HIP in here: compiled with g++ in the CPU
-// tests too.
+// Host-side arithmetic of the gated products: their backward's plan and the checks of their arguments. No HIP in here: compiled
+// with g++ in the CPU tests too.
 #pragma once
 
 #include "layer_ops.h"
@@ -19,6 +19,51 @@ struct GatedArgs {
 
 // gate's and up's gradients lie side by side, each padded to whole tiles of 64
 inline int64_t gated_half(int64_t N) { return (N + 63) / 64 * 64; }
+
+// The backward products' plan: the other products', or one launch of 256 x 256 tiles for both, dX's workgroups first. Its time is
+// the last workgroup's end when 256 CUs take nx workgroups of tx microseconds and then nw of tw: after the last full round of dX's,
+// nx % 256 CUs start dW's a tx later than the rest. A tile of 64 along K counts 1.5 microseconds, a workgroup's start and stores 4,
+// the launch 5, and it is taken where that is 6% below the other plan's estimate: fitted to 79 shapes from 32 to 8192 rows, on which
+// the choice is 0.8% above the better of both on average and never more than 3% above the plan without it. dW's contraction, M, stays
+// whole: in two splits it lost on every shape tried. Measured on MI355X (M x K -> N, bf16, whole backward calls, us: the plan without
+// this launch / 256 x 256 tiles in dX's best split; * what this chooses): 2176 x 1536 -> 6144 212 / 194*, 4096 x 2048 -> 2048 155 /
+// 137*, 8192 x 1536 -> 6144 769 / 626*, 2048 x 2048 -> 8192 312 / 307*, 6000 x 4096 -> 6000 1189 / 1069*, 512 x 4096 -> 11008 280 /
+// 240*, 1600 x 4832 -> 712 66 / 58*, 4294 x 1384 -> 4632 310* / 284, 3000 x 1000 -> 3500 133* / 120, 1088 x 1536 -> 6144 113* / 116,
+// 815 x 1392 -> 2568 53* / 54, 700 x 1536 -> 6144 81* / 90, 1435 x 3320 -> 1192 74* / 84, 160 x 1920 -> 592 18* / 26.
+inline double gated_span(int64_t nx, double tx, int64_t nw, double tw) {
+    const int64_t late = nx % 256;
+    const double early_from = (double)(nx / 256) * tx, late_from = early_from + tx;
+    const double least = ((double)nx * tx + (double)nw * tw) / 256.0;   // no end is before the work shared evenly
+    double best = 1e300;
+    for (int side = 0; side < 2; ++side) {   // the last end lies whole workgroups of dW after one of both starts
+        const double from = side ? early_from : late_from;
+        for (int64_t k = least > from ? (int64_t)((least - from) / tw) : 0;; ++k) {
+            const double end = from + (double)k * tw;
+            if (late && end < late_from) continue;
+            const int64_t by_late = late ? (int64_t)((end - late_from) / tw + 1e-9) * late : 0;
+            if (by_late + (int64_t)((end - early_from) / tw + 1e-9) * (256 - late) < nw) continue;
+            if (end < best) best = end;
+            break;
+        }
+    }
+    return best;
+}
+inline ProdPair gated_pair(int64_t M, int64_t N, int64_t K) {
+    const int64_t cols = 2 * gated_half(N), kx = cols / 64, kw = (M + 63) / 64;
+    ProdPair best = prod_pair({M, K, cols}, {cols, K, M});
+    double least = 0.94 * (best.together ? best.a.us : best.a.us + best.b.us + 4.0);
+    const int64_t nk = (K + 255) / 256, nx = (M + 255) / 256 * nk, nw = (cols + 255) / 256 * nk;
+    const double tw = 1.5 * (double)kw + 4.0;
+    for (int64_t n = 1; n <= 8; ++n) {
+        if (!split_fits(n, kx, M, K)) continue;
+        const int64_t per = (kx + n - 1) / n;
+        const double t = gated_span(nx * n, 1.5 * (double)per + 4.0, nw, tw) + split_sum_us(n, M, K) + 5.0;
+        if (t >= least) continue;
+        least = t;
+        best = ProdPair{true, ProdPlan{256, (int)n, (int)per, t}, ProdPlan{256, 1, (int)kw, t}};
+    }
+    return best;
+}
 
 inline const char* gated_check(const GatedArgs& a, bool bwd, int* code) {
     *code = SA3K_ERR_INVALID;

@@ -480,12 +480,11 @@ struct FinishOf<T, kGatedForward, EDGE, NT, EROW> {
 // time): four waves of 128 x 128, 579 us against 530 (its epilogue stalls the only wave of a SIMD); fragments read a step
 // ahead, 519 against 512; steps of 32 of K, 527 against 512.
 template <class T, int P>
-__global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
+__device__ __forceinline__ void big_body(const GemmArgs& a, int L, char* lds) {
     typedef typename Vec<T>::x8 x8;
     constexpr int EDGE = 256, NT = 512, FM = 2, FN = 4, OPB = EDGE * 128, STAGE = 2 * OPB, EROW = EDGE + 8;
     static_assert(64 * EROW * 4 <= 2 * STAGE, "staged rows fit the stages' memory");
-    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
-    const TilePlace tp = tile_place<EDGE, Is<P>::gated_fwd ? EDGE / 2 : EDGE>(a, blockIdx.x);
+    const TilePlace tp = tile_place<EDGE, Is<P>::gated_fwd ? EDGE / 2 : EDGE>(a, L);
     if (tp.none) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm0 = (wave & 3) * 64, wn0 = (wave >> 2) * 128;
@@ -570,6 +569,20 @@ __global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
         fin.rows(a, tp.z, st, rb);
         __syncthreads();
     }
+}
+
+constexpr int kBigLds = 2 * 2 * 256 * 128;   // two stages of both operands
+template <class T, int P>
+__global__ __launch_bounds__(512, 2) void prod_big_kernel(GemmArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[kBigLds];
+    big_body<T, P>(a, blockIdx.x, lds);
+}
+// dX and dW in one launch of these tiles: the CUs that dX's last round leaves take dW's (gated_pair has the sizes and figures)
+template <class T, int PX, int PW>
+__global__ __launch_bounds__(512, 2) void prod_pair_big_kernel(GemmArgs x, GemmArgs w, int x_wgs) {
+    __shared__ __attribute__((aligned(1024))) char lds[kBigLds];
+    if ((int)blockIdx.x < x_wgs) big_body<T, PX>(x, blockIdx.x, lds);
+    else big_body<T, PW>(w, (int)blockIdx.x - x_wgs, lds);
 }
 
 // Tiles of 128 x 128: four waves of 64 x 64. STAGES 2: 64 KB of LDS, two workgroups a CU; STAGES 4: one. A wave keeps its MFMAs

@@ -1,13 +1,14 @@
 """The gated products' argument checks (csrc/gated.h) and the variants that their GPU tests' shapes take, which are host
 arithmetic: compiled with g++ and checked without a GPU."""
 import ctypes as C
+import heapq
 import os
 import subprocess
 
 import pytest
 
 from conftest import PKG, ROOT, sa3k
-from gated_shapes import BACKWARD, FORWARD
+from gated_shapes import BACKWARD, DW_ALONE, DX_ALONE, FORWARD
 
 INVALID, UNSUPPORTED = 1, 4
 P = ("X", "Wg", "Wu", "dY", "G", "U", "Y", "Go", "Uo", "dX", "dWg", "dWu", "bg", "bu", "dbg", "dbu")
@@ -24,6 +25,7 @@ def host(tmp_path_factory):
     lib = C.CDLL(out)
     lib.gated.argtypes = [C.c_int, C.c_int] + [C.POINTER(C.c_int64)] * 3 + [C.c_int] * 3
     lib.plans.argtypes = [C.c_int64] * 3 + [C.POINTER(C.c_int)]
+    lib.span.argtypes, lib.span.restype = [C.c_int64, C.c_double] * 2, C.c_double
     return lib
 
 
@@ -72,10 +74,26 @@ def test_backward_refuses(host, want, change):
 
 
 def test_shapes_take_their_variants(host):
-    o = (C.c_int * 7)()
+    o = (C.c_int * 11)()
     for (M, N, K), want in FORWARD.items():
         host.plans(M, N, K, o)
         assert (o[0], o[1] > 1) == want, (M, N, K, list(o))
     for (M, N, K), want in BACKWARD.items():
         host.plans(M, N, K, o)
         assert (bool(o[2]), o[3], o[4] > 1, o[5], o[6] > 1) == want, (M, N, K, list(o))
+    for shapes, at in ((DX_ALONE, 7), (DW_ALONE, 9)):
+        for (M, N, K), want in shapes.items():
+            host.plans(M, N, K, o)
+            assert (o[at], o[at + 1] > 1) == want, (M, N, K, list(o))
+
+
+@pytest.mark.parametrize("nx,tx,nw,tw", [(1, 5.0, 1, 3.0), (256, 5.0, 256, 3.0), (216, 76.0, 288, 55.0), (300, 10.0, 1, 100.0), (40, 100.0, 900, 7.0),
+                                         (1000, 3.5, 5, 2.25), (255, 1.0, 257, 1.0), (512, 9.0, 513, 8.0), (3, 1000.0, 20000, 1.0)])
+def test_span_is_the_greedy_schedules_end(host, nx, tx, nw, tw):
+    """256 CUs, each taking the next workgroup when it is done"""
+    free = [0.0] * 256
+    for job in [tx] * nx + [tw] * nw:
+        at = heapq.heappop(free)
+        heapq.heappush(free, at + job)
+    # the order of additions differs: relative 2^-53 for each of at most nx + nw of them
+    assert host.span(nx, tx, nw, tw) == pytest.approx(max(free), rel=2.0 ** -53 * 2 * (nx + nw))

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from conftest import sa3k
-from gated_shapes import BACKWARD, FORWARD
+from gated_shapes import BACKWARD, DW_ALONE, DX_ALONE, FORWARD
 from layer_ops_util import TORCH, TYPE, U32, Pitched, down, draw, half_step, up
 
 pytestmark = pytest.mark.gpu
@@ -74,13 +74,14 @@ def test_forward_on_every_tile(ctx, shape):
 
 
 def backward_case(ctx, kind, M, N, K, variant):
-    """variant 0: plain and aligned; 1: relu, odd pitches, f32 dW added to; 2: dX and one bias' gradient only; 3: the products only"""
+    """variant 0: plain and aligned; 1: relu, odd pitches, f32 dW added to; 2: dX and one bias' gradient only; 3: the products only;
+    4: dX only; 5: the weights' gradients only"""
     act = "relu" if variant == 1 else "none"
     x, w, dy = whole(1, (M, K), 2, kind), whole(2, (2 * N, K), 2, kind), whole(5, (M, N), 1, kind)
     g, u = whole(6, (M, N), 2, kind), whole(7, (M, N), 2, kind)
     f, s = (torch.relu(g.float()), (g > 0).float()) if variant == 1 else (g.float(), 1.0)
     dg, du = dy.float() * u.float() * s, dy.float() * f
-    odd, some, bare = variant == 1, variant == 2, variant == 3
+    odd, some, bare, no_dx = variant == 1, variant in (2, 4), variant in (3, 4, 5), variant == 5
     pad, off = ((1, 3, 2, 5, 1, 2), 1) if odd else ((0,) * 6, 0)
     ddy, dG, dU, dxx = (Pitched(ctx, t, t.shape[1] + p, off) for t, p in ((dy, pad[0]), (g, pad[1]), (u, pad[1]), (x, pad[2])))
     dw = [Pitched(ctx, t, K + pad[3], off) for t in (w[:N], w[N:])]
@@ -89,11 +90,15 @@ def backward_case(ctx, kind, M, N, K, variant):
     ox = Pitched(ctx, torch.zeros_like(x), K + pad[4], off)
     ow = [Pitched(ctx, t if odd else torch.zeros((N, K), dtype=TORCH[kind]), K + pad[5], off) for t in old]
     ob = [up(ctx, t) for t in oldb]
-    sa3k.gated_linear_bwd(ctx, TYPE[kind], ACTS[act], ddy, dG, dU, None if some else dxx, dw[0], dw[1], M, N, K, dx=ox,
+    sa3k.gated_linear_bwd(ctx, TYPE[kind], ACTS[act], ddy, dG, dU, None if some else dxx, None if no_dx else dw[0],
+                          None if no_dx else dw[1], M, N, K, dx=None if no_dx else ox,
                           dw_gate=None if some else ow[0], dw_up=None if some else ow[1], db_gate=None if some or bare else ob[0],
                           db_up=None if bare else ob[1], dw_type=TYPE["f32"] if odd else None, accumulate=odd, lddy=ddy.ld, ldz=dG.ld, ldx=dxx.ld,
                           ldw=dw[0].ld, lddx=ox.ld, lddw=ow[0].ld)
-    same(ox.get(), dg @ w[:N].float() + du @ w[N:].float())
+    if no_dx:
+        assert not bool(ox.get().any())
+    else:
+        same(ox.get(), dg @ w[:N].float() + du @ w[N:].float())
     for i, d in enumerate((dg, du)):
         if bare or (some and i == 0):
             assert np.array_equal(ob[i].numpy(), oldb[i].numpy())
@@ -122,6 +127,12 @@ def test_backward_of_many_rows(ctx):
 def test_backward_on_every_tile(ctx, shape):
     backward_case(ctx, "bf16", *shape, 0)
     backward_case(ctx, "f16", *shape, 1)
+
+
+@pytest.mark.parametrize("variant,shape", [(v, s) for v, d in ((4, DX_ALONE), (5, DW_ALONE)) for s in d])
+def test_backward_products_alone_on_every_tile(ctx, variant, shape):
+    backward_case(ctx, "bf16", *shape, variant)
+    backward_case(ctx, "f16", *shape, variant)
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
