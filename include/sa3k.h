@@ -575,7 +575,7 @@ SA3K_API int sa3k_head_norm_fwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const vo
  * turned back and h = w gain, r = 1 / sqrt(mean x^2 + eps),
  *   dx = r (h - x r mean(h x r)),  dgain = sum over tokens and heads of w x r
  * dq and dk lie as q and k do and may be dq_out and dk_out themselves (same strides). q and k (with their gradients) and the gains'
- * gradients (f32 [head_dim]) are each nullable; accumulate = 1 adds to the latter. Tokens past a sample's length are not read, add nothing,
+ * gradients (f32 [head_dim], two vectors) are each nullable; accumulate = 1 adds to the latter. Tokens past a sample's length are not read, add nothing,
  * and their gradients stay as they were. Sums run in a fixed order. */
 SA3K_API int sa3k_head_norm_bwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const void* q, const void* k, const void* dq_out,
                                 const void* dk_out, const float* q_gain, const float* k_gain, const int32_t* pos,
@@ -594,7 +594,7 @@ typedef struct sa3k_tensors sa3k_tensors;   /* a list of them, cut into pieces, 
 
 /* A list of `count` tensors (0: none). It keeps their addresses, not their memory, which has to outlive its calls. An output must not
  * meet another tensor's gradient or output, nor its own gradient but in place; gradients may repeat. Tensors need only be
- * aligned to their elements. It belongs to the context that made it. Synchronises the stream. */
+ * aligned to their elements. It belongs to the context that made it (calls on another are refused). Synchronises the stream. */
 SA3K_API int sa3k_tensors_create(sa3k_ctx* ctx, const sa3k_tensor* tensors, int64_t count, sa3k_tensors** out);
 SA3K_API int sa3k_tensors_destroy(sa3k_ctx* ctx, sa3k_tensors* t);
 /* Over all of them, as sa3k_average_and_clip does over an arena:

@@ -33,7 +33,8 @@ inline int64_t gated_half(int64_t N) { return (N + 63) / 64 * 64; }
 inline double gated_span(int64_t nx, double tx, int64_t nw, double tw) {
     const int64_t late = nx % 256;
     const double early_from = (double)(nx / 256) * tx, late_from = early_from + tx;
-    const double least = ((double)nx * tx + (double)nw * tw) / 256.0;   // no end is before the work shared evenly
+    // no end is before the work shared evenly, nor before the last of dX's
+    const double shared = ((double)nx * tx + (double)nw * tw) / 256.0, least = late && late_from > shared ? late_from : shared;
     double best = 1e300;
     for (int side = 0; side < 2; ++side) {   // the last end lies whole workgroups of dW after one of both starts
         const double from = side ? early_from : late_from;
@@ -63,6 +64,14 @@ inline ProdPair gated_pair(int64_t M, int64_t N, int64_t K) {
         best = ProdPair{true, ProdPlan{256, (int)n, (int)per, t}, ProdPlan{256, 1, (int)kw, t}};
     }
     return best;
+}
+
+// whether an element of x and one of y lie in the same place: rows of both `ld` apart
+inline bool rows_meet(const void* x, const void* y, int64_t ld, int64_t rows, int64_t cols, int bytes) {
+    if (!x || !y || rows <= 0) return false;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+    const int64_t d = (int64_t)((a > b ? a - b : b - a) / (uintptr_t)bytes), q = d / ld, r = d % ld;
+    return (q < rows && r < cols) || (q + 1 < rows && ld - r < cols);
 }
 
 inline const char* gated_check(const GatedArgs& a, bool bwd, int* code) {
@@ -95,6 +104,9 @@ inline const char* gated_check(const GatedArgs& a, bool bwd, int* code) {
         *code = SA3K_ERR_UNSUPPORTED;
         return "M x N is too large for one launch";
     }
+    if (rows_meet(a.Go, a.Uo, a.ldz, a.M, a.N, 2) || rows_meet(a.dWg, a.dWu, a.lddw, a.N, a.K, elem_bytes(a.dw_type)) ||
+        rows_meet(a.dbg, a.dbu, a.N, 1, a.N, 4))
+        return "gate's output meets up's";
     if (!bwd) {
         if (!a.Wg || !a.Wu) return "the weights must not be null";
         if (a.M > 0 && (!a.X || !a.Y)) return "X and Y must not be null";

@@ -74,6 +74,10 @@ inline const char* head_norm_check(const sa3k_head_norm* d, const HeadPtrs& p, b
     const void* f[7] = {p.q_gain, p.k_gain, p.pos, p.slot, p.len, p.dq_gain, p.dk_gain};
     for (const void* x : f)
         if (!elem_aligned(x, 4)) return "gains, positions, slots and lengths must be 4-byte aligned";
+    if (p.dq_gain && p.dk_gain) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p.dq_gain), b = reinterpret_cast<uintptr_t>(p.dk_gain);
+        if ((a > b ? a - b : b - a) < 4 * (uintptr_t)d->head_dim) return "the gains' gradients overlap";
+    }
     if (d->batch == 0 || d->tokens == 0) return nullptr;   // nothing is read or written but the gains' gradients
     const int eb = elem_bytes(d->type), D = d->head_dim;
     const int64_t nq[3] = {d->batch, d->tokens, d->heads}, nk[3] = {d->batch, d->tokens, d->kv_heads};
@@ -96,6 +100,7 @@ inline const char* head_norm_check(const sa3k_head_norm* d, const HeadPtrs& p, b
         {p.vo, d->v_out_stride, nc, true}, {p.dqo, d->q_out_stride, nq, false}, {p.dko, d->k_out_stride, nk, false}};
     for (const auto& x : t)
         if (x.p && (m = head_tensor_check(x.p, x.st, x.n, D, eb, x.out))) return m;
+    if ((p.qo && (p.qo == p.ko || p.qo == p.vo)) || (p.ko && p.ko == p.vo)) return "two outputs are the same tensor";
     if (!bwd && p.slot && ((p.ko && p.ko == p.k) || (p.vo && p.vo == p.v))) return "k and v cannot move within themselves";
     if (!same_place(bwd ? p.dqo : p.q, p.qo, bwd ? d->q_out_stride : d->q_stride, bwd ? d->q_stride : d->q_out_stride, nq) ||
         !same_place(bwd ? p.dko : p.k, p.ko, bwd ? d->k_out_stride : d->k_stride, bwd ? d->k_stride : d->k_out_stride, nk) ||

@@ -16,6 +16,7 @@
 #include "tensors.h"
 
 struct sa3k_tensors {
+    const sa3k_ctx* ctx = nullptr;   // that made it
     sa3k::TensorPiece* pieces = nullptr;
     double* partials = nullptr;   // [grid], then the norm and the factor of the last call
     int64_t n = 0;
@@ -181,6 +182,7 @@ SA3K_API int sa3k_tensors_create(sa3k_ctx* ctx, const sa3k_tensor* tensors, int6
         DeviceScope dev(ctx);
         const std::vector<TensorPiece> pieces = tensor_pieces(tensors, count);
         std::unique_ptr<sa3k_tensors, void (*)(sa3k_tensors*)> t(new sa3k_tensors(), tensors_free);
+        t->ctx = ctx;
         t->n = (int64_t)pieces.size();
         t->grid = (int)std::max<int64_t>(1, std::min<int64_t>(t->n, kMostGroups));
         SA3K_HIP(hipMalloc(&t->partials, sizeof(double) * (size_t)(t->grid + 2)));
@@ -198,6 +200,7 @@ SA3K_API int sa3k_tensors_create(sa3k_ctx* ctx, const sa3k_tensor* tensors, int6
 SA3K_API int sa3k_tensors_destroy(sa3k_ctx* ctx, sa3k_tensors* t) {
     return sa3k_guard(ctx, "sa3k_tensors_destroy", [&] {
         if (!t) return;
+        SA3K_REQUIRE(t->ctx == ctx, "the list belongs to another context");
         DeviceScope dev(ctx);
         SA3K_HIP(hipStreamSynchronize(ctx->stream));
         tensors_free(t);
@@ -207,6 +210,7 @@ SA3K_API int sa3k_tensors_destroy(sa3k_ctx* ctx, sa3k_tensors* t) {
 SA3K_API int sa3k_tensors_clip(sa3k_ctx* ctx, sa3k_tensors* t, int count, float max_norm, double* stat, double* norm_out) {
     return sa3k_guard(ctx, "sa3k_tensors_clip", [&] {
         SA3K_REQUIRE(t != nullptr, "null list");
+        SA3K_REQUIRE(t->ctx == ctx, "the list belongs to another context");
         int code;
         const char* msg = clip_check(count, max_norm, stat, &code);
         require_ok(msg, code);

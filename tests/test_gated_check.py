@@ -31,7 +31,7 @@ def host(tmp_path_factory):
 
 def check(host, bwd=False, type=sa3k.TYPE_BF16, act=2, M=4, N=24, K=16, dw_type=None, accumulate=0, ld=None, **p):
     at = dict(Wg=64, Wu=128, X=192)
-    at.update(dict(dY=256, G=320, U=384, dX=448, dWg=512, dWu=576) if bwd else dict(Y=256))
+    at.update(dict(dY=256, G=320, U=384, dX=448, dWg=512, dWu=8192) if bwd else dict(Y=256))
     at.update(p)
     lds = dict(x=K, w=K, dy=N, z=N, y=N, dx=K, dw=K)
     lds.update(ld or {})
@@ -41,13 +41,26 @@ def check(host, bwd=False, type=sa3k.TYPE_BF16, act=2, M=4, N=24, K=16, dw_type=
 
 def test_accepts(host):
     assert check(host) == 0 and check(host, bwd=True) == 0
-    assert check(host, Go=64, Uo=64, bg=64, bu=68) == 0 and check(host, Go=64) == 0
+    assert check(host, Go=64, Uo=8192, bg=64, bu=68) == 0 and check(host, Go=64) == 0
     assert check(host, X=194, ld=dict(x=17)) == 0
     assert check(host, M=0, X=0, Y=0) == 0 and check(host, bwd=True, M=0, X=0, dY=0, G=0, U=0) == 0
     assert check(host, bwd=True, dX=0, dWg=0, dWu=0, dbg=64) == 0 and check(host, bwd=True, dX=0, Wg=0, Wu=0) == 0
     assert check(host, bwd=True, dWg=0, dWu=0, X=0) == 0
     assert check(host, bwd=True, dw_type=sa3k.TYPE_F32, accumulate=1) == 0
     assert check(host, N=(1 << 21) - 64, K=1, M=1) == 0
+
+
+def test_gates_outputs_and_ups_lie_apart(host):
+    """N 24, K 16: rows that take turns in one tensor are apart, rows that share an element are not"""
+    f, b, f32 = dict(Go=1024), dict(bwd=True, dWg=1024), dict(bwd=True, dWg=1024, dw_type=sa3k.TYPE_F32)
+    for want, kw in ((INVALID, dict(f, Uo=1024)), (INVALID, dict(f, Uo=1024 + 2 * 95)), (0, dict(f, Uo=1024 + 2 * 96)),
+                     (0, dict(f, Uo=1024 + 2 * 24, ld=dict(z=48))), (INVALID, dict(f, Uo=1024 + 2 * 23, ld=dict(z=48))),
+                     (0, dict(f, Uo=1024 - 2 * 24, ld=dict(z=48))), (INVALID, dict(f, Uo=1024 - 2 * 25, ld=dict(z=48))),
+                     (INVALID, dict(b, dWu=1024)), (0, dict(b, dWu=1024 + 32, ld=dict(dw=32))), (0, dict(b, dWu=1024 + 768)),
+                     (INVALID, dict(b, dWu=1024 + 766)), (0, dict(f32, dWu=1024 + 1536)), (INVALID, dict(f32, dWu=1024 + 1532)),
+                     (INVALID, dict(b, dbg=64, dbu=64)), (INVALID, dict(b, dbg=64, dbu=64 + 92)), (0, dict(b, dbg=64, dbu=64 + 96))):
+        assert check(host, **kw) == want, kw
+    assert check(host, M=1, Go=1024, Uo=1024 + 48, ld=dict(z=30)) == 0
 
 
 @pytest.mark.parametrize("want,change", [

@@ -100,3 +100,15 @@ def test_two_contexts_in_turns(two):
                 assert np.array_equal(a.numpy(), b)
         for layer in layers:
             layer.done()
+
+
+def test_a_list_is_its_contexts_own(two):
+    a = two[0].zeros(64)
+    t = sa3k.Tensors(two[0], [(a.ptr, 64, TYPE["f32"], None, TYPE["f32"])])
+    t.ctx = two[1]
+    for call in (lambda: t.clip(1, 1.0), t.destroy):
+        with pytest.raises(sa3k.Sa3kError, match="another context"):
+            call()
+    t.ctx = two[0]
+    assert t.clip(1, 1.0, want_norm=True) == 0.0
+    t.destroy()

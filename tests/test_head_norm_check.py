@@ -89,6 +89,15 @@ def test_backward_refuses(host, want, change):
     assert check(host, bwd=True, **change) == want
 
 
+def test_outputs_are_each_their_own(host):
+    for kw in (dict(ko=1024), dict(v=64, vo=1024), dict(v=64, vo=2048), dict(bwd=True, ko=1024),
+               dict(bwd=True, dq_gain=4096, dk_gain=4096), dict(bwd=True, dq_gain=4096, dk_gain=4096 + 4 * 63),
+               dict(bwd=True, dq_gain=4096, dk_gain=4096 - 4 * 63)):
+        assert check(host, **kw) == INVALID, kw
+    assert check(host, bwd=True, dq_gain=4096, dk_gain=4096 + 4 * 64) == 0
+    assert check(host, q_gain=64, k_gain=64) == 0   # one gain for both
+
+
 def test_null_shape(host):
     assert host.head_norm_null() == INVALID
 
