@@ -20,21 +20,20 @@ struct GatedArgs {
 // gate's and up's gradients lie side by side, each padded to whole tiles of 64
 inline int64_t gated_half(int64_t N) { return (N + 63) / 64 * 64; }
 
-// The backward products' plan: the other products', or one launch of 256 x 256 tiles for both, dX's workgroups first. Its time is
-// the last workgroup's end when 256 CUs take nx workgroups of tx microseconds and then nw of tw: after the last full round of dX's,
-// nx % 256 CUs start dW's a tx later than the rest. A tile of 64 along K counts 1.5 microseconds, a workgroup's start and stores 4,
-// the launch 5, and it is taken where that is 6% below the other plan's estimate: fitted to 79 shapes from 32 to 8192 rows, on which
-// the choice is 0.8% above the better of both on average and never more than 3% above the plan without it. dW's contraction, M, stays
-// whole: in two splits it lost on every shape tried. Measured on MI355X (M x K -> N, bf16, whole backward calls, us: the plan without
-// this launch / 256 x 256 tiles in dX's best split; * what this chooses): 2176 x 1536 -> 6144 212 / 194*, 4096 x 2048 -> 2048 155 /
-// 137*, 8192 x 1536 -> 6144 769 / 626*, 2048 x 2048 -> 8192 312 / 307*, 6000 x 4096 -> 6000 1189 / 1069*, 512 x 4096 -> 11008 280 /
-// 240*, 1600 x 4832 -> 712 66 / 58*, 4294 x 1384 -> 4632 310* / 284, 3000 x 1000 -> 3500 133* / 120, 1088 x 1536 -> 6144 113* / 116,
-// 815 x 1392 -> 2568 53* / 54, 700 x 1536 -> 6144 81* / 90, 1435 x 3320 -> 1192 74* / 84, 160 x 1920 -> 592 18* / 26.
-inline double gated_span(int64_t nx, double tx, int64_t nw, double tw) {
-    const int64_t late = nx % 256;
-    const double early_from = (double)(nx / 256) * tx, late_from = early_from + tx;
+// The backward products' plan: one after the other, or both in one launch of 128 x 128 or 256 x 256 tiles, dX's workgroups first. A
+// launch ends with its last workgroup: each XCD takes every eighth; its 32 CUs hold 64 of the small tiles or 32 of the large, and
+// after the last full round of dX's, nx % slots of those start dW's later than the rest (pair_span). The times below are fitted to
+// whole calls on MI355X at 160 shapes of 16 to 40000 rows and at all their splits, 9% off them; the plan chosen is 1.6% above the
+// best of them on average and 13% at most (with the other products' plan, prod_pair, 6.8%). The large tiles' dW stays whole: in two
+// splits it lost on every shape tried. bf16, us (M x K -> N: prod_pair's plan / this one): 2176 x 1536 -> 6144 212 / 194 (256, dX in
+// four splits), 8192 x 1536 -> 6144 769 / 626 (256, whole), 4096 x 2048 -> 2048 155 / 137 (256, whole), 512 x 4096 -> 11008 280 / 260
+// (256, three), 1031 x 1001 -> 2731 63.5 / 55 (256, six), 1500 x 1024 -> 2048 60 / 47 (128, two), 2982 x 304 -> 1496 54 / 42 (128,
+// three and three), 784 x 760 -> 1848 32 (128, five, as before).
+inline double pair_span(int64_t nx, double tx, int64_t nw, double tw, int64_t slots) {
+    const int64_t late = nx % slots;
+    const double early_from = (double)(nx / slots) * tx, late_from = early_from + tx;
     // no end is before the work shared evenly, nor before the last of dX's
-    const double shared = ((double)nx * tx + (double)nw * tw) / 256.0, least = late && late_from > shared ? late_from : shared;
+    const double shared = ((double)nx * tx + (double)nw * tw) / (double)slots, least = late && late_from > shared ? late_from : shared;
     double best = 1e300;
     for (int side = 0; side < 2; ++side) {   // the last end lies whole workgroups of dW after one of both starts
         const double from = side ? early_from : late_from;
@@ -42,26 +41,54 @@ inline double gated_span(int64_t nx, double tx, int64_t nw, double tw) {
             const double end = from + (double)k * tw;
             if (late && end < late_from) continue;
             const int64_t by_late = late ? (int64_t)((end - late_from) / tw + 1e-9) * late : 0;
-            if (by_late + (int64_t)((end - early_from) / tw + 1e-9) * (256 - late) < nw) continue;
+            if (by_late + (int64_t)((end - early_from) / tw + 1e-9) * (slots - late) < nw) continue;
             if (end < best) best = end;
             break;
         }
     }
     return best;
 }
-inline ProdPair gated_pair(int64_t M, int64_t N, int64_t K) {
+// Microseconds of a workgroup with `per` tiles of 64 along K, of a launch that gives each XCD `wgs` workgroups; of the pass over
+// the split sums of M x N; and of a product in a launch of its own.
+inline double pair_wg_us(int edge, int64_t wgs, int64_t per) {
+    return edge == 256 ? 1.43 * (double)per + 7.4 : (wgs <= 32 ? 0.74 : 0.94) * (double)per + 3.7;
+}
+inline double pair_sum_us(int64_t n, int64_t M, int64_t N) { return n > 1 ? 8.0 * (double)n * (double)M * (double)N / 6.7e6 : 0.0; }
+inline int64_t xcd_tiles(int edge, int64_t M, int64_t N) { return ((M + edge - 1) / edge * ((N + edge - 1) / edge) + 7) / 8; }
+inline int64_t xcd_slots(int edge) { return edge == 256 ? 32 : 64; }
+constexpr double kPairSums = 4.6;   // a launch that adds splits up
+inline double alone_us(const ProdPlan& p, int64_t M, int64_t N) {
+    const int64_t n = xcd_tiles(p.edge, M, N) * p.splits, slots = xcd_slots(p.edge);
+    const double sums = p.splits > 1 ? pair_sum_us(p.splits, M, N) + kPairSums : 0.0;
+    return (double)((n + slots - 1) / slots) * pair_wg_us(p.edge, n, p.per) + sums;
+}
+inline ProdPair gated_pair(int64_t M, int64_t N, int64_t K, const ProdPlan& x, const ProdPlan& w) {
     const int64_t cols = 2 * gated_half(N), kx = cols / 64, kw = (M + 63) / 64;
-    ProdPair best = prod_pair({M, K, cols}, {cols, K, M});
-    double least = 0.94 * (best.together ? best.a.us : best.a.us + best.b.us + 4.0);
-    const int64_t nk = (K + 255) / 256, nx = (M + 255) / 256 * nk, nw = (cols + 255) / 256 * nk;
-    const double tw = 1.5 * (double)kw + 4.0;
-    for (int64_t n = 1; n <= 8; ++n) {
-        if (!split_fits(n, kx, M, K)) continue;
-        const int64_t per = (kx + n - 1) / n;
-        const double t = gated_span(nx * n, 1.5 * (double)per + 4.0, nw, tw) + split_sum_us(n, M, K) + 5.0;
-        if (t >= least) continue;
-        least = t;
-        best = ProdPair{true, ProdPlan{256, (int)n, (int)per, t}, ProdPlan{256, 1, (int)kw, t}};
+    ProdPair best{false, x, w};
+    double least = alone_us(x, M, K) + alone_us(w, cols, K) + 9.4;
+    constexpr int kMost = 8;     // splits
+    int64_t per[2][kMost + 1];   // tiles of 64 along K that a split of dX, of dW takes; 0: not one to try
+    double sums[2][kMost + 1];
+    for (int64_t n = 1; n <= kMost; ++n) {
+        per[0][n] = split_fits(n, kx, M, K) ? (kx + n - 1) / n : 0;
+        per[1][n] = split_fits(n, kw, cols, K) ? (kw + n - 1) / n : 0;
+        sums[0][n] = pair_sum_us(n, M, K);
+        sums[1][n] = pair_sum_us(n, cols, K);
+    }
+    for (int edge = 128; edge <= 256; edge *= 2) {
+        const int64_t slots = xcd_slots(edge), tiles_x = xcd_tiles(edge, M, K), tiles_w = xcd_tiles(edge, cols, K);
+        for (int n = 1; n <= kMost; ++n)
+            for (int m = 1; m <= (edge == 256 ? 1 : kMost); m += m < 4 ? 1 : 2) {
+                if (!per[0][n] || !per[1][m]) continue;
+                const int64_t nx = tiles_x * n, nw = tiles_w * m;
+                const double tx = pair_wg_us(edge, nx + nw, per[0][n]), tw = pair_wg_us(edge, nx + nw, per[1][m]);
+                const double rest = sums[0][n] + sums[1][m] + (n > 1 || m > 1 ? kPairSums : 0.0) + (edge == 256 ? 1.6 : 0.0);
+                if (((double)nx * tx + (double)nw * tw) / (double)slots + rest >= least) continue;   // no span is below that
+                const double t = pair_span(nx, tx, nw, tw, slots) + rest;
+                if (t >= least) continue;
+                least = t;
+                best = ProdPair{true, ProdPlan{edge, n, (int)per[0][n], t}, ProdPlan{edge, m, (int)per[1][m], t}};
+            }
     }
     return best;
 }

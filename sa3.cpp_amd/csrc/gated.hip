@@ -9,7 +9,7 @@
 // Bound by MFMA with the loads beside it (prod_dev.h), few rows by HBM. Measured on MI355X: 2176 x 1536 -> 6144 bf16 silu with g and u
 // stored 98 to 104 us (788 TFLOP/s; its 432 tiles fill 256 CUs to 84%), 8191 x 4096 -> 8192 f16 gelu_tanh 948 to 980 us (1122 to 1160
 // TFLOP/s), backward 2176 x 1536 -> 6144 199 us (27 the pass over dY, g and u; the rest both products and what is
-// left to add up), 1031 x 1001 -> 2731 f16 65.5 us. Forward plans are the products' own (prod_plan over 2 N columns), the fastest of
+// left to add up), 1031 x 1001 -> 2731 f16 59.5 us. Forward plans are the products' own (prod_plan over 2 N columns), the fastest of
 // 128 and 256 and 1 to 16 splits on ten of eleven shapes from 17 to 4096 rows.
 #include "gated.h"
 #include "prod_dev.h"
@@ -249,7 +249,7 @@ void bwd_run(sa3k_ctx* ctx, const GatedArgs& p) {
     const bool px = do_w && M > 0 && !loads16(p.X, p.ldx, K);
     const bool pw = do_x && (!loads16(p.Wg, p.ldw, K) || !loads16(p.Wu, p.ldw, K));
     ProdPair plan{false, prod_plan(M > 0 ? M : 1, K, 2 * half), prod_plan(2 * half, K, M > 0 ? M : 1)};
-    if (do_x && do_w) plan = gated_pair(M, N, K);
+    if (do_x && do_w) plan = gated_pair(M, N, K, plan.a, plan.b);
     const DzPlan dz = dz_plan(M, half, sums);
     Scratch s;
     const size_t oz = s.take(products ? (size_t)M * 2 * half * 2 : 0), ox = s.take(px ? (size_t)M * Kp * 2 : 0);

@@ -4,12 +4,15 @@
 FORWARD = {(417, 8435, 316): (256, False), (17, 82, 302): (128, False), (19, 80, 516): (128, True), (156, 8820, 3596): (256, True)}
 # backward, both products: (dX and dW in one launch, edge of dX's tiles, whether its contraction is split, the same of dW)
 BACKWARD = {
-    (421, 1503, 5364): (False, 128, False, 256, False), (131, 8117, 149): (False, 128, True, 128, False),
-    (142, 8768, 409): (False, 128, True, 256, False), (2728, 685, 5560): (False, 256, False, 128, False),
-    (7375, 144, 6594): (False, 256, False, 128, True), (1728, 745, 8765): (True, 256, False, 256, False),
-    (131, 3914, 8405): (True, 256, True, 256, False), (139, 141, 158): (True, 128, False, 128, False),
-    (858, 141, 132): (True, 128, False, 128, True), (158, 278, 130): (True, 128, True, 128, False),
-    (1310, 446, 132): (True, 128, True, 128, True),
+    (139, 141, 158): (True, 128, False, 128, False), (421, 1503, 5364): (True, 128, False, 128, False),
+    (16, 195, 16): (True, 128, True, 128, False), (142, 8768, 409): (True, 128, True, 128, False),
+    (644, 18, 16): (True, 128, False, 128, True), (7375, 144, 6594): (True, 128, False, 128, True),
+    (158, 278, 130): (True, 128, True, 128, True), (858, 141, 132): (True, 128, True, 128, True),
+    (1310, 446, 132): (True, 128, True, 128, True), (1728, 745, 8765): (True, 256, False, 256, False),
+    (131, 3914, 8405): (True, 256, True, 256, False), (131, 8117, 149): (False, 128, True, 128, False),
+    (9766, 16, 672): (False, 128, False, 128, True), (1775, 1098, 4583): (False, 128, False, 256, False),
+    (16, 11997, 276): (False, 128, True, 256, False), (2728, 685, 5560): (False, 256, False, 128, False),
+    (12111, 18, 1153): (False, 256, False, 128, True), (2321, 2250, 1695): (False, 256, True, 128, False),
 }
 # a backward product by itself: (edge of its tiles, whether its contraction is split)
 DX_ALONE = {(17, 267, 48): (128, True), (17, 16, 200): (128, False), (4609, 16, 1700): (256, False), (136, 3538, 8222): (256, True)}

@@ -25,7 +25,7 @@ def host(tmp_path_factory):
     lib = C.CDLL(out)
     lib.gated.argtypes = [C.c_int, C.c_int] + [C.POINTER(C.c_int64)] * 3 + [C.c_int] * 3
     lib.plans.argtypes = [C.c_int64] * 3 + [C.POINTER(C.c_int)]
-    lib.span.argtypes, lib.span.restype = [C.c_int64, C.c_double] * 2, C.c_double
+    lib.span.argtypes, lib.span.restype = [C.c_int64, C.c_double] * 2 + [C.c_int64], C.c_double
     return lib
 
 
@@ -100,13 +100,13 @@ def test_shapes_take_their_variants(host):
             assert (o[at], o[at + 1] > 1) == want, (M, N, K, list(o))
 
 
-@pytest.mark.parametrize("nx,tx,nw,tw", [(1, 5.0, 1, 3.0), (256, 5.0, 256, 3.0), (216, 76.0, 288, 55.0), (300, 10.0, 1, 100.0), (40, 100.0, 900, 7.0),
-                                         (1000, 3.5, 5, 2.25), (255, 1.0, 257, 1.0), (512, 9.0, 513, 8.0), (3, 1000.0, 20000, 1.0)])
-def test_span_is_the_greedy_schedules_end(host, nx, tx, nw, tw):
-    """256 CUs, each taking the next workgroup when it is done"""
-    free = [0.0] * 256
+@pytest.mark.parametrize("slots", [32, 64])
+@pytest.mark.parametrize("nx,tx,nw,tw", [(1, 5.0, 1, 3.0), (32, 5.0, 32, 3.0), (27, 76.0, 36, 55.0), (40, 10.0, 1, 100.0), (5, 100.0, 115, 7.0),
+                                         (125, 3.5, 5, 2.25), (63, 1.0, 65, 1.0), (64, 9.0, 65, 8.0), (3, 1000.0, 2500, 1.0), (7, 0.5, 64, 90.0)])
+def test_span_is_the_greedy_schedules_end(host, slots, nx, tx, nw, tw):
+    """each place takes the next workgroup when it is done"""
+    free = [0.0] * slots
     for job in [tx] * nx + [tw] * nw:
-        at = heapq.heappop(free)
-        heapq.heappush(free, at + job)
-    # the order of additions differs: relative 2^-53 for each of at most nx + nw of them
-    assert host.span(nx, tx, nw, tw) == pytest.approx(max(free), rel=2.0 ** -53 * 2 * (nx + nw))
+        heapq.heapreplace(free, free[0] + job)
+    # the additions' order differs: 2^-53 of the sum for each, and two more
+    assert host.span(nx, tx, nw, tw, slots) == pytest.approx(max(free), rel=2.0 ** -53 * (nx + nw + 2))
