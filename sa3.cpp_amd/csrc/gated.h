@@ -20,6 +20,32 @@ struct GatedArgs {
 // gate's and up's gradients lie side by side, each padded to whole tiles of 64
 inline int64_t gated_half(int64_t N) { return (N + 63) / 64 * 64; }
 
+// tiles of an M x N result that an XCD takes of a launch, and how many its 32 CUs hold at a time
+inline int64_t xcd_tiles(int edge, int64_t M, int64_t N) { return ((M + edge - 1) / edge * ((N + edge - 1) / edge) + 7) / 8; }
+inline int64_t xcd_slots(int edge) { return edge == 256 ? 32 : 64; }
+
+// The forward's plan: rounds of workgroups on an XCD, and the split sums. The times are fitted to whole calls on MI355X at 70 shapes of
+// 17 to 8191 rows, 128 and 256 wide tiles, 1 to 16 splits, 9% off them; the plan chosen is 0.3% above the best of them on average and
+// 4% at most (prod_plan 2.8% and 26%). bf16, us (M x K -> N: prod_plan's / this one's): 1836 x 384 -> 4433 45 / 35 (128 whole), 56 x
+// 3768 -> 1045 19.4 / 16.3 (128, six splits), 7083 x 4920 -> 2507 475 / 428 (256 whole), 17 x 1536 -> 6144 16.5 / 14.8 (128, two),
+// 2176 x 1536 -> 6144 104 (256 whole, as before).
+inline ProdPlan gated_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t kt = (K + 63) / 64;
+    ProdPlan best{128, 1, (int)kt, 1e300};
+    for (int edge = 256; edge >= 128; edge /= 2) {
+        const int64_t tiles = xcd_tiles(edge, M, 2 * N), slots = xcd_slots(edge);
+        for (int64_t n = 1; n <= 16; ++n) {
+            if (!split_fits(n, kt, M, 2 * N)) continue;
+            const int64_t per = (kt + n - 1) / n, wgs = tiles * n;
+            const double wg = edge == 256 ? 1.52 * (double)per + 14.4 : (wgs <= 32 ? 0.5 : 1.0) * (double)per + 5.8;
+            const double sums = n > 1 ? 2.0 + 0.3 * (double)n + 16.0 * (double)n * (double)M * (double)N / 3.5e6 : 0.0;
+            const double t = (double)((wgs + slots - 1) / slots) * wg + sums;
+            if (t < best.us) best = ProdPlan{edge, (int)n, (int)per, t};
+        }
+    }
+    return best;
+}
+
 // The backward products' plan: one after the other, or both in one launch of 128 x 128 or 256 x 256 tiles, dX's workgroups first. A
 // launch ends with its last workgroup: each XCD takes every eighth; its 32 CUs hold 64 of the small tiles or 32 of the large, and
 // after the last full round of dX's, nx % slots of those start dW's later than the rest (pair_span). The times below are fitted to
@@ -54,8 +80,6 @@ inline double pair_wg_us(int edge, int64_t wgs, int64_t per) {
     return edge == 256 ? 1.43 * (double)per + 7.4 : (wgs <= 32 ? 0.74 : 0.94) * (double)per + 3.7;
 }
 inline double pair_sum_us(int64_t n, int64_t M, int64_t N) { return n > 1 ? 8.0 * (double)n * (double)M * (double)N / 6.7e6 : 0.0; }
-inline int64_t xcd_tiles(int edge, int64_t M, int64_t N) { return ((M + edge - 1) / edge * ((N + edge - 1) / edge) + 7) / 8; }
-inline int64_t xcd_slots(int edge) { return edge == 256 ? 32 : 64; }
 constexpr double kPairSums = 4.6;   // a launch that adds splits up
 inline double alone_us(const ProdPlan& p, int64_t M, int64_t N) {
     const int64_t n = xcd_tiles(p.edge, M, N) * p.splits, slots = xcd_slots(p.edge);

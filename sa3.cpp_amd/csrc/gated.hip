@@ -9,8 +9,7 @@
 // Bound by MFMA with the loads beside it (prod_dev.h), few rows by HBM. Measured on MI355X: 2176 x 1536 -> 6144 bf16 silu with g and u
 // stored 98 to 104 us (788 TFLOP/s; its 432 tiles fill 256 CUs to 84%), 8191 x 4096 -> 8192 f16 gelu_tanh 948 to 980 us (1122 to 1160
 // TFLOP/s), backward 2176 x 1536 -> 6144 199 us (27 the pass over dY, g and u; the rest both products and what is
-// left to add up), 1031 x 1001 -> 2731 f16 59.5 us. Forward plans are the products' own (prod_plan over 2 N columns), the fastest of
-// 128 and 256 and 1 to 16 splits on ten of eleven shapes from 17 to 4096 rows.
+// left to add up), 1031 x 1001 -> 2731 f16 59.5 us. Plans: gated_plan, gated_pair.
 #include "gated.h"
 #include "prod_dev.h"
 
@@ -212,7 +211,7 @@ void fwd_run(sa3k_ctx* ctx, const GatedArgs& p) {
     }
     const bool padded = !loads16(p.X, p.ldx, p.K) || !loads16(p.Wg, p.ldw, p.K) || !loads16(p.Wu, p.ldw, p.K);
     const int64_t Kp = padded ? up8(p.K) : p.K;
-    const ProdPlan plan = prod_plan(p.M, 2 * p.N, Kp);
+    const ProdPlan plan = gated_plan(p.M, p.N, Kp);
     Scratch s;
     // (they share K: if one is padded, all are)
     const size_t ox = s.take(padded ? (size_t)p.M * Kp * 2 : 0), og = s.take(padded ? (size_t)p.N * Kp * 2 : 0);

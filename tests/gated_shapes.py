@@ -1,7 +1,10 @@
 """Shapes of gated products that take one certain variant; that they do is checked on the CPU, what it computes on the GPU."""
 
 # (M, N, K) forward: (edge of the tiles, whether K is split)
-FORWARD = {(417, 8435, 316): (256, False), (17, 82, 302): (128, False), (19, 80, 516): (128, True), (156, 8820, 3596): (256, True)}
+FORWARD = {
+    (417, 8435, 316): (128, False), (17, 82, 302): (128, False), (19, 80, 516): (128, True), (156, 8820, 3596): (128, False),
+    (513, 6628, 325): (256, False), (155, 8511, 4009): (256, True),
+}
 # backward, both products: (dX and dW in one launch, edge of dX's tiles, whether its contraction is split, the same of dW)
 BACKWARD = {
     (139, 141, 158): (True, 128, False, 128, False), (421, 1503, 5364): (True, 128, False, 128, False),
