@@ -15,21 +15,26 @@
 
 namespace {
 
-// Few rows (at most 16): 16 columns of the output a workgroup, whose eight waves split K in steps of 32 and read both weights
+// Few rows, RB blocks of 16: 16 columns of the output a workgroup, whose eight waves split K in steps of 32 and read both weights
 // straight from memory into the MFMA's registers (each element once); the waves' sums are joined in LDS. Bound by HBM and the
 // latency of a launch: 1 x 1536 -> 6144 bf16 9.0 us, 38 MB (4.2 TB/s).
-template <class T>
+template <class T, int RB>
 __global__ __launch_bounds__(512) void gated_few_kernel(GemmArgs a) {
     typedef typename Vec<T>::x8 x8;
-    constexpr int W = 8, U = 6;
-    __shared__ float red[2][W][16][17];
+    constexpr int W = 8, U = RB == 1 ? 6 : 4;
+    __shared__ float red[2][W][16 * RB][17];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15;
     const int64_t n0 = (int64_t)blockIdx.x * 16, wn = n0 + r;
     const int64_t steps = (a.K + 31) / 32;
     const T* gp = static_cast<const T*>(a.B) + min(wn, a.N - 1) * a.ldb;
     const T* up = static_cast<const T*>(a.B2) + min(wn, a.N - 1) * a.ldb;
-    const T* xp = static_cast<const T*>(a.A) + min((int64_t)r, a.M - 1) * a.lda;
-    f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    const T* xp[RB];
+    f32x4 acc[2][RB];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        xp[b] = static_cast<const T*>(a.A) + min((int64_t)(16 * b + r), a.M - 1) * a.lda;
+        acc[0][b] = acc[1][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     // eight of K at k, zeros past its end (rows and columns past theirs repeat the last one: never stored)
     auto ld = [&](const T* p, int64_t k) {
         x8 v;
@@ -43,31 +48,36 @@ __global__ __launch_bounds__(512) void gated_few_kernel(GemmArgs a) {
         return v;
     };
     for (int64_t s0 = wave; s0 < steps; s0 += W * U) {
-        x8 g[U], u[U], x[U];
+        x8 g[U], u[U], x[U][RB];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int64_t k = (s0 + i * W) * 32 + 8 * (lane >> 4);
             g[i] = ld(gp, k);
             u[i] = ld(up, k);
-            x[i] = ld(xp, k);
+#pragma unroll
+            for (int b = 0; b < RB; ++b) x[i][b] = ld(xp[b], k);
         }
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            if constexpr (__is_same(T, bf16)) {
-                acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(g[i], x[i], acc[0], 0, 0, 0);
-                acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u[i], x[i], acc[1], 0, 0, 0);
-            } else {
-                acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(g[i], x[i], acc[0], 0, 0, 0);
-                acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[i], x[i], acc[1], 0, 0, 0);
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                if constexpr (__is_same(T, bf16)) {
+                    acc[0][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(g[i], x[i][b], acc[0][b], 0, 0, 0);
+                    acc[1][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u[i], x[i][b], acc[1][b], 0, 0, 0);
+                } else {
+                    acc[0][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(g[i], x[i][b], acc[0][b], 0, 0, 0);
+                    acc[1][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u[i], x[i][b], acc[1][b], 0, 0, 0);
+                }
             }
-        }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) red[i][wave][r][4 * (lane >> 4) + v] = acc[i][v];
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) red[i][wave][16 * b + r][4 * (lane >> 4) + v] = acc[i][b][v];
     __syncthreads();
-    if (tid >= 256) return;
+    if (tid >= 256 * RB) return;
     const int64_t m = tid >> 4, n = n0 + (tid & 15);
     if (m >= a.M || n >= a.N) return;
     float g[1] = {0.f}, u = 0.f;
@@ -203,9 +213,10 @@ void fwd_run(sa3k_ctx* ctx, const GatedArgs& p) {
     a.A = p.X; a.lda = p.ldx; a.B = p.Wg; a.B2 = p.Wu; a.ldb = p.ldw;
     a.M = p.M; a.N = p.N; a.K = p.K;
     a.C = p.Y; a.ldc = p.ldy; a.act = p.act; a.bias = p.bg; a.bias2 = p.bu; a.Z = p.Go; a.Z2 = p.Uo; a.ldz = p.ldz;
-    if (p.M <= kFewRows) {
+    if (const int blocks = few_blocks(p.M, p.N, p.K)) {
         KernelScope ks(ctx, "gated_linear_few", 4.0 * (double)a.M * (double)a.N * (double)a.K);
-        launch_k(ctx, true, gated_few_kernel<T>, dim3((unsigned)ceil_div(a.N, 16)), dim3(512), 0, a);
+        launch_k(ctx, true, blocks == 1 ? gated_few_kernel<T, 1> : gated_few_kernel<T, 2>, dim3((unsigned)ceil_div(a.N, 16)), dim3(512), 0,
+                 a);
         SA3K_LAUNCHED();
         return;
     }

@@ -1,9 +1,11 @@
 """Shapes of gated products that take one certain variant; that they do is checked on the CPU, what it computes on the GPU."""
 
-# (M, N, K) forward: (edge of the tiles, whether K is split)
+# (M, N, K) forward: (edge of the tiles, or blocks of few rows; whether K is split)
 FORWARD = {
-    (417, 8435, 316): (128, False), (17, 82, 302): (128, False), (19, 80, 516): (128, True), (156, 8820, 3596): (128, False),
-    (513, 6628, 325): (256, False), (155, 8511, 4009): (256, True),
+    (417, 8435, 316): (128, False), (33, 82, 302): (128, False), (35, 80, 516): (128, True), (156, 8820, 3596): (128, False),
+    (513, 6628, 325): (256, False), (155, 8511, 4009): (256, True), (17, 82, 302): (2, False), (19, 80, 516): (2, False),
+    (32, 8192, 40): (2, False), (31, 8193, 40): (128, False), (32, 40, 1024): (2, False), (17, 40, 1025): (128, True),
+    (16, 33, 2000): (1, False),
 }
 # backward, both products: (dX and dW in one launch, edge of dX's tiles, whether its contraction is split, the same of dW)
 BACKWARD = {

@@ -19,12 +19,13 @@ int gated(int type, int act, const int64_t* mnk, const int64_t* p, const int64_t
     int code = -1;
     return gated_check(a, bwd != 0, &code) ? code : 0;
 }
-// forward: edge, splits; both of the backward's products: together, edge and splits of dX, of dW; dX alone: edge, splits; dW alone
+// forward: edge (of few rows: their blocks), splits; both of the backward's products: together, edge and splits of dX, of dW; dX alone: edge, splits; dW alone
 void plans(int64_t M, int64_t N, int64_t K, int* out) {
     const int64_t h = 2 * gated_half(N), Kp = (K + 7) / 8 * 8;
     const ProdPlan f = gated_plan(M, N, Kp), x = prod_plan(M, K, h), w = prod_plan(h, K, M);
     const ProdPair p = gated_pair(M, N, K, x, w);
-    out[0] = f.edge; out[1] = f.splits;
+    const int few = few_blocks(M, N, K);
+    out[0] = few ? few : f.edge; out[1] = few ? 1 : f.splits;
     out[2] = p.together; out[3] = p.a.edge; out[4] = p.a.splits; out[5] = p.b.edge; out[6] = p.b.splits;
     out[7] = x.edge; out[8] = x.splits; out[9] = w.edge; out[10] = w.splits;
 }
