@@ -32,11 +32,10 @@ inline int few_blocks(int64_t M, int64_t N, int64_t K) {
 inline int64_t xcd_tiles(int edge, int64_t M, int64_t N) { return ((M + edge - 1) / edge * ((N + edge - 1) / edge) + 7) / 8; }
 inline int64_t xcd_slots(int edge) { return edge == 256 ? 32 : 64; }
 
-// The forward's plan: rounds of workgroups on an XCD, and the split sums. The times are fitted to whole calls on MI355X at 70 shapes of
-// 17 to 8191 rows, 128 and 256 wide tiles, 1 to 16 splits, 9% off them; the plan chosen is 0.3% above the best of them on average and
-// 4% at most (prod_plan 2.8% and 26%). bf16, us (M x K -> N: prod_plan's / this one's): 1836 x 384 -> 4433 45 / 35 (128 whole), 56 x
-// 3768 -> 1045 19.4 / 16.3 (128, six splits), 7083 x 4920 -> 2507 475 / 428 (256 whole), 17 x 1536 -> 6144 16.5 / 14.8 (128, two),
-// 2176 x 1536 -> 6144 104 (256 whole, as before).
+// The forward's plan: rounds of workgroups on an XCD, and the split sums. The times are fitted to whole calls on MI355X at 136 shapes of
+// 17 to 8191 rows, 128 and 256 wide tiles, 1 to 16 splits, 9% off them; the plan chosen is 0.6% above the best of them on average and
+// 11% at most (prod_plan 2.8% and 26%). bf16, us (M x K -> N: prod_plan's / this one's): 1836 x 384 -> 4433 45 / 34 (128 whole), 56 x
+// 3768 -> 1045 19.4 / 16.3 (128, six splits), 17 x 1536 -> 6144 16.5 / 14.8 (128, two).
 inline ProdPlan gated_plan(int64_t M, int64_t N, int64_t K) {
     const int64_t kt = (K + 63) / 64;
     ProdPlan best{128, 1, (int)kt, 1e300};
@@ -45,8 +44,8 @@ inline ProdPlan gated_plan(int64_t M, int64_t N, int64_t K) {
         for (int64_t n = 1; n <= 16; ++n) {
             if (!split_fits(n, kt, M, 2 * N)) continue;
             const int64_t per = (kt + n - 1) / n, wgs = tiles * n;
-            const double wg = edge == 256 ? 1.52 * (double)per + 14.4 : (wgs <= 32 ? 0.5 : 1.0) * (double)per + 5.8;
-            const double sums = n > 1 ? 2.0 + 0.3 * (double)n + 16.0 * (double)n * (double)M * (double)N / 3.5e6 : 0.0;
+            const double wg = edge == 256 ? 1.6 * (double)per + 8.1 : (wgs <= 32 ? 0.44 : 0.98) * (double)per + 5.8;
+            const double sums = n > 1 ? 0.6 + 0.3 * (double)n + 16.0 * (double)n * (double)M * (double)N / 4.5e6 : 0.0;
             const double t = (double)((wgs + slots - 1) / slots) * wg + sums;
             if (t < best.us) best = ProdPlan{edge, (int)n, (int)per, t};
         }

@@ -384,7 +384,7 @@ struct Finish {
     float b[8];
     Pack<T, 8> res[ROUNDS];
 
-    __device__ __forceinline__ void init(const GemmArgs& a, const TilePlace& tp, int tid) {
+    __device__ __forceinline__ void init(const GemmArgs& a, const TilePlace& tp, int tid, bool) {
         cq = (tid % CPR) * 8;
         r0 = tid / CPR;
         m0 = tp.m0;
@@ -429,15 +429,16 @@ struct FinishGated {
     int r0, cq;
     float bg[8], bu[8];
 
-    __device__ __forceinline__ void init(const GemmArgs& a, const TilePlace& tp, int tid) {
+    // added: the sums hold the biases
+    __device__ __forceinline__ void init(const GemmArgs& a, const TilePlace& tp, int tid, bool added) {
         const int c = (tid % CPR) * 8;
         cq = (c / WC) * 2 * WC + c % WC;
         r0 = tid / CPR;
         m0 = tp.m0;
         n = tp.n0 + c;
         if (a.part) return;
-        bias8(a, a.bias, n, bg);
-        bias8(a, a.bias2, n, bu);
+        bias8(a, added ? nullptr : a.bias, n, bg);
+        bias8(a, added ? nullptr : a.bias2, n, bu);
     }
     __device__ __forceinline__ void fetch(const GemmArgs&, int) {}
     __device__ __forceinline__ void rows(const GemmArgs& a, int z, const float* st, int rb) {
@@ -464,6 +465,139 @@ struct FinishGated {
         }
     }
 };
+// The end of a wave of a gated forward's 256 x 256 tile, 64 rows x 64 columns of both products, without LDS and without waiting for other
+// waves: the products were made with the weights' fragments first, so a lane holds 16 sums of one row of a block of 32 x 32 (column
+// 8 (v / 4) + 4 (lane / 32) + v % 4), gate's and up's of the same element. Lanes 32 apart swap their fours for eights (16 bits), lanes 16
+// apart halves of their rows, so that a store takes 64 bytes of 16 rows. Measured on MI355X (us, staged through LDS as the other
+// products' / so): 2176 x 1536 -> 6144 bf16 92 / 82, with g and u stored 94 / 89, 8191 x 4096 -> 8192 f16 957 / 922; rows that begin off 16
+// bytes stay staged (1952 x 320 -> 2239 25 / 35). The backward's products gained nothing (2176 x 1536 -> 6144 both 197).
+template <int A, int B>
+__device__ __forceinline__ void swap_lanes(uint32_t (&w)[16], int n, int by) {
+#pragma unroll
+    for (int e = 0; e < n; ++e) {
+        const auto r = by == 32 ? __builtin_amdgcn_permlane32_swap(w[A + e], w[B + e], false, false)
+                                : __builtin_amdgcn_permlane16_swap(w[A + e], w[B + e], false, false);
+        w[A + e] = r[0];
+        w[B + e] = r[1];
+    }
+}
+// a block of 32 x 32 at (m, n) of C [rows][cols]: rounded to T
+template <class T>
+__device__ __forceinline__ void store_block(void* C, int64_t ld, int64_t m, int64_t n, int64_t rows, int64_t cols, int lane,
+                                            const float (&v)[16]) {
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const Pack<T, 2> q{{(T)v[2 * e], (T)v[2 * e + 1]}};
+        w[e] = __builtin_bit_cast(uint32_t, q);
+    }
+    swap_lanes<0, 2>(w, 2, 32);   // 0 .. 3: eight columns, the lower lanes' from 0 on, the upper's from 8 on
+    swap_lanes<4, 6>(w, 2, 32);   // 4 .. 7: the same from 16 on
+    swap_lanes<0, 4>(w, 4, 16);   // 0 .. 3: of rows 0 .. 15; 4 .. 7: of rows 16 .. 31
+    n += 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int64_t row = m + 16 * h + (lane & 15);
+        if (row >= rows) continue;
+        const Pack<T, 8> q = __builtin_bit_cast(Pack<T, 8>, u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]});
+        T* c = static_cast<T*>(C) + row * ld;
+        if (n + 8 <= cols) {
+            *reinterpret_cast<Pack<T, 8>*>(c + n) = q;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < cols) c[n + e] = q.v[e];
+        }
+    }
+}
+// the same in f32, whole fours of columns
+__device__ __forceinline__ void store_block_f32(float* C, int64_t ld, int64_t m, int64_t n, int64_t rows, int64_t cols, int lane,
+                                                const float (&v)[16]) {
+    uint32_t w[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(v[e]);
+    swap_lanes<0, 4>(w, 4, 16);    // 0 .. 3: sixteen columns of rows 0 .. 15; 4 .. 7: of rows 16 .. 31
+    swap_lanes<8, 12>(w, 4, 16);   // 8 ..: the same from 16 on
+    n += 8 * ((lane >> 4) & 1) + 4 * (lane >> 5);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int64_t row = m + 16 * (q & 1) + (lane & 15), at = n + 16 * (q >> 1);
+        if (row < rows && at < cols)
+            *reinterpret_cast<uint4*>(C + row * ld + at) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    }
+}
+__device__ __forceinline__ void block_of(const f32x16& acc, float (&v)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = acc[e];
+}
+// whether the outputs' rows begin on 16 bytes: those of others lie across lines, whose stores of 64 bytes are then two each
+template <class T>
+__device__ __forceinline__ bool rows_whole(const GemmArgs& a) {
+    const uint64_t at = reinterpret_cast<uint64_t>(a.C) | reinterpret_cast<uint64_t>(a.Z) | reinterpret_cast<uint64_t>(a.Z2);
+    return ((at | (uint64_t)(a.ldc * (int64_t)sizeof(T)) | (a.Z || a.Z2 ? (uint64_t)(a.ldz * (int64_t)sizeof(T)) : 0)) & 15) == 0;
+}
+// The sums begin with the biases, whose loads are then under way beside the first tile's (read at the end, 2176 x 1536 -> 6144 took
+// 2 us more)
+__device__ __forceinline__ void gated_biases(const GemmArgs& a, int64_t n0, int lane, f32x16 (&acc)[2][4]) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const float* bias = w ? a.bias2 : a.bias;
+        if (!bias) continue;   // (uniform)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t c = n0 + 32 * j + 8 * q + 4 * (lane >> 5);
+                Pack<float, 4> b;
+                if (c + 4 <= a.N) {
+                    b = *reinterpret_cast<const Pack<float, 4>*>(bias + c);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) b.v[e] = c + e < a.N ? bias[c + e] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[0][2 * w + j][4 * q + e] += b.v[e];
+                    acc[1][2 * w + j][4 * q + e] += b.v[e];
+                }
+            }
+    }
+}
+template <class T>
+__device__ __forceinline__ void finish_gated_wave(const GemmArgs& a, int z, int64_t m0, int64_t n0, int lane, f32x16 (&acc)[2][4]) {
+    float v[16];
+    if (a.part) {   // (uniform) rows of the splits' sums: gate's, then up's, each of whole eights
+        const int64_t up = a.pitch / 2;
+        float* s = a.part + (int64_t)z * a.M * a.pitch;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                block_of(acc[i][j], v);
+                store_block_f32(s + (j >> 1) * up, a.pitch, m0 + 32 * i, n0 + 32 * (j & 1), a.M, up, lane, v);
+            }
+        return;
+    }
+    // One output after the other: with the three in turn for every 16 columns, 8192 x 1536 -> 6144 with g and u took 428 us, not 301.
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {
+            void* C = w == 0 ? a.Z : w == 1 ? a.Z2 : a.C;
+            if (!C) continue;   // (uniform)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                block_of(acc[i][w == 1 ? j + 2 : j], v);
+                if (w == 2) {
+                    act_values(v, a.act);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] *= acc[i][j + 2][e];
+                }
+                store_block<T>(C, w == 2 ? a.ldc : a.ldz, m0 + 32 * i, n0 + 32 * j, a.M, a.N, lane, v);
+            }
+        }
+}
+
 template <class T, int P, int EDGE, int NT, int EROW>
 struct FinishOf {
     typedef Finish<T, P, EDGE, NT, EROW> type;
@@ -513,6 +647,9 @@ __device__ __forceinline__ void big_body(const GemmArgs& a, int L, char* lds) {
     // the last step's first barrier, which comes before either group's first read of t + 1.
     const bool late = wave >= 4;
     if (t0 < t1) issue(0, t0);
+    if constexpr (Is<P>::gated_fwd) {
+        if (!a.part) gated_biases(a, tp.n0 + wn0 / 2, lane, acc);
+    }
     wait_vmcnt<0>();
     asm volatile("s_barrier" ::: "memory");
     if (late) asm volatile("s_barrier" ::: "memory");
@@ -539,7 +676,8 @@ __device__ __forceinline__ void big_body(const GemmArgs& a, int L, char* lds) {
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = Vec<T>::mfma(af[i], bf[j], acc[i][j]);
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] = Is<P>::gated_fwd ? Vec<T>::mfma(bf[j], af[i], acc[i][j]) : Vec<T>::mfma(af[i], bf[j], acc[i][j]);
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_barrier" ::: "memory");
@@ -548,9 +686,15 @@ __device__ __forceinline__ void big_body(const GemmArgs& a, int L, char* lds) {
     if (!late) asm volatile("s_barrier" ::: "memory");
 #pragma unroll
     for (int i = 0; i < FM; ++i) wattn::settle(acc[i]);
+    if constexpr (Is<P>::gated_fwd) {
+        if (a.part || rows_whole<T>(a)) {   // (uniform)
+            finish_gated_wave<T>(a, tp.z, tp.m0 + wm0, tp.n0 + wn0 / 2, lane, acc);
+            return;
+        }
+    }
     float* st = reinterpret_cast<float*>(lds);
     typename FinishOf<T, P, EDGE, NT, EROW>::type fin;
-    fin.init(a, tp, tid);
+    fin.init(a, tp, tid, true);
     __syncthreads();
 #pragma unroll 1
     for (int rb = 0; rb < EDGE; rb += 64) {
@@ -561,9 +705,10 @@ __device__ __forceinline__ void big_body(const GemmArgs& a, int L, char* lds) {
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        st[(32 * i + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3)) * EROW + wn0 + 32 * j + (lane & 31)] =
-                            acc[i][j][v];
+                    for (int v = 0; v < 16; ++v) {
+                        const int b = 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3), c = lane & 31;   // of A's block and of B's
+                        st[(32 * i + (Is<P>::gated_fwd ? c : b)) * EROW + wn0 + 32 * j + (Is<P>::gated_fwd ? b : c)] = acc[i][j][v];
+                    }
         }
         __syncthreads();
         fin.rows(a, tp.z, st, rb);
@@ -679,7 +824,7 @@ __device__ __forceinline__ void tile_body(const GemmArgs& a, int L, char* lds) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     float* st = reinterpret_cast<float*>(lds);
     typename FinishOf<T, P, EDGE, NT, EROW>::type fin;
-    fin.init(a, tp, tid);
+    fin.init(a, tp, tid, false);
     __syncthreads();
 #pragma unroll 1
     for (int rb = 0; rb < EDGE; rb += 64) {

@@ -2,8 +2,8 @@
 
 # (M, N, K) forward: (edge of the tiles, or blocks of few rows; whether K is split)
 FORWARD = {
-    (417, 8435, 316): (128, False), (33, 82, 302): (128, False), (35, 80, 516): (128, True), (156, 8820, 3596): (128, False),
-    (513, 6628, 325): (256, False), (155, 8511, 4009): (256, True), (17, 82, 302): (2, False), (19, 80, 516): (2, False),
+    (417, 8435, 316): (256, False), (33, 82, 302): (128, False), (35, 80, 516): (128, True), (156, 8820, 3596): (256, True),
+    (513, 6632, 325): (256, False), (155, 8511, 4009): (256, True), (396, 9688, 16): (256, False), (300, 520, 1000): (128, True), (17, 82, 302): (2, False), (19, 80, 516): (2, False),
     (32, 8192, 40): (2, False), (31, 8193, 40): (128, False), (32, 40, 1024): (2, False), (17, 40, 1025): (128, True),
     (16, 33, 2000): (1, False),
 }

@@ -32,13 +32,14 @@ def same(got, want):
 
 
 def forward_case(ctx, kind, M, N, K, variant):
-    """variant 0: plain and aligned; 1: everything, odd pitches, relu; 2: the weights as one tensor's halves, only u kept"""
+    """variant 0: plain and aligned; 1: everything, odd pitches, relu; 2: the weights as one tensor's halves, only u kept; 3: as 1
+    with even pitches"""
     x = whole(1, (M, K), 2, kind)
     w = whole(2, (2 * N, K), 1 if K > 1500 else 2, kind)
-    odd = variant == 1
-    b = [whole(3 + i, (N,), 9) if odd else None for i in range(2)]
-    g, u = (x.float() @ t.float().t() + (c if odd else 0) for t, c in zip((w[:N], w[N:]), b))
-    act = "relu" if odd else "none"
+    odd, full = variant == 1, variant in (1, 3)
+    b = [whole(3 + i, (N,), 9) if full else None for i in range(2)]
+    g, u = (x.float() @ t.float().t() + (c if full else 0) for t, c in zip((w[:N], w[N:]), b))
+    act = "relu" if full else "none"
     want = F64[act](g) * u
     pad, off = ((1, 3, 2, 5), 1) if odd else ((0,) * 4, 0)
     dx = Pitched(ctx, x, K + pad[0], off)
@@ -52,11 +53,11 @@ def forward_case(ctx, kind, M, N, K, variant):
         dw = [Pitched(ctx, t, K + pad[1], off + 2 * i * odd) for i, t in enumerate((w[:N], w[N:]))]
     dy = Pitched(ctx, torch.zeros((M, N), dtype=TORCH[kind]), N + pad[2], off)
     kept = [Pitched(ctx, torch.zeros((M, N), dtype=TORCH[kind]), N + pad[3], off) for _ in range(2)]
-    sa3k.gated_linear_fwd(ctx, TYPE[kind], ACTS[act], dx, dw[0], dw[1], M, N, K, dy, gate_bias=up(ctx, b[0]) if odd else None,
-                          up_bias=up(ctx, b[1]) if odd else None, gate=kept[0] if odd else None, up=kept[1] if variant else None,
+    sa3k.gated_linear_fwd(ctx, TYPE[kind], ACTS[act], dx, dw[0], dw[1], M, N, K, dy, gate_bias=up(ctx, b[0]) if full else None,
+                          up_bias=up(ctx, b[1]) if full else None, gate=kept[0] if full else None, up=kept[1] if variant else None,
                           ldx=dx.ld, ldw=K + pad[1], ldy=dy.ld, ldz=kept[0].ld)
     same(dy.get(), want)
-    same(kept[0].get(), g if odd else g * 0)
+    same(kept[0].get(), g if full else g * 0)
     same(kept[1].get(), u if variant else u * 0)
 
 
@@ -69,8 +70,9 @@ def test_forward_is_exact_on_whole_numbers(ctx, kind, M, N, K):
 
 @pytest.mark.parametrize("shape", list(FORWARD), ids=lambda s: "x".join(map(str, s)))
 def test_forward_on_every_tile(ctx, shape):
-    for variant in (0, 1):
+    for variant in (0, 1, 2, 3):
         forward_case(ctx, "bf16", *shape, variant)
+    forward_case(ctx, "f16", *shape, 3)
 
 
 def backward_case(ctx, kind, M, N, K, variant):
