@@ -7,9 +7,9 @@
 // columns, then up's), and so are the weights' gradients (rows of gate's, then of up's).
 //
 // Bound by MFMA with the loads beside it (prod_dev.h), few rows by HBM. Measured on MI355X: 2176 x 1536 -> 6144 bf16 silu with g and u
-// stored 98 to 104 us (788 TFLOP/s; its 432 tiles fill 256 CUs to 84%), 8191 x 4096 -> 8192 f16 gelu_tanh 948 to 980 us (1122 to 1160
-// TFLOP/s), backward 2176 x 1536 -> 6144 199 us (27 the pass over dY, g and u; the rest both products and what is
-// left to add up), 1031 x 1001 -> 2731 f16 59.5 us. Plans: gated_plan, gated_pair.
+// stored 103 us (798 TFLOP/s; its 432 tiles fill 256 CUs to 84%), without 92, 8191 x 4096 -> 8192 f16 gelu_tanh 948 to 957 us (1150
+// TFLOP/s), backward 2176 x 1536 -> 6144 199 us (27 the pass over dY, g and u, 170 both products, 12 the split sums, each by
+// itself), 1031 x 1001 -> 2731 f16 59 us. Plans: gated_plan, gated_pair.
 #include "gated.h"
 #include "prod_dev.h"
 
