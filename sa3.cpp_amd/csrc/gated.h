@@ -22,10 +22,13 @@ inline int64_t gated_half(int64_t N) { return (N + 63) / 64 * 64; }
 
 // The blocks of 16 rows that the kernel for few rows takes (0: tiles). A second block pays while the weights are one round of
 // loads (K) on one round of workgroups (N). Measured on MI355X, 32 rows bf16, us (tiles / few): 1024 -> 4096 12.8 / 7.5, 512 -> 1024
-// 9.7 / 6.8, 768 -> 8192 12.2 / 9.7, 1023 -> 8192 28.5 / 28.0, 128 -> 512 7.2 / 7.1; past that 1536 -> 6144 15.1 / 16.0, 256 -> 20000
-// 10.7 / 18.0, 8192 -> 1024 17.5 / 30.3.
-inline int few_blocks(int64_t M, int64_t N, int64_t K) {
-    return M <= kFewRows ? 1 : M <= 2 * kFewRows && K <= 1024 && N <= 8192 ? 2 : 0;
+// 9.7 / 6.8, 768 -> 8192 12.2 / 9.7, 128 -> 512 7.2 / 7.1; past that 1536 -> 6144 15.1 / 16.0, 256 -> 20000 10.7 / 18.0, 8192 -> 1024
+// 17.5 / 30.3. Operands off the tiles' 16-byte grid, which those copy first (padded), run here unless few workgroups have long rows to
+// read: 4100 -> 11008 123 / 47, 1535 -> 6144 31.5 / 20.6, 4095 -> 11008 131 / 64, 255 -> 20000 24.6 / 22.5, 4095 -> 256 18.5 / 20.9,
+// 8191 -> 1024 32 / 47.
+inline int few_blocks(int64_t M, int64_t N, int64_t K, bool padded) {
+    if (M <= kFewRows) return 1;
+    return M <= 2 * kFewRows && (padded ? N >= 2048 || K <= 2048 : K <= 1024 && N <= 8192) ? 2 : 0;
 }
 
 // tiles of an M x N result that an XCD takes of a launch, and how many its 32 CUs hold at a time

@@ -15,10 +15,24 @@
 
 namespace {
 
+// Sixteen bytes of 16-bit elements wherever they begin, from whole dwords. A load off the dwords takes the memory pipe several times
+// as long: 1 x 1535 -> 6144 21.8 us with such loads, 1 x 1534 9.3. (The dwords read each hold one of the eight elements.)
+template <class T>
+__device__ __forceinline__ u32x4a load16_any(const T* p) {
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint32_t odd = (uint32_t)at & 2u;
+    const SA3K_GLOBAL uint32_t* q = (const SA3K_GLOBAL uint32_t*)(at & ~(uint64_t)3);
+    const u32x4at4 w = *(const SA3K_GLOBAL u32x4at4*)q;
+    const uint32_t last = q[3 + (odd >> 1)], shift = odd * 8;
+    return u32x4a{__builtin_amdgcn_alignbit(w[1], w[0], shift), __builtin_amdgcn_alignbit(w[2], w[1], shift),
+                  __builtin_amdgcn_alignbit(w[3], w[2], shift), __builtin_amdgcn_alignbit(last, w[3], shift)};
+}
+inline bool off_dwords(const void* p, int64_t ld) { return p && (reinterpret_cast<uintptr_t>(p) % 4 != 0 || ld % 2 != 0); }
+
 // Few rows, RB blocks of 16: 16 columns of the output a workgroup, whose eight waves split K in steps of 32 and read both weights
 // straight from memory into the MFMA's registers (each element once); the waves' sums are joined in LDS. Bound by HBM and the
-// latency of a launch: 1 x 1536 -> 6144 bf16 9.0 us, 38 MB (4.2 TB/s).
-template <class T, int RB>
+// latency of a launch: 1 x 1536 -> 6144 bf16 9.0 us, 38 MB (4.2 TB/s), 1 x 1535 12.5, 16 x 4095 -> 6144 31 (its loads as they lie: 76).
+template <class T, int RB, bool ODD>   // ODD: rows may begin off a dword
 __global__ __launch_bounds__(512) void gated_few_kernel(GemmArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int W = 8, U = RB == 1 ? 6 : 4;
@@ -39,8 +53,12 @@ __global__ __launch_bounds__(512) void gated_few_kernel(GemmArgs a) {
     auto ld = [&](const T* p, int64_t k) {
         x8 v;
         if (k + 8 <= a.K) {
-            const Pack<T, 8> q = *reinterpret_cast<const Pack<T, 8>*>(p + k);
-            v = __builtin_bit_cast(x8, q);
+            if constexpr (ODD) {
+                v = __builtin_bit_cast(x8, load16_any(p + k));
+            } else {
+                const Pack<T, 8> q = *reinterpret_cast<const Pack<T, 8>*>(p + k);
+                v = __builtin_bit_cast(x8, q);
+            }
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? p[k + e] : (T)0.f;
@@ -213,14 +231,16 @@ void fwd_run(sa3k_ctx* ctx, const GatedArgs& p) {
     a.A = p.X; a.lda = p.ldx; a.B = p.Wg; a.B2 = p.Wu; a.ldb = p.ldw;
     a.M = p.M; a.N = p.N; a.K = p.K;
     a.C = p.Y; a.ldc = p.ldy; a.act = p.act; a.bias = p.bg; a.bias2 = p.bu; a.Z = p.Go; a.Z2 = p.Uo; a.ldz = p.ldz;
-    if (const int blocks = few_blocks(p.M, p.N, p.K)) {
+    const bool padded = !loads16(p.X, p.ldx, p.K) || !loads16(p.Wg, p.ldw, p.K) || !loads16(p.Wu, p.ldw, p.K);
+    if (const int blocks = few_blocks(p.M, p.N, p.K, padded)) {
         KernelScope ks(ctx, "gated_linear_few", 4.0 * (double)a.M * (double)a.N * (double)a.K);
-        launch_k(ctx, true, blocks == 1 ? gated_few_kernel<T, 1> : gated_few_kernel<T, 2>, dim3((unsigned)ceil_div(a.N, 16)), dim3(512), 0,
-                 a);
+        const bool odd = off_dwords(p.X, p.ldx) || off_dwords(p.Wg, p.ldw) || off_dwords(p.Wu, p.ldw);
+        launch_k(ctx, true, blocks == 1 ? (odd ? gated_few_kernel<T, 1, true> : gated_few_kernel<T, 1, false>)
+                                        : (odd ? gated_few_kernel<T, 2, true> : gated_few_kernel<T, 2, false>),
+                 dim3((unsigned)ceil_div(a.N, 16)), dim3(512), 0, a);
         SA3K_LAUNCHED();
         return;
     }
-    const bool padded = !loads16(p.X, p.ldx, p.K) || !loads16(p.Wg, p.ldw, p.K) || !loads16(p.Wu, p.ldw, p.K);
     const int64_t Kp = padded ? up8(p.K) : p.K;
     const ProdPlan plan = gated_plan(p.M, p.N, Kp);
     Scratch s;

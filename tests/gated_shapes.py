@@ -4,7 +4,8 @@
 FORWARD = {
     (417, 8435, 316): (256, False), (33, 82, 302): (128, False), (35, 80, 516): (128, True), (156, 8820, 3596): (256, True),
     (513, 6632, 325): (256, False), (155, 8511, 4009): (256, True), (396, 9688, 16): (256, False), (300, 520, 1000): (128, True), (17, 82, 302): (2, False), (19, 80, 516): (2, False),
-    (32, 8192, 40): (2, False), (31, 8193, 40): (128, False), (32, 40, 1024): (2, False), (17, 40, 1025): (128, True),
+    (32, 8192, 40): (2, False), (31, 8193, 40): (128, False), (32, 40, 1024): (2, False), (17, 40, 1032): (128, True),
+    (17, 40, 1025): (2, False), (21, 40, 2049): (128, True), (32, 2048, 2049): (2, False), (29, 8200, 250): (2, False),
     (16, 33, 2000): (1, False),
 }
 # backward, both products: (dX and dW in one launch, edge of dX's tiles, whether its contraction is split, the same of dW)

@@ -24,7 +24,7 @@ void plans(int64_t M, int64_t N, int64_t K, int* out) {
     const int64_t h = 2 * gated_half(N), Kp = (K + 7) / 8 * 8;
     const ProdPlan f = gated_plan(M, N, Kp), x = prod_plan(M, K, h), w = prod_plan(h, K, M);
     const ProdPair p = gated_pair(M, N, K, x, w);
-    const int few = few_blocks(M, N, K);
+    const int few = few_blocks(M, N, K, K % 8 != 0);   // (tensors without gaps)
     out[0] = few ? few : f.edge; out[1] = few ? 1 : f.splits;
     out[2] = p.together; out[3] = p.a.edge; out[4] = p.a.splits; out[5] = p.b.edge; out[6] = p.b.splits;
     out[7] = x.edge; out[8] = x.splits; out[9] = w.edge; out[10] = w.splits;
