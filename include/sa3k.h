@@ -525,8 +525,8 @@ SA3K_API int sa3k_linear_act_bwd(sa3k_ctx* ctx, int type, int act, const void* d
  *   g = X Wg^T + bg,  u = X Wu^T + bu,  Y = act(g) u
  * X [M][K], Wg and Wu [N][K] (two tensors, or halves of one), Y, G and U [M][N]; biases f32 [N]; biases, G and U (g and u,
  * for the backward) nullable. Activation and product apply to the f32 g and u; every output is rounded once. Any M
- * (0: nothing), N below 2^21 - 63 and K below 2^22, row pitches below 2^22. Outputs overlap no other tensor. NaN and infinities go
- * through the formulas as they stand. */
+ * (0: nothing), N below 2^21 - 63 and K below 2^22, row pitches below 2^22. Outputs overlap no other tensor (refused
+ * where they do). NaN and infinities go through the formulas as they stand. */
 SA3K_API int sa3k_gated_linear_fwd(sa3k_ctx* ctx, int type, int act, const void* X, int64_t ldx, const void* Wg, const void* Wu,
                                    int64_t ldw, const float* bg, const float* bu, int64_t M, int64_t N, int64_t K, void* Y,
                                    int64_t ldy, void* G, void* U, int64_t ldz);
@@ -534,7 +534,7 @@ SA3K_API int sa3k_gated_linear_fwd(sa3k_ctx* ctx, int type, int act, const void*
 /* Its backward from dY and the stored g and u: dg = dY u act'(g), du = dY act(g),
  *   dX = dg Wg + du Wu,  dWg = dg^T X,  dWu = du^T X (both or neither),  dbg and dbu = column sums of dg and du
  * (each nullable). dg and du are rounded to `type` for the products, not for the biases' gradients. dw_type: `type`, or f32;
- * accumulate = 1 adds to dWg and dWu (f32 only), dbg and dbu. Outputs overlap no other tensor. act' as in sa3k_linear_act_bwd; in f16
+ * accumulate = 1 adds to dWg and dWu (f32 only), dbg and dbu. Outputs overlap no other tensor (refused where they do). act' as in sa3k_linear_act_bwd; in f16
  * a dg or du past 65504 is an infinity, as in any f16 backward without loss scaling. Sums run in a fixed order. */
 SA3K_API int sa3k_gated_linear_bwd(sa3k_ctx* ctx, int type, int act, const void* dY, int64_t lddy, const void* G, const void* U,
                                    int64_t ldz, const void* X, int64_t ldx, const void* Wg, const void* Wu, int64_t ldw, int64_t M,

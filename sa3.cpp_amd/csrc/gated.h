@@ -127,12 +127,32 @@ inline ProdPair gated_pair(int64_t M, int64_t N, int64_t K, const ProdPlan& x, c
     return best;
 }
 
-// whether an element of x and one of y lie in the same place: rows of both `ld` apart
-inline bool rows_meet(const void* x, const void* y, int64_t ld, int64_t rows, int64_t cols, int bytes) {
-    if (!x || !y || rows <= 0) return false;
-    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
-    const int64_t d = (int64_t)((a > b ? a - b : b - a) / (uintptr_t)bytes), q = d / ld, r = d % ld;
-    return (q < rows && r < cols) || (q + 1 < rows && ld - r < cols);
+// Rows in memory, in bytes. (A pitch is no shorter than its rows, but where there is one row.)
+struct Rows {
+    uintptr_t at;
+    int64_t ld, n, width;
+};
+inline Rows rows_of(const void* p, int64_t ld, int64_t n, int64_t cols, int bytes) {
+    return Rows{reinterpret_cast<uintptr_t>(p), ld * bytes, p && n > 0 ? n : 0, cols * bytes};
+}
+// whether a byte is of both: rows that take turns in one buffer have none
+inline bool rows_meet(const Rows& x, const Rows& y) {
+    if (x.n == 0 || y.n == 0) return false;
+    auto end = [](const Rows& r) { return r.at + (uintptr_t)((r.n - 1) * r.ld + r.width); };
+    if (end(x) <= y.at || end(y) <= x.at) return false;
+    if (x.n > 1 && y.n > 1 && x.ld == y.ld) {   // the higher one's rows begin r behind rows q, q + 1, .. of the lower one
+        const Rows &lo = x.at < y.at ? x : y, &hi = x.at < y.at ? y : x;
+        const int64_t d = (int64_t)(hi.at - lo.at), q = d / lo.ld, r = d % lo.ld;
+        return (q < lo.n && r < lo.width) || (q + 1 < lo.n && lo.ld - r < hi.width);
+    }
+    // Other pitches within one range of addresses: row by row of the one with fewer
+    const Rows &a = x.n <= y.n ? x : y, &b = x.n <= y.n ? y : x;
+    for (int64_t i = 0; i < a.n; ++i) {
+        const int64_t from = (int64_t)(a.at - b.at) + i * a.ld;   // from b's first row on
+        const int64_t j = from < b.width ? 0 : (from - b.width) / b.ld + 1;   // the first of b's rows that ends behind it
+        if (j < b.n && j * b.ld < from + a.width) return true;
+    }
+    return false;
 }
 
 inline const char* gated_check(const GatedArgs& a, bool bwd, int* code) {
@@ -165,8 +185,10 @@ inline const char* gated_check(const GatedArgs& a, bool bwd, int* code) {
         *code = SA3K_ERR_UNSUPPORTED;
         return "M x N is too large for one launch";
     }
-    if (rows_meet(a.Go, a.Uo, a.ldz, a.M, a.N, 2) || rows_meet(a.dWg, a.dWu, a.lddw, a.N, a.K, elem_bytes(a.dw_type)) ||
-        rows_meet(a.dbg, a.dbu, a.N, 1, a.N, 4))
+    const int wb = elem_bytes(a.dw_type);
+    if (rows_meet(rows_of(a.Go, a.ldz, a.M, a.N, 2), rows_of(a.Uo, a.ldz, a.M, a.N, 2)) ||
+        rows_meet(rows_of(a.dWg, a.lddw, a.N, a.K, wb), rows_of(a.dWu, a.lddw, a.N, a.K, wb)) ||
+        rows_meet(rows_of(a.dbg, a.N, 1, a.N, 4), rows_of(a.dbu, a.N, 1, a.N, 4)))
         return "gate's output meets up's";
     if (!bwd) {
         if (!a.Wg || !a.Wu) return "the weights must not be null";
@@ -175,6 +197,26 @@ inline const char* gated_check(const GatedArgs& a, bool bwd, int* code) {
         if (a.M > 0 && (!a.dY || !a.G || !a.U)) return "dY, G and U must not be null";
         if (a.M > 0 && a.dWg && !a.X) return "dW needs X";
         if (a.dX && (!a.Wg || !a.Wu)) return "dX needs the weights";
+    }
+    return nullptr;
+}
+
+// What gated_check found in order, taken two by two: an output that meets another output would be written over (Y over the kept g
+// leaves a wrong g behind), one that meets an input is written while other workgroups still read that.
+inline const char* gated_apart(const GatedArgs& a, bool bwd) {
+    const int wb = bwd ? elem_bytes(a.dw_type) : 2;
+    auto vec = [&](const void* p) { return rows_of(p, a.N, 1, a.N, 4); };
+    const Rows out[8] = {rows_of(a.Y, a.ldy, a.M, a.N, 2), rows_of(a.Go, a.ldz, a.M, a.N, 2), rows_of(a.Uo, a.ldz, a.M, a.N, 2),
+                         rows_of(a.dX, a.lddx, a.M, a.K, 2), rows_of(a.dWg, a.lddw, a.N, a.K, wb),
+                         rows_of(a.dWu, a.lddw, a.N, a.K, wb), vec(a.dbg), vec(a.dbu)};
+    const Rows in[8] = {rows_of(a.X, a.ldx, a.M, a.K, 2), rows_of(a.Wg, a.ldw, a.N, a.K, 2), rows_of(a.Wu, a.ldw, a.N, a.K, 2),
+                        rows_of(a.dY, a.lddy, a.M, a.N, 2), rows_of(a.G, a.ldz, a.M, a.N, 2), rows_of(a.U, a.ldz, a.M, a.N, 2),
+                        vec(a.bg), vec(a.bu)};
+    for (int i = 0; i < 8; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (rows_meet(out[i], out[j])) return "an output meets another";
+        for (const Rows& r : in)
+            if (rows_meet(out[i], r)) return "an output meets an input";
     }
     return nullptr;
 }

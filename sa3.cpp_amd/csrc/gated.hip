@@ -355,7 +355,7 @@ SA3K_API int sa3k_gated_linear_fwd(sa3k_ctx* ctx, int type, int act, const void*
         p.Y = Y; p.ldy = ldy; p.Go = G; p.Uo = U; p.ldz = ldz;
         int code;
         const char* msg = gated_check(p, false, &code);
-        require_ok(msg, code);
+        require_ok(msg ? msg : gated_apart(p, false), code);
         if (M == 0) return;
         DeviceScope dev(ctx);
         if (type == SA3K_TYPE_BF16) fwd_run<bf16>(ctx, p);
@@ -375,7 +375,7 @@ SA3K_API int sa3k_gated_linear_bwd(sa3k_ctx* ctx, int type, int act, const void*
         p.accumulate = accumulate;
         int code;
         const char* msg = gated_check(p, true, &code);
-        require_ok(msg, code);
+        require_ok(msg ? msg : gated_apart(p, true), code);
         DeviceScope dev(ctx);
         if (type == SA3K_TYPE_BF16) bwd_run<bf16>(ctx, p);
         else bwd_run<f16>(ctx, p);
