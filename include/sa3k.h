@@ -565,7 +565,7 @@ typedef struct {
  * [batch][tokens] (nullable): the row of k_out and v_out that a token's k and v go to, else row t; a slot outside 0 .. cache_tokens - 1 is not stored, and the
  * slots of a sample that are must differ. len device int32 [batch] (nullable): tokens past a sample's length are not read, and
  * their outputs stay as they were. q_out may be q with the same strides; k_out and v_out likewise without slots; outputs overlap
- * nothing else. Sums and angles f32 (a head whose squares pass 3e38 gives 0), outputs rounded once. Tensors need only be aligned to
+ * nothing else (refused where one begins at another tensor's address). Sums and angles f32 (a head whose squares pass 3e38 gives 0), outputs rounded once. Tensors need only be aligned to
  * their elements. */
 SA3K_API int sa3k_head_norm_fwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const void* q, const void* k, const void* v,
                                 const float* q_gain, const float* k_gain, const int32_t* pos, const int32_t* slot,
@@ -574,7 +574,8 @@ SA3K_API int sa3k_head_norm_fwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const vo
 /* Its backward from the outputs' gradients, which lie as q_out and k_out do (row t; there are no slots): with w the gradient
  * turned back and h = w gain, r = 1 / sqrt(mean x^2 + eps),
  *   dx = r (h - x r mean(h x r)),  dgain = sum over tokens and heads of w x r
- * dq and dk lie as q and k do and may be dq_out and dk_out themselves (same strides). q and k (with their gradients) and the gains'
+ * dq and dk lie as q and k do and may be dq_out and dk_out themselves (same strides); they overlap no tensor of the
+ * other's. q and k (with their gradients) and the gains'
  * gradients (f32 [head_dim], two vectors) are each nullable; accumulate = 1 adds to the latter. Tokens past a sample's length are not read, add nothing,
  * and their gradients stay as they were. Sums run in a fixed order. */
 SA3K_API int sa3k_head_norm_bwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const void* q, const void* k, const void* dq_out,

@@ -109,6 +109,23 @@ inline const char* head_norm_check(const sa3k_head_norm* d, const HeadPtrs& p, b
     return nullptr;
 }
 
+// What head_norm_check found in order: whether an output begins where another tensor does that it may not be (its own input, forward, and
+// its own head's gradient or input, backward, it may). Such calls would read what other workgroups write. (The gains' gradients are written
+// when all is read. Tensors that share elements, but not their first, are the caller's to keep apart.)
+inline const char* head_norm_apart(const sa3k_head_norm& d, const HeadPtrs& p, bool bwd) {
+    if (d.batch == 0 || d.tokens == 0) return nullptr;
+    const void* const out[5] = {p.qo, p.ko, p.vo, p.dq_gain, p.dk_gain};
+    const void* const in[10] = {p.q, p.k, p.v, p.dqo, p.dko, p.q_gain, p.k_gain, p.pos, p.slot, p.len};
+    for (int i = 0; i < 5; ++i) {
+        if (!out[i]) continue;
+        for (int j = 0; j < i; ++j)
+            if (out[i] == out[j]) return "two outputs are the same tensor";
+        for (int j = 0; i < 3 && j < 10; ++j)
+            if (out[i] == in[j] && j != i && !(bwd && j == i + 3)) return "an output is another head's tensor, or a vector's";
+    }
+    return nullptr;
+}
+
 // Pair i turns by pos base^(-2i / dims) radians. A position is a whole number, so only the fraction of a turn that one
 // position makes matters: as 64 bits behind the point, pos times it is exact modulo a turn, and off by at most
 // |pos| 2^-65 turns of the real number (2^-34 at the furthest position) whatever the position. Powers by repeated

@@ -439,7 +439,7 @@ SA3K_API int sa3k_head_norm_fwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const vo
         p.qo = q_out; p.ko = k_out; p.vo = v_out;
         int code;
         const char* msg = head_norm_check(d, p, false, &code);
-        require_ok(msg, code);
+        require_ok(msg ? msg : head_norm_apart(*d, p, false), code);
         head_dispatch(ctx, *d, p, false);
     });
 }
@@ -453,7 +453,7 @@ SA3K_API int sa3k_head_norm_bwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const vo
         p.qo = dq; p.ko = dk; p.dq_gain = dq_gain; p.dk_gain = dk_gain; p.accumulate = accumulate;
         int code;
         const char* msg = head_norm_check(d, p, true, &code);
-        require_ok(msg, code);
+        require_ok(msg ? msg : head_norm_apart(*d, p, true), code);
         head_dispatch(ctx, *d, p, true);
     });
 }
