@@ -560,8 +560,8 @@ typedef struct {
 /* For each head x of q and of k, of token t of sample b:
  *   n = x / sqrt(mean x^2 + eps) * gain,  y = n with pair i of its first rope_dims elements turned by
  *   pos rope_base^(-2i / rope_dims) radians: (a, c) -> (a cos - c sin, c cos + a sin)
- * q_gain and k_gain f32 [head_dim] (null: ones). pos device int32 [batch][tokens] (null: t; any value, the angles are exact
- * modulo a turn to 2^-33 turns). q, k and v with their outputs are each nullable; v is copied. slot device int32
+ * q_gain and k_gain f32 [head_dim] (null: ones). pos device int32 [batch][tokens] (null: t; any value: an angle modulo a
+ * turn is off by less than 2^-30 turns). q, k and v with their outputs are each nullable; v is copied. slot device int32
  * [batch][tokens] (nullable): the row of k_out and v_out that a token's k and v go to, else row t; a slot outside 0 .. cache_tokens - 1 is not stored, and the
  * slots of a sample that are must differ. len device int32 [batch] (nullable): tokens past a sample's length are not read, and
  * their outputs stay as they were. q_out may be q with the same strides; k_out and v_out likewise without slots; outputs overlap

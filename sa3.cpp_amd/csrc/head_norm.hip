@@ -7,8 +7,8 @@
 //
 // Eight elements of a head a lane, 4 to 32 lanes a head, several heads a wave. A wave takes up to three such groups of heads of one row
 // (token) and one tensor, so that nothing but the lane's own head is chosen inside it; the row's sines and cosines, which the heads share,
-// are worked out a pair a lane while the loads are under way. Angles are exact modulo a turn (head_turns), so a position a million tokens
-// out is as good as the first.
+// are worked out a pair a lane while the loads are under way. Angles are taken modulo a turn in whole numbers (head_turns), so a position a
+// million tokens out is as good as the first.
 //
 // Forward bound by HBM, or by a launch. Measured on MI355X: 8192 x (32 + 8) heads of 128 f16 33.0 us with its inputs in the memory-side
 // cache (5.1 TB/s), 38 a call without; 2 x 1088 x (24 + 24) heads of 64 bf16 8.4 (3.2 TB/s, one round of loads); 8 new tokens 5.2. Backward
@@ -90,7 +90,7 @@ __device__ __forceinline__ void row_turns(const HeadArgs& a, const Row& r, int c
     if (a.rope == 0) return;   // (uniform)
     const int pairs = a.rope >> 1;
     const int64_t pos = a.pos ? a.pos[r.row] : (int64_t)r.t;
-    for (int p = lane; p < pairs; p += 64) tab[p] = cos_sin((uint32_t)(((uint64_t)pos * a.turn[p]) >> 32));
+    for (int p = lane; p < pairs; p += 64) tab[p] = cos_sin((uint32_t)(((uint64_t)pos * a.turn[p] + 0x80000000u) >> 32));
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
