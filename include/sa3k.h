@@ -565,7 +565,8 @@ typedef struct {
  * [batch][tokens] (nullable): the row of k_out and v_out that a token's k and v go to, else row t; a slot outside 0 .. cache_tokens - 1 is not stored, and the
  * slots of a sample that are must differ. len device int32 [batch] (nullable): tokens past a sample's length are not read, and
  * their outputs stay as they were. q_out may be q with the same strides; k_out and v_out likewise without slots; outputs overlap
- * nothing else (refused where one begins at another tensor's address). Sums and angles f32 (a head whose squares pass 3e38 gives 0), outputs rounded once. Tensors need only be aligned to
+ * nothing else (refused where one begins at another tensor's address). Sums and angles f32 (a head whose squares pass 3e38 gives 0; one whose squares
+ * are all below 2^-150 is one of zeros), outputs rounded once. Tensors need only be aligned to
  * their elements. */
 SA3K_API int sa3k_head_norm_fwd(sa3k_ctx* ctx, const sa3k_head_norm* d, const void* q, const void* k, const void* v,
                                 const float* q_gain, const float* k_gain, const int32_t* pos, const int32_t* slot,

@@ -64,8 +64,13 @@ __device__ __forceinline__ float2 cos_sin(uint32_t t) {
 
 template <class T>
 __device__ __forceinline__ float inverse_root(float v) {
-    if constexpr (sizeof(T) == 4) return 1.f / sqrtf(v);
-    else return __builtin_amdgcn_rsqf(v);   // off by 2^-23, against the 2^-9 or 2^-12 of the output's rounding
+    if constexpr (sizeof(T) == 4) {
+        return 1.f / sqrtf(v);
+    } else {   // off by 2^-23, against the 2^-9 or 2^-12 of the output's rounding; the instruction takes what is below 2^-126 as 0
+        const bool small = v < 0x1p-126f;
+        const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p64f : v);
+        return small ? r * 0x1p32f : r;
+    }
 }
 
 // The row (a token of a sample) of a wave
