@@ -20,15 +20,22 @@ struct GatedArgs {
 // gate's and up's gradients lie side by side, each padded to whole tiles of 64
 inline int64_t gated_half(int64_t N) { return (N + 63) / 64 * 64; }
 
-// The blocks of 16 rows that the kernel for few rows takes (0: tiles). A second block pays while the weights are one round of
-// loads (K) on one round of workgroups (N). Measured on MI355X, 32 rows bf16, us (tiles / few): 1024 -> 4096 12.8 / 7.5, 512 -> 1024
-// 9.7 / 6.8, 768 -> 8192 12.2 / 9.7, 128 -> 512 7.2 / 7.1; past that 1536 -> 6144 15.1 / 16.0, 256 -> 20000 10.7 / 18.0, 8192 -> 1024
-// 17.5 / 30.3. Operands off the tiles' 16-byte grid, which those copy first (padded), run here unless few workgroups have long rows to
-// read: 4100 -> 11008 123 / 47, 1535 -> 6144 31.5 / 20.6, 4095 -> 11008 131 / 64, 255 -> 20000 24.6 / 22.5, 4095 -> 256 18.5 / 20.9,
-// 8191 -> 1024 32 / 47.
+// The blocks of 16 rows that the kernel for few rows takes (0: tiles). A workgroup of it reads 16 columns' weights whole, so long rows (K)
+// on fewer workgroups (N / 16) than CUs wait for memory where the tiles split K, and x, read again for every 16 columns, takes
+// over with more than 8 rows of large weights. Measured on MI355X, bf16, us (few / tiles), 1 and 16 rows: 1536 -> 6144 10.0 / 15.1 and 11.7 /
+// 15.5, 4608 -> 2048 13.5 / 16.2 and 16.8 / 16.4, 4608 -> 64 11.1 / 12.9 and 14.2 / 12.8, 5120 -> 2048 18.7 / 17.1 and 22.7 / 17.3, 8192 ->
+// 1024 23.5 / 16.9 and 30.1 / 18.1, 16384 -> 1024 41.7 / 23.4 and 55.1 / 24.6, 8192 -> 4096 32.4 / 39.5 and 36.5 / 40.1, 3584 -> 16384
+// 47.0 / 44.4 and 56.3 / 44.2, 5120 -> 16384 70.1 / 59.8 and 86.5 / 60.3, 8192 -> 8192 54.4 / 67.7 and 63.2 / 67.5.
+// A second block pays while the weights are one round of loads (K) on one round of workgroups (N): 32 rows 1024 -> 4096 7.5 / 12.8, 512 ->
+// 1024 6.8 / 9.7, 768 -> 8192 9.7 / 12.2, 128 -> 512 7.1 / 7.2; past that 1536 -> 6144 16.0 / 15.1, 256 -> 20000 18.0 / 10.7, 8192 -> 1024
+// 30.3 / 17.5. Operands off the tiles' 16-byte grid, which those copy first (padded), run here unless few workgroups have long rows to
+// read: 1 row 2559 -> 333 15.0 / 16.5, 4095 -> 1001 28.7 / 25.2, 8191 -> 1001 53.4 / 35.9, 8191 -> 4099 56.9 / 92.5, 16 rows 4099 -> 16000 72 /
+// 163, 32 rows 4100 -> 11008 47 / 123, 1535 -> 6144 20.6 / 31.5, 255 -> 20000 22.5 / 24.6, 4095 -> 256 20.9 / 18.5, 8191 -> 1024 47 / 32.
 inline int few_blocks(int64_t M, int64_t N, int64_t K, bool padded) {
-    if (M <= kFewRows) return 1;
-    return M <= 2 * kFewRows && (padded ? N >= 2048 || K <= 2048 : K <= 1024 && N <= 8192) ? 2 : 0;
+    if (M > 2 * kFewRows) return 0;
+    if (M > kFewRows) return (padded ? N >= 2048 || K <= 2048 : K <= 1024 && N <= 8192) ? 2 : 0;
+    if (padded) return N >= 2048 || K <= 2560 ? 1 : 0;
+    return (N >= 4096 || K <= 4608) && (M <= 8 || N * K <= 40000000) ? 1 : 0;
 }
 
 // tiles of an M x N result that an XCD takes of a launch, and how many its 32 CUs hold at a time

@@ -149,3 +149,10 @@ def test_activations_at_every_end(ctx, M, N, K, act):
         if kept:
             assert torch.equal(down(out[1], kind), g + 0)
             assert torch.equal(down(out[2], kind), c.to(TORCH[kind]).expand(M, N))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 4616), (5, 333, 6001), (9, 8200, 5120), (16, 1024, 8192), (16, 88, 14344)])
+def test_few_rows_on_tiles(ctx, M, N, K):
+    """up to 16 rows of weights that the kernel for few rows would read slowly (gated.h: few_blocks)"""
+    test_forward_among_nan(ctx, M, N, K, "aligned")
+    test_forward_among_nan(ctx, M, N, K, "even")
