@@ -21,7 +21,8 @@ class InNan:
 
     def __init__(self, ctx, t, gap, before=8):
         self.rows, self.cols = t.shape
-        self.kind, self.ld, self.off = {v: k for k, v in TORCH.items()}[t.dtype], self.cols + gap, before
+        ld = self.cols + gap if gap else -(-self.cols // 8) * 8 + 8
+        self.kind, self.ld, self.off = {v: k for k, v in TORCH.items()}[t.dtype], ld, before
         host = torch.full((before + self.rows * self.ld + 16,), NAN, dtype=t.dtype)
         host.as_strided(t.shape, (self.ld, 1), before).copy_(t)
         self.buf = up(ctx, host)
@@ -49,7 +50,8 @@ FORWARDS = [(1, 33, 40), (16, 100, 256), (5, 17, 7), (32, 304, 520), (17, 40, 10
             (396, 9688, 16), (417, 8435, 316), (155, 8511, 4009)]
 BACKWARDS = [(1, 33, 40), (65, 768, 1032), (16, 195, 16), (158, 278, 130), (644, 18, 16), (131, 3914, 8405), (2321, 2250, 1695), (131, 8117, 149)]
 assert {s for s in FORWARDS if s in FORWARD} and {s for s in BACKWARDS if s in BACKWARD}
-LAYOUTS = {"aligned": (8, 8), "odd": (3, 1), "even": (2, 2)}   # gap between rows, elements before the first
+# gap between rows (0: up to the next multiple of 8 and 8 more), elements before the first
+LAYOUTS = {"aligned": (8, 8), "odd": (3, 1), "even": (2, 2), "eights": (0, 8)}
 
 
 def product(a, b):
