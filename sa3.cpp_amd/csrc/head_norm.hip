@@ -11,9 +11,11 @@
 // million tokens out is as good as the first.
 //
 // Forward bound by HBM, or by a launch. Measured on MI355X: 8192 x (32 + 8) heads of 128 f16 33.0 us with its inputs in the memory-side
-// cache (5.1 TB/s), 38 a call without; 2 x 1088 x (24 + 24) heads of 64 bf16 8.4 (3.2 TB/s, one round of loads); 8 new tokens 5.2. Backward
-// 3 x 2049 x (16 + 2) heads of 128 f32 27.6 (5.1 TB/s) and 4.9 for the second launch; 2 x 1088 x (24 + 24) bf16 12.6 and 3.8, bound by its
-// vector instructions. (A wave over all of a row's heads, choosing the tensor for each group: 12.7 and 28.8 us in place of 8.4 and 12.6.)
+// cache (5.1 TB/s), 38 a call without, f32 70 a call (4.8 TB/s); 2 x 1088 x (24 + 24) heads of 64 bf16 8.4 (3.2 TB/s, one round of loads); 8
+// new tokens 5.2. Backward 3 x 2049 x (16 + 2) heads of 128 f32 27.5 (5.1 TB/s) and 4.9 for the second launch; 2 x 1088 x (24 + 24) bf16
+// 12.8 and 3.9, bound by latency: two waves a SIMD, two rows each one after the other, that wait for 56% of their time; vector instructions
+// take a third of the SIMDs' cycles. (A wave over all of a row's heads, choosing the tensor for each group: 12.7 and 28.8 us in place of 8.4
+// and 12.6.)
 #include <algorithm>
 
 #include "head_norm.h"

@@ -468,9 +468,10 @@ struct FinishGated {
 // The end of a wave of a gated forward's 256 x 256 tile, 64 rows x 64 columns of both products, without LDS and without waiting for other
 // waves: the products were made with the weights' fragments first, so a lane holds 16 sums of one row of a block of 32 x 32 (column
 // 8 (v / 4) + 4 (lane / 32) + v % 4), gate's and up's of the same element. Lanes 32 apart swap their fours for eights (16 bits), lanes 16
-// apart halves of their rows, so that a store takes 64 bytes of 16 rows. Measured on MI355X (us, staged through LDS as the other
-// products' / so): 2176 x 1536 -> 6144 bf16 92 / 82, with g and u stored 94 / 89, 8191 x 4096 -> 8192 f16 957 / 922; rows that begin off 16
-// bytes stay staged (1952 x 320 -> 2239 25 / 35). The backward's products gained nothing (2176 x 1536 -> 6144 both 197).
+// apart halves of their rows, so that a store takes 64 bytes of 16 rows. Measured on MI355X, us a call, in turn on one card (staged
+// through LDS as the other products' / so): 2176 x 1536 -> 6144 bf16 106 / 96, with biases, g and u stored 112 / 106, 8192 x 1536 -> 6144 with
+// them 340 / 320, 8191 x 4096 -> 8192 f16 1004 / 963. Rows that begin off 16 bytes stay staged: with g and u stored 1952 x 320 -> 2239 27 /
+// 35, 2176 x 1536 -> 6145 115 / 132, 4096 x 2048 -> 4100 189 / 194 (of Y alone 21.3 / 19.4, 103 / 99 and 180 / 163: not told apart). The backward's products gained nothing (2176 x 1536 -> 6144 both 197).
 template <int A, int B>
 __device__ __forceinline__ void swap_lanes(uint32_t (&w)[16], int n, int by) {
 #pragma unroll
